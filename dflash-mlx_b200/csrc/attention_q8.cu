@@ -1,0 +1,744 @@
+// Grouped-query attention over the 8-bit K/V cache (dfl_kv_q8).
+//
+//   x_j = scale * ks_j * (q . Kc_j)            Kc, Vc codes; ks, vs their scales; j < lim(row)
+//   o   = sum_j e_j vs_j Vc_j / sum_j e_j      e_j = exp(x_j - max x)
+//
+// Work split: one CTA per (run tile, kv head, key chunk). A run is the rows of one sequence; its
+// tile's rows are (token, query head of the group) pairs packed without gaps, so a single token
+// with G heads fills G rows of one 16-row MMA tile and a 16-token verify block with G = 4 the 64
+// rows of a full CTA: K and V are read once for all of them. The four warps of a row group are
+// four strands: strand s takes the 32-key blocks s, s + 4, ... of the chunk with its own running
+// maximum and sum, and the strands are merged in order at the end. Chunks are merged in order by
+// a second kernel (one chunk: written directly). A row's arithmetic depends on the chunk size and
+// on its own query and keys alone, whatever the tile's other rows, row groups or masks are: the
+// rows of a verify block and of single-token decode agree bit for bit.
+//
+// Codes go to fp16 exactly (int8 by placing the biased byte into 1024 + u and subtracting 1152;
+// e4m3 by the conversion instruction) and the products run on mma.sync m16n8k16 with fp32
+// accumulators. Both products contract over permuted dims / keys so that no byte is moved to be
+// transposed: a K register of four codes holds four consecutive dims, so Q is stored in that
+// order, and a V register read by ldmatrix.trans holds two keys of two adjacent dims, so even and
+// odd dims go to two accumulator tiles.
+//  * q is scaled by a power of two per row to [2^14, 2^15) at its largest element: every bf16 value
+//    down to 2^-29 of it stays exact in fp16.
+//  * The V scale goes into the weight, w_j = e_j vs_j, which is rounded to fp16 (2^-12 relative).
+//    e_j is taken relative to M = max x - 14 + log2 of the largest V scale the row has seen, so
+//    w_j < 2^15 whatever the scales are, and weights down to 2^-29 of the largest keep all their
+//    bits; the sum of e_j uses the same M, which cancels in the quotient.
+// Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales,
+// codes or query products may be anything), so infinities and NaN there do not reach the row.
+#include "kv_q8.cuh"
+
+#include <type_traits>
+
+namespace dfl {
+
+constexpr int Q8_KB = 32;       // keys per block
+constexpr int Q8_STRANDS = 4;   // blocks in flight per chunk, each a warp of every row group
+constexpr int Q8_CHUNK_UNIT = Q8_KB * Q8_STRANDS;
+
+struct AttnQ8Args {
+  const __nv_bfloat16* q;  // [M][Hq][hd]
+  Q8Cache c;
+  const int* pos;
+  const int* row_seq;
+  const int* kv_len;
+  float* part_o;    // [chunks][M][Hq][hd]
+  float2* part_ml;  // [chunks][M][Hq]: (M, sum)
+  __nv_bfloat16* out;
+  long long ldo;
+  const __nv_bfloat16* gate;
+  long long ldg;
+  int gate_hs;
+  int M, Hq, G, causal, max_kv, n_chunks, key_chunk;
+  int run_rows;   // rows per run
+  int tile_toks;  // tokens per tile
+  int run_tiles;  // tiles per run
+  float scale_log2;  // |softmax scale| * log2(e); 1 when the scale is 0
+  float q_sign;      // sign of the softmax scale (0 when it is 0): folded into q
+  int* err;
+};
+
+// ---- fp16 fragments ------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Four codes b0..b3 to two half2: (b0, b1), (b2, b3) with PAIRED (K: consecutive dims) or
+// (b0, b2), (b1, b3) without (V: the same dim of two keys).
+template <bool E4M3, bool PAIRED>
+__device__ __forceinline__ void q8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (E4M3) {
+    if (!PAIRED) w = __byte_perm(w, 0, 0x3120);
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
+    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
+  } else {
+    // fp16 0x6400 | u is 1024 + u; the biased byte u = c + 128
+    w ^= 0x80808080u;
+    lo = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4140 : 0x4240), 0x64806480u);
+    hi = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4342 : 0x4341), 0x64806480u);
+  }
+}
+
+// byte offset of 16-byte chunk c of key row r in a stage's [32][HD]-byte tile: ldmatrix reads the
+// same chunk of eight consecutive rows, which then lie in eight different 16-byte bank groups
+template <int HD>
+__device__ __forceinline__ int q8_swz(int r, int c) {
+  return r * HD + ((HD == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4);
+}
+
+// keys row m sees: clamped to what the cache and the call allow (an excess sets the error word)
+__device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, int seq, int* err) {
+  const long long lim = a.causal ? (long long)p + 1 : a.kv_len[seq];
+  const int most = min(a.max_kv, a.c.cap);
+  if (lim > most) q8_error(err, Q8_ERR_POS);
+  return lim > most ? most : lim < 0 ? 0 : (int)lim;
+}
+
+template <int HD, int MT, int RG, int ST>
+struct AttnQ8Layout {
+  static constexpr int ROWS = 16 * MT * RG;
+  static constexpr int STAGE = 2 * Q8_KB * HD + 2 * Q8_KB * 4;
+  static constexpr int RING = Q8_STRANDS * ST * STAGE;
+  static constexpr int MERGE = Q8_STRANDS * ROWS * HD * 4 + Q8_STRANDS * ROWS * 8;
+  static constexpr int BASE = RING > MERGE ? RING : MERGE;  // the merge reuses the ring
+  static constexpr int OFF_Q = BASE;
+  static constexpr int OFF_F = OFF_Q + ROWS * HD * 2;  // row factors, row limits
+  static constexpr int SMEM = OFF_F + ROWS * 8;
+};
+
+template <int HD, int MT, int RG, int ST, bool E4M3>
+__global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __grid_constant__ AttnQ8Args a) {
+  using L = AttnQ8Layout<HD, MT, RG, ST>;
+  constexpr int NC = HD / 16;
+  constexpr int NWARPS = Q8_STRANDS * RG;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __half* sQ = reinterpret_cast<__half*>(smem + L::OFF_Q);
+  float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_F);
+  int* s_lim = reinterpret_cast<int*>(smem + L::OFF_F) + L::ROWS;
+  __shared__ int s_tok_lim[L::ROWS], s_tok_ok[L::ROWS];
+
+  grid_dependency_launch_dependents();
+  grid_dependency_wait();
+
+  const int run = blockIdx.x / a.run_tiles, tile = blockIdx.x % a.run_tiles, kvh = blockIdx.y, chunk = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int strand = warp % Q8_STRANDS, rg = warp / Q8_STRANDS;
+  const int g = lane >> 2, t = lane & 3;
+  const int m0 = run * a.run_rows + tile * a.tile_toks;
+  const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
+  if (ntok <= 0) return;
+
+  // the run's sequence: that of the tile's first row with a position
+  int seq = -1;
+  for (int i = 0; i < ntok && seq < 0; ++i)
+    if (a.pos[m0 + i] >= 0) seq = a.row_seq ? a.row_seq[m0 + i] : 0;
+  if (seq < 0 || seq >= a.c.n_seqs) {  // nothing to do, or no such sequence
+    if (seq >= 0 && threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
+    return;
+  }
+  if (threadIdx.x < ntok) {
+    const int m = m0 + threadIdx.x, p = a.pos[m];
+    int lim = 0, ok = p >= 0;
+    if (ok && a.row_seq && a.row_seq[m] != seq) {
+      q8_error(a.err, Q8_ERR_SEQ);
+      ok = 0;
+    }
+    if (ok) lim = q8_row_limit(a, m, p, seq, chunk == 0 && kvh == 0 ? a.err : nullptr);
+    s_tok_lim[threadIdx.x] = lim;
+    s_tok_ok[threadIdx.x] = ok;
+  }
+  __syncthreads();
+  int lim_max = 0, lim_min = 0x7fffffff;
+  for (int i = 0; i < ntok; ++i) {
+    const int lim = s_tok_lim[i];
+    lim_max = max(lim_max, lim);
+    if (lim > 0) lim_min = min(lim_min, lim);
+  }
+  const int k_begin = chunk * a.key_chunk;
+  if (k_begin >= lim_max && a.n_chunks > 1) return;  // the merge kernel writes rows without keys
+  const int k_end = min(k_begin + a.key_chunk, lim_max);
+
+  // ---- K/V blocks of this strand into its ring ----
+  unsigned char* ring = smem + strand * ST * L::STAGE;
+  const unsigned char* Kh = a.c.k + kvh * a.c.head_stride;
+  const unsigned char* Vh = a.c.v + kvh * a.c.head_stride;
+  const float* KSh = a.c.ks + kvh * a.c.s_head_stride;
+  const float* VSh = a.c.vs + kvh * a.c.s_head_stride;
+  const int n_blocks = (max(k_end - k_begin, 0) + Q8_KB - 1) / Q8_KB;
+  const int my_n = n_blocks > strand ? (n_blocks - strand + Q8_STRANDS - 1) / Q8_STRANDS : 0;
+  auto load = [&](int i) {  // block i of the strand
+    const int kb = k_begin + (strand + i * Q8_STRANDS) * Q8_KB;
+    unsigned char* st = ring + (i % ST) * L::STAGE;
+    long long page;
+    int row;
+    const bool ok = q8_place(a.c, seq, kb, lane == 0 ? a.err : nullptr, page, row);
+    if (!ok) page = row = 0;
+    const long long off = page * a.c.seq_stride + (long long)row * HD;
+    const long long soff = page * a.c.s_seq_stride + row;
+    const int n = ok ? min(Q8_KB, k_end - kb) : 0;  // rows of the block that hold keys
+    const int first = rg * 32 + lane;
+#pragma unroll
+    for (int u = 0; u < Q8_KB * NC / (32 * RG); ++u) {
+      const int idx = first + u * 32 * RG;
+      const int r = idx / NC, c = idx % NC;
+      const int bytes = r < n ? 16 : 0;
+      const long long o = off + (r < n ? idx * 16 : 0);
+      cp_async16(smem_u32(st + q8_swz<HD>(r, c)), Kh + o, bytes);
+      cp_async16(smem_u32(st + Q8_KB * HD + q8_swz<HD>(r, c)), Vh + o, bytes);
+    }
+    if (rg == 0) {
+      float* sc = reinterpret_cast<float*>(st + 2 * Q8_KB * HD);
+      if (lane < n) {
+        cp_async4(smem_u32(sc + lane), KSh + soff + lane);
+        cp_async4(smem_u32(sc + Q8_KB + lane), VSh + soff + lane);
+      } else {
+        sc[lane] = 0.f;
+        sc[Q8_KB + lane] = 0.f;
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) {
+    if (i < my_n) load(i);
+    cp_async_commit();
+  }
+
+  // ---- Q rows to scaled fp16, dims permuted within 16 to the order of a K register ----
+  for (int r = warp; r < L::ROWS; r += NWARPS) {
+    const int tok = r / a.G, hg = r % a.G;
+    const bool ok = tok < ntok && s_tok_lim[min(tok, ntok - 1)] > 0;
+    constexpr int VEC = HD / 32;
+    float x[VEC];
+    float mx = 0.f;
+    const __nv_bfloat16* src = a.q + ((long long)(ok ? m0 + tok : m0) * a.Hq + kvh * a.G + (ok ? hg : 0)) * HD;
+    uint32_t u[VEC / 2];
+    if constexpr (VEC == 2) {
+      u[0] = reinterpret_cast<const uint32_t*>(src)[lane];
+    } else if constexpr (VEC == 4) {
+      const uint2 w = reinterpret_cast<const uint2*>(src)[lane];
+      u[0] = w.x, u[1] = w.y;
+    } else {
+      const uint4 w = reinterpret_cast<const uint4*>(src)[lane];
+      u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      x[j] = !ok ? 0.f : __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
+      mx = fmaxf(mx, fabsf(x[j]));
+    }
+    mx = warp_max(mx);
+    // 2^(14 - floor(log2 mx)), within fp32's normal powers of two; 1 for zero or non-finite rows
+    int sh = 0;
+    if (mx > 0.f && mx < INFINITY) sh = min(14 - ((int)(__float_as_uint(mx) >> 23) - 127), 120);
+    const float f = __uint_as_float((uint32_t)(sh + 127) << 23);
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) {
+      const int d = lane * VEC + j;
+      const int c = d >> 4, dd = d & 15;
+      const int kp = 2 * (dd >> 2) + (dd & 2) * 4;  // place of dims (dd, dd + 1) among the 16
+      const int cc = 2 * c + (kp >> 3);
+      const __half2 h = __floats2half2_rn(x[j] * f * a.q_sign, x[j + 1] * f * a.q_sign);
+      *reinterpret_cast<__half2*>(sQ + r * HD + ((cc ^ (r & 7)) << 3) + (kp & 7)) = h;
+    }
+    if (lane == 0) {
+      s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
+      s_lim[r] = ok ? s_tok_lim[tok] : 0;
+    }
+  }
+  __syncthreads();
+
+  const int r0 = rg * MT * 16;  // this warp's rows: r0 + mt * 16 + g (+ 8)
+  float rowf[MT][2], Mr[MT][2], mrow[MT][2], lrow[MT][2];
+  int lim[MT][2], er[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      rowf[mt][h] = s_rowf[r0 + mt * 16 + g + 8 * h];
+      lim[mt][h] = s_lim[r0 + mt * 16 + g + 8 * h];
+      mrow[mt][h] = Mr[mt][h] = -INFINITY;
+      lrow[mt][h] = 0.f;
+      er[mt][h] = -90;
+    }
+  float o[MT][2 * NC][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int j = 0; j < 2 * NC; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
+
+  auto sync_strand = [&]() {
+    if (RG == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + strand), "n"(32 * RG) : "memory");
+  };
+
+  for (int i = 0; i < my_n; ++i) {
+    cp_async_wait<ST - 2>();
+    sync_strand();  // block i is there for every warp of the strand; the stage refilled below was read last time
+    if (i + ST - 1 < my_n) load(i + ST - 1);
+    cp_async_commit();
+    const unsigned char* sK = ring + (i % ST) * L::STAGE;
+    const unsigned char* sV = sK + Q8_KB * HD;
+    const float* sc = reinterpret_cast<const float*>(sK + 2 * Q8_KB * HD);
+    const int kb = k_begin + (strand + i * Q8_STRANDS) * Q8_KB;
+    const bool full = kb + Q8_KB <= lim_min;  // every row with keys sees the whole block
+
+    float s[MT][4][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint32_t af[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int row = r0 + mt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+        const int cc = 2 * c + (lane >> 4);
+        ldmatrix_x4(smem_u32(sQ + row * HD + ((cc ^ (row & 7)) << 3)), af[mt][0], af[mt][1], af[mt][2], af[mt][3]);
+      }
+      uint32_t kr[4];  // keys 0-7, 8-15, 16-23, 24-31: dims 16 c + 4 t .. + 3 of key g
+      ldmatrix_x4(smem_u32(sK + q8_swz<HD>(lane, c)), kr[0], kr[1], kr[2], kr[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t b0, b1;
+        q8_to_half<E4M3, true>(kr[j], b0, b1);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) mma_f16_16816(s[mt][j], af[mt], b0, b1);
+      }
+    }
+
+    uint32_t pf[MT][2][4];  // weights, as A fragments of the two 16-key steps
+    auto softmax = [&](auto full_c) {
+      constexpr bool FULL = decltype(full_c)::value;
+      float2 ks[4], vs[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ks[j] = *reinterpret_cast<const float2*>(sc + j * 8 + 2 * t);
+        vs[j] = *reinterpret_cast<const float2*>(sc + Q8_KB + j * 8 + 2 * t);
+      }
+      uint32_t vmax_all = 0;
+      if (FULL) {
+        const uint32_t b = __float_as_uint(sc[Q8_KB + lane]) & 0x7fffffffu;
+        vmax_all = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float fac[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int lm = lim[mt][h];
+          float mx = -INFINITY;
+          uint32_t vm = vmax_all;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kb + j * 8 + 2 * t;
+            float t0 = s[mt][j][2 * h] * ks[j].x, t1 = s[mt][j][2 * h + 1] * ks[j].y;
+            if (!FULL) {
+              t0 = key < lm ? t0 : -INFINITY;
+              t1 = key + 1 < lm ? t1 : -INFINITY;
+              const uint32_t v0 = __float_as_uint(vs[j].x) & 0x7fffffffu, v1 = __float_as_uint(vs[j].y) & 0x7fffffffu;
+              if (key < lm && v0 < 0x7f800000u) vm = max(vm, v0);
+              if (key + 1 < lm && v1 < 0x7f800000u) vm = max(vm, v1);
+            }
+            s[mt][j][2 * h] = t0;
+            s[mt][j][2 * h + 1] = t1;
+            mx = fmaxf(mx, fmaxf(t0, t1));
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (!FULL) {
+            vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+            vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+          }
+          const float mn = fmaxf(mrow[mt][h], mx * rowf[mt][h]);
+          const int en = max(er[mt][h], (int)(vm >> 23) - 127);
+          mrow[mt][h] = mn;
+          er[mt][h] = en;
+          const float Mn = mn + (float)(en - 14);  // -inf while the row has seen no key
+          const float mu = Mn == -INFINITY ? 0.f : Mn;
+          fac[h] = exp2f(Mr[mt][h] - mu);
+          Mr[mt][h] = Mn;
+          float ps = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = kb + j * 8 + 2 * t;
+            const float e0 = exp2f(__fmaf_rn(s[mt][j][2 * h], rowf[mt][h], -mu));
+            const float e1 = exp2f(__fmaf_rn(s[mt][j][2 * h + 1], rowf[mt][h], -mu));
+            ps += e0 + e1;
+            float w0 = e0 * vs[j].x, w1 = e1 * vs[j].y;
+            if (!FULL) {
+              w0 = key < lm ? w0 : 0.f;
+              w1 = key + 1 < lm ? w1 : 0.f;
+            }
+            const __half2 w = __floats2half2_rn(w0, w1);
+            pf[mt][j >> 1][(j & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&w);
+          }
+          lrow[mt][h] = lrow[mt][h] * fac[h] + ps;
+        }
+        if (__any_sync(0xffffffffu, fac[0] != 1.f || fac[1] != 1.f)) {  // a factor of 1 is exact
+#pragma unroll
+          for (int j = 0; j < 2 * NC; ++j) {
+            o[mt][j][0] *= fac[0];
+            o[mt][j][1] *= fac[0];
+            o[mt][j][2] *= fac[1];
+            o[mt][j][3] *= fac[1];
+          }
+        }
+      }
+    };
+    if (full) softmax(std::true_type{});
+    else softmax(std::false_type{});
+
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint32_t vr[4];  // keys (2 t, 2 t + 1) + 0, 8, 16, 24 of dims 16 c + 2 g, + 1
+      ldmatrix_x4_trans(smem_u32(sV + q8_swz<HD>(lane, c)), vr[0], vr[1], vr[2], vr[3]);
+      uint32_t ev[4], od[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) q8_to_half<E4M3, false>(vr[u], ev[u], od[u]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma_f16_16816(o[mt][2 * c], pf[mt][0], ev[0], ev[1]);
+        mma_f16_16816(o[mt][2 * c + 1], pf[mt][0], od[0], od[1]);
+        mma_f16_16816(o[mt][2 * c], pf[mt][1], ev[2], ev[3]);
+        mma_f16_16816(o[mt][2 * c + 1], pf[mt][1], od[2], od[3]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+
+  // ---- merge the strands in order: every warp writes its accumulators (the same lane holds the
+  // same elements in all four), then strand s finishes a quarter of the dims ----
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lrow[mt][h] += __shfl_xor_sync(0xffffffffu, lrow[mt][h], 1);
+      lrow[mt][h] += __shfl_xor_sync(0xffffffffu, lrow[mt][h], 2);
+    }
+  __syncthreads();  // the rings are read no more
+  float4* s_o = reinterpret_cast<float4*>(smem);
+  float2* s_ml = reinterpret_cast<float2*>(smem + Q8_STRANDS * L::ROWS * HD * 4);  // [strand][row]
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        s_o[((((rg * MT + mt) * NC + c) * Q8_STRANDS + strand) * 2 + h) * 32 + lane] =
+            make_float4(o[mt][2 * c][2 * h], o[mt][2 * c + 1][2 * h], o[mt][2 * c][2 * h + 1], o[mt][2 * c + 1][2 * h + 1]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t == 0) s_ml[strand * L::ROWS + r0 + mt * 16 + g + 8 * h] = make_float2(Mr[mt][h], lrow[mt][h]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + mt * 16 + g + 8 * h;
+      const int tok = r / a.G, hg = r % a.G;
+      if (tok >= ntok || !s_tok_ok[tok]) continue;
+      const int lm = s_lim[r];
+      if (a.n_chunks > 1 && lm <= k_begin) continue;
+      float2 ml[Q8_STRANDS];
+      float mm = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < Q8_STRANDS; ++u) {
+        ml[u] = s_ml[u * L::ROWS + r];
+        mm = fmaxf(mm, ml[u].x);
+      }
+      const float mu = mm == -INFINITY ? 0.f : mm;
+      float w[Q8_STRANDS], den = 0.f;
+#pragma unroll
+      for (int u = 0; u < Q8_STRANDS; ++u) {
+        w[u] = exp2f(ml[u].x - mu);
+        den += w[u] * ml[u].y;
+      }
+      const int m = m0 + tok, head = kvh * a.G + hg;
+      const long long base = ((long long)chunk * a.M + m) * a.Hq + head;
+#pragma unroll
+      for (int cq = 0; cq < NC / Q8_STRANDS; ++cq) {
+        const int c = strand * (NC / Q8_STRANDS) + cq;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < Q8_STRANDS; ++u) {
+          const float4 v = s_o[((((rg * MT + mt) * NC + c) * Q8_STRANDS + u) * 2 + h) * 32 + lane];
+          y.x += w[u] * v.x;
+          y.y += w[u] * v.y;
+          y.z += w[u] * v.z;
+          y.w += w[u] * v.w;
+        }
+        const int d = c * 16 + 4 * t;
+        if (a.n_chunks > 1) {
+          *reinterpret_cast<float4*>(a.part_o + base * HD + d) = y;
+        } else {
+          const float inv = lm > 0 ? 1.f / den : 0.f;
+          float f[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+          if (a.gate) {
+            const __nv_bfloat16* gr = a.gate + (long long)m * a.ldg + (long long)head * a.gate_hs + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = f[e] / (1.f + __expf(-bf2f(gr[e])));
+          }
+          *reinterpret_cast<uint2*>(a.out + (long long)m * a.ldo + (long long)head * HD + d) =
+              make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+        }
+      }
+      if (a.n_chunks > 1 && strand == 0 && t == 0) a.part_ml[base] = make_float2(mm, den);
+    }
+}
+
+// Merges the chunk partials of one (row, head) in chunk order: one warp each, hd / 32 dims a lane.
+template <int HD>
+__global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constant__ AttnQ8Args a) {
+  grid_dependency_launch_dependents();
+  grid_dependency_wait();
+  constexpr int VEC = HD / 32;
+  constexpr int FL = 8;  // chunks' loads in flight
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
+  if (item >= (long long)a.M * a.Hq) return;
+  const int m = (int)(item / a.Hq), h = (int)(item % a.Hq);
+  const int p = a.pos[m];
+  if (p < 0) return;
+  const int seq = a.row_seq ? a.row_seq[m] : 0;
+  if (seq < 0 || seq >= a.c.n_seqs) return;
+  if (a.row_seq && a.run_rows > 1) {  // a row that is not of its tile's sequence was refused
+    const int run0 = m / a.run_rows * a.run_rows;
+    const int t0 = run0 + (m - run0) / a.tile_toks * a.tile_toks;
+    int first = t0;
+    while (a.pos[first] < 0) ++first;  // ends at m at the latest
+    if (a.row_seq[first] != seq) return;
+  }
+  const int lim = q8_row_limit(a, m, p, seq, nullptr);
+  const int nch = min((lim + a.key_chunk - 1) / a.key_chunk, a.n_chunks);
+  const long long cstride = (long long)a.M * a.Hq;
+  const float2* ml = a.part_ml + item;
+  const float* po = a.part_o + item * HD + lane * VEC;
+  float mmax = -INFINITY;
+  for (int c = lane; c < nch; c += 32) mmax = fmaxf(mmax, ml[c * cstride].x);
+  mmax = warp_max(mmax);
+  const float mu = mmax == -INFINITY ? 0.f : mmax;
+  float acc[VEC], den = 0.f;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  for (int c0 = 0; c0 < nch; c0 += 32) {
+    const float2 x = c0 + lane < nch ? ml[(c0 + lane) * cstride] : make_float2(-INFINITY, 0.f);
+    const float w = exp2f(x.x - mu);
+    den += warp_sum(w * x.y);
+    const int n = min(32, nch - c0);
+    for (int j0 = 0; j0 < n; j0 += FL) {
+      float v[FL][VEC];
+#pragma unroll
+      for (int u = 0; u < FL; ++u)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[u][i] = j0 + u < n ? po[(long long)(c0 + j0 + u) * cstride * HD + i] : 0.f;
+#pragma unroll
+      for (int u = 0; u < FL; ++u) {
+        const float wj = __shfl_sync(0xffffffffu, w, (j0 + u) & 31);
+        if (j0 + u < n) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc[i] += wj * v[u][i];
+        }
+      }
+    }
+  }
+  const float inv = lim > 0 ? 1.f / den : 0.f;
+  __nv_bfloat16* dst = a.out + (long long)m * a.ldo + (long long)h * HD + lane * VEC;
+  float y[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) y[i] = acc[i] * inv;
+  if (a.gate) {
+    const __nv_bfloat16* gr = a.gate + (long long)m * a.ldg + (long long)h * a.gate_hs + lane * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = y[i] / (1.f + __expf(-bf2f(gr[i])));
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(y[i], y[i + 1]);
+}
+
+template <int HD, int MT, int RG, int ST, bool E4M3>
+static int launch_attn_q8(const AttnQ8Args& a, int tiles, cudaStream_t st) {
+  using L = AttnQ8Layout<HD, MT, RG, ST>;
+  static bool opted[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !opted[dev]) {
+    if (cudaFuncSetAttribute(attn_q8_kernel<HD, MT, RG, ST, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             L::SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      set_error("dfl_attention_q8: cannot opt in to %d bytes of shared memory", L::SMEM);
+      return DFL_ERR_UNSUPPORTED;
+    }
+    if (dev >= 0 && dev < 64) opted[dev] = true;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles, a.c.Hkv, a.n_chunks);
+  cfg.blockDim = dim3(32 * Q8_STRANDS * RG);
+  cfg.dynamicSmemBytes = L::SMEM;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_kernel<HD, MT, RG, ST, E4M3>, a);
+  if (e == cudaSuccess && a.n_chunks > 1) {
+    const long long items = (long long)a.M * a.Hq;
+    cfg.gridDim = dim3((unsigned)((items + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<HD>, a);
+  }
+  if (e != cudaSuccess) {
+    set_error("dfl_attention_q8: launch failed: %s", cudaGetErrorString(e));
+    return DFL_ERR_CUDA;
+  }
+  return DFL_OK;
+}
+
+template <int HD, bool E4M3>
+static int launch_attn_q8_rows(const AttnQ8Args& a, int rows, int tiles, cudaStream_t st) {
+  if (rows <= 16) return launch_attn_q8<HD, 1, 1, 3, E4M3>(a, tiles, st);
+  if constexpr (HD == 256) {
+    return launch_attn_q8<HD, 1, 2, 2, E4M3>(a, tiles, st);
+  } else {
+    if (rows <= 32) return launch_attn_q8<HD, 2, 1, 2, E4M3>(a, tiles, st);
+    return launch_attn_q8<HD, 2, 2, 4, E4M3>(a, tiles, st);
+  }
+}
+
+}  // namespace dfl
+
+using namespace dfl;
+
+// Keys per chunk for a call of `runs` sequences: enough chunks for about eight CTAs per SM at
+// one tile a run, between one block per strand and 2048 keys. Runs, not rows, so that decode
+// and verify of the same sequences split alike.
+static int q8_key_chunk(int key_chunk, long long runs, int Hkv, int max_kv) {
+  if (key_chunk > 0) return key_chunk;
+  const long long c = (long long)max_kv * runs * Hkv / (148 * 8);
+  const long long r = (c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT;
+  return (int)(r < Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : r > 2048 ? 2048 : r);
+}
+
+static int q8_run_rows(int M, int seq_rows, bool one_seq) {
+  return one_seq ? M : seq_rows > 0 ? (seq_rows < M ? seq_rows : M) : 1;
+}
+
+static size_t q8_workspace(int M, int Hq, int hd, int n_chunks) {
+  if (n_chunks <= 1) return 0;
+  const size_t o = (size_t)n_chunks * M * Hq * hd * sizeof(float);
+  return ((o + 255) & ~(size_t)255) + (size_t)n_chunks * M * Hq * sizeof(float2);
+}
+
+extern "C" size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq,
+                                                   int max_kv, int key_chunk) {
+  if (!cache || M <= 0 || Hq <= 0 || max_kv <= 0 || key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT || cache->n_kv_heads <= 0)
+    return 0;
+  const int rr = q8_run_rows(M, seq_rows, one_seq != 0);
+  const int kc = q8_key_chunk(key_chunk, (M + rr - 1) / rr, cache->n_kv_heads, max_kv);
+  return q8_workspace(M, Hq, cache->head_dim, (max_kv + kc - 1) / kc);
+}
+
+extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq,
+                                const int32_t* kv_len, int seq_rows, int M, int Hq, int causal, float scale,
+                                int max_kv, int key_chunk, void* out, int64_t ldo, const void* gate, int64_t ldg,
+                                int gate_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dfl_attention_q8";
+  if (M == 0) return DFL_OK;
+  AttnQ8Args a;
+  if (const int s = q8_cache(cache, who, &a.c)) return s;
+  const int hd = cache->head_dim, Hkv = cache->n_kv_heads;
+  if (!q || !pos || !out || (!causal && !kv_len) || M < 0 || Hq <= 0 || Hq % Hkv || max_kv <= 0 || seq_rows < 0) {
+    set_error("%s: bad arguments (M=%d Hq=%d Hkv=%d max_kv=%d)", who, M, Hq, Hkv, max_kv);
+    return DFL_ERR_INVALID;
+  }
+  const int G = Hq / Hkv;
+  if (G > 16) {
+    set_error("%s: query heads per kv head must be 1..16 (got %d)", who, G);
+    return DFL_ERR_UNSUPPORTED;
+  }
+  if (key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT) {
+    set_error("%s: key_chunk %d must be a multiple of %d", who, key_chunk, Q8_CHUNK_UNIT);
+    return DFL_ERR_INVALID;
+  }
+  if (!(scale == scale) || scale - scale != 0.f) {
+    set_error("%s: the softmax scale must be finite", who);
+    return DFL_ERR_INVALID;
+  }
+  if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 8 || ldo % 4 ||
+      ldo < (int64_t)Hq * hd) {
+    set_error("%s: q must be 16-byte and out 8-byte aligned, ldo a multiple of 4 and at least Hq * hd (ldo=%lld)",
+              who, (long long)ldo);
+    return DFL_ERR_UNSUPPORTED;
+  }
+  const int run_rows = q8_run_rows(M, seq_rows, row_seq == nullptr);
+  const int runs = (M + run_rows - 1) / run_rows;
+  a.key_chunk = q8_key_chunk(key_chunk, runs, Hkv, max_kv);
+  a.n_chunks = (int)(((long long)max_kv + a.key_chunk - 1) / a.key_chunk);
+  if (a.n_chunks > 65535) {
+    set_error("%s: %d key chunks; a larger key_chunk is needed", who, a.n_chunks);
+    return DFL_ERR_UNSUPPORTED;
+  }
+  const size_t need = q8_workspace(M, Hq, hd, a.n_chunks);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) {
+    set_error("%s: workspace missing, misaligned or too small (%zu < %zu)", who, workspace_bytes, need);
+    return DFL_ERR_WORKSPACE;
+  }
+  // rows a CTA takes: 16, 32 or (head_dim <= 128) 64 rows of (token, head) pairs
+  const int most = hd == 256 ? 32 : 64;
+  const long long want = (long long)run_rows * G;
+  const int rows = want <= 16 ? 16 : want <= 32 ? 32 : most;
+  a.run_rows = run_rows;
+  a.run_tiles = (run_rows + rows / G - 1) / (rows / G);
+  a.tile_toks = (run_rows + a.run_tiles - 1) / a.run_tiles;
+  const long long tiles = (long long)runs * a.run_tiles;
+  if (tiles > 0x7fffffffLL) {
+    set_error("%s: too many rows (%d)", who, M);
+    return DFL_ERR_UNSUPPORTED;
+  }
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.pos = pos;
+  a.row_seq = row_seq;
+  a.kv_len = kv_len;
+  a.part_o = static_cast<float*>(workspace);
+  const size_t o_bytes = (size_t)a.n_chunks * M * Hq * hd * sizeof(float);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + ((o_bytes + 255) & ~(size_t)255));
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.ldo = ldo;
+  a.gate = static_cast<const __nv_bfloat16*>(gate);
+  a.ldg = ldg;
+  a.gate_hs = gate_head_stride > 0 ? gate_head_stride : hd;
+  a.M = M;
+  a.Hq = Hq;
+  a.G = G;
+  a.causal = causal;
+  a.max_kv = max_kv;
+  a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+  a.scale_log2 = scale == 0.f ? 1.f : (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  a.err = device_error_word();
+  cudaStream_t st = as_stream(stream);
+  const bool e4 = cache->type == DFL_KV_E4M3;
+  switch (hd) {
+    case 64: return e4 ? launch_attn_q8_rows<64, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<64, false>(a, rows, (int)tiles, st);
+    case 128: return e4 ? launch_attn_q8_rows<128, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<128, false>(a, rows, (int)tiles, st);
+    default: return e4 ? launch_attn_q8_rows<256, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<256, false>(a, rows, (int)tiles, st);
+  }
+}

@@ -448,6 +448,175 @@ def attention_qkv(qkv: torch.Tensor, pos: torch.Tensor, q_norm: torch.Tensor, k_
     return out
 
 
+class KvQ8(ctypes.Structure):
+    """dfl_kv_q8: one layer's 8-bit K/V cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("seq_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("scale_seq_stride", ctypes.c_int64), ("scale_head_stride", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("pt_stride", ctypes.c_int64), ("page_size", ctypes.c_int),
+                ("n_seqs", ctypes.c_int), ("n_pages", ctypes.c_int), ("cap", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("type", ctypes.c_int)]
+
+
+KV_Q8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # DFL_KV_INT8, DFL_KV_E4M3
+
+
+class QuantKV:
+    """One layer's 8-bit K/V cache (dfl_kv_q8), checked once: codes ``k`` / ``v``
+    [seq, Hkv, cap, hd] int8 or float8_e4m3fn and fp32 scales [seq, Hkv, cap], the value held
+    being code * scale; or, with ``page_table`` [seq, pages] int32, page pools
+    [n_pages, Hkv, page_size, hd] and [n_pages, Hkv, page_size]. The tensors may be views
+    (sequence and head strides are free), K and V alike."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 page_table: torch.Tensor | None = None, page_size: int = 0):
+        _need_cuda(k, v, k_scale, v_scale, page_table)
+        if k.dtype not in KV_Q8_TYPES or v.dtype != k.dtype:
+            raise ValueError(f"8-bit cache codes are int8 or float8_e4m3fn, K and V alike (got {k.dtype}, {v.dtype})")
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride():
+            raise ValueError("k and v must be [seq, Hkv, cap, hd] (or [pages, Hkv, page_size, hd]) alike")
+        hd = k.shape[3]
+        if k.stride(3) != 1 or (k.shape[2] > 1 and k.stride(2) != hd):
+            raise ValueError("a head's positions must follow one another (strides [.., hd, 1])")
+        if (k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != k.shape[:3]
+                or v_scale.shape != k.shape[:3] or k_scale.stride() != v_scale.stride()
+                or (k.shape[2] > 1 and k_scale.stride(2) != 1)):
+            raise ValueError("k_scale and v_scale must be fp32 [seq, Hkv, cap] alike, a head's positions dense")
+        if any(t is not None and t.device != k.device for t in (v, k_scale, v_scale, page_table)):
+            raise ValueError("an 8-bit cache's tensors live on one device")
+        if page_table is not None:
+            if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+                raise ValueError("page_table must be int32 [seq, pages], row-major")
+            if page_size != k.shape[2]:
+                raise ValueError(f"page_size {page_size} is not the pools' ({k.shape[2]})")
+        elif page_size:
+            raise ValueError("page_size given without a page_table")
+        self.tensors = (k, v, k_scale, v_scale, page_table)  # keeps the memory alive
+        self.device, self.dtype = k.device, k.dtype
+        self.n_kv_heads, self.head_dim = k.shape[1], hd
+        self.n_seqs = page_table.shape[0] if page_table is not None else k.shape[0]
+        self.cap = page_table.shape[1] * page_size if page_table is not None else k.shape[2]
+        one = lambda t, d: t.stride(d) if t.shape[d] > 1 else 0  # noqa: E731
+        self.desc = KvQ8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), one(k, 0), one(k, 1),
+                         one(k_scale, 0), one(k_scale, 1), _ptr(page_table),
+                         page_table.stride(0) if page_table is not None else 0, int(page_size), self.n_seqs,
+                         k.shape[0] if page_table is not None else 0, self.cap, self.n_kv_heads, hd,
+                         KV_Q8_TYPES[k.dtype])
+        self._ref = ctypes.byref(self.desc)
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point on ``device``'s current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _index_rows(what: str, t: torch.Tensor | None, n: int, device: torch.device) -> None:
+    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or t.device != device
+                          or (n > 1 and t.stride(0) != 1)):
+        raise ValueError(f"{what} must be contiguous int32 with at least {n} entries on {device}")
+
+
+def qkv_rope_append_q8(qkv: torch.Tensor, pos: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor,
+                       inv_freq: torch.Tensor, kv: QuantKV, Hq: int, rot_dim: int, eps: float,
+                       q_out: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
+                       q_stride: int | None = None, do_q: bool = True) -> torch.Tensor | None:
+    """q/k head norm + RoPE of the projection rows ``qkv`` [M, q heads | k heads | v heads], the
+    keys and values quantised into the 8-bit cache as they are written (dfl_qkv_rope_append_q8);
+    returns the rotated queries [M, Hq, hd] bf16. Rows with pos < 0 are skipped. The rows of one
+    call must name distinct (sequence, position) pairs."""
+    dev, hd, M = kv.device, kv.head_dim, qkv.shape[0]
+    qs = hd if q_stride is None else q_stride
+    if qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 \
+            or qkv.shape[1] < Hq * qs + 2 * kv.n_kv_heads * hd:
+        raise ValueError(f"qkv must be bf16 rows of at least {Hq * qs + 2 * kv.n_kv_heads * hd} columns on {dev}")
+    _index_rows("pos", pos, M, dev)
+    _index_rows("row_seq", row_seq, M, dev)
+    for w in (q_norm, k_norm) if do_q else (k_norm,):
+        if w.dtype != torch.bfloat16 or w.shape != (hd,) or not w.is_contiguous() or w.device != dev:
+            raise ValueError(f"norm weights must be contiguous bf16 [{hd}] on {dev}")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous() \
+            or inv_freq.device != dev:
+        raise ValueError(f"inv_freq must be contiguous fp32 with rot_dim / 2 entries on {dev}")
+    if not do_q:
+        q_out = None
+    elif q_out is None:
+        q_out = torch.empty((M, Hq, hd), dtype=torch.bfloat16, device=dev)
+    elif q_out.dtype != torch.bfloat16 or q_out.shape != (M, Hq, hd) or not q_out.is_contiguous() \
+            or q_out.device != dev:
+        raise ValueError(f"q_out must be contiguous bf16 [{M}, {Hq}, {hd}] on {dev}")
+    _call_on(dev, "dfl_qkv_rope_append_q8", qkv.data_ptr(), _row_stride(qkv), qs, pos.data_ptr(), _ptr(row_seq),
+             _ptr(q_norm), k_norm.data_ptr(), inv_freq.data_ptr(), _ptr(q_out), kv._ref, M, Hq, rot_dim, float(eps),
+             int(do_q))
+    return q_out
+
+
+def kv_read_q8(kv: QuantKV, pos: torch.Tensor, row_seq: torch.Tensor | None = None,
+               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of position pos[r] of sequence row_seq[r] (None: sequence 0) of an 8-bit
+    cache as bf16 [M, Hkv, hd] (dfl_kv_read_q8). Rows with pos < 0 are left as they are."""
+    dev, M = kv.device, pos.shape[0]
+    _index_rows("pos", pos, M, dev)
+    _index_rows("row_seq", row_seq, M, dev)
+    shape = (M, kv.n_kv_heads, kv.head_dim)
+    outs = []
+    for t in (k_out, v_out):
+        if t is None:
+            t = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        elif t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"outputs must be contiguous bf16 {list(shape)} on {dev}")
+        outs.append(t)
+    _call_on(dev, "dfl_kv_read_q8", kv._ref, pos.data_ptr(), _ptr(row_seq), M, outs[0].data_ptr(), outs[1].data_ptr())
+    return outs[0], outs[1]
+
+
+def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, max_kv: int,
+                 kv_len: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
+                 scale: float | None = None, out: torch.Tensor | None = None, ws: Workspace | None = None,
+                 gate: torch.Tensor | None = None, gate_head_stride: int = 0, seq_rows: int = 0,
+                 key_chunk: int = 0) -> torch.Tensor:
+    """attention() over an 8-bit cache (dfl_attention_q8): q [M, Hq, hd] bf16 against ``kv``;
+    returns [M, Hq*hd] bf16. seq_rows: rows per sequence when row_seq groups contiguous runs (0 =
+    any layout). key_chunk (a multiple of 128; 0 = chosen from the sequences, heads and max_kv):
+    results depend on it. Rows with pos < 0 are left as they are; rows that see no key are zero.
+    ``ws``: partial results live in its attention scratch (one workspace per stream and captured
+    graph, as for attention()); without it each call allocates its own."""
+    dev, hd = kv.device, kv.head_dim
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != hd or not q.is_contiguous() or q.device != dev:
+        raise ValueError(f"q must be contiguous bf16 [M, Hq, {hd}] on {dev}")
+    M, Hq = q.shape[0], q.shape[1]
+    _index_rows("pos", pos, M, dev)
+    _index_rows("row_seq", row_seq, M, dev)
+    _index_rows("kv_len", kv_len, kv.n_seqs, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    if out is None:
+        out = torch.empty((M, Hq * hd), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or out.shape != (M, Hq * hd) or out.device != dev:
+        raise ValueError(f"out must be bf16 [{M}, {Hq * hd}] on {dev}")
+    if gate is not None:
+        ghs = gate_head_stride if gate_head_stride > 0 else hd
+        if gate.dtype != torch.bfloat16 or gate.device != dev or gate.dim() != 2 or gate.shape[0] < M \
+                or gate.shape[1] < (Hq - 1) * ghs + hd:
+            raise ValueError(f"gate must be bf16 rows covering {Hq} heads on {dev}")
+    need = int(_lib.query("dfl_attention_q8_workspace_bytes", kv._ref, M, Hq, int(seq_rows), int(row_seq is None),
+                          int(max_kv), int(key_chunk)))
+    if ws is not None:
+        ws.ensure_attn(need)
+        scratch = ws.attn
+    else:
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call_on(dev, "dfl_attention_q8", q.data_ptr(), kv._ref, pos.data_ptr(), _ptr(row_seq), _ptr(kv_len),
+             int(seq_rows), M, Hq, int(causal), float(scale), int(max_kv), int(key_chunk), out.data_ptr(),
+             _row_stride(out), _ptr(gate), _row_stride(gate) if gate is not None else 0, int(gate_head_stride),
+             _ptr(scratch), scratch.numel() if scratch is not None else 0)
+    return out
+
+
 def argmax_reduce(partials: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     _need_cuda(partials, out)
     M, ntiles = partials.shape[0], partials.shape[1]

@@ -316,6 +316,73 @@ int dfl_attention_qkv(const void* qkv, int64_t ldqkv, const void* q_norm, const 
                       int max_kv, int key_chunk, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* ---- 8-bit K/V cache --------------------------------------------------------
+ * A layer's cache held in one byte per element with an fp32 scale for every (position, kv
+ * head) of K and of V: the value held is code * scale. The scale block is one position, so
+ * that a row's codes depend on that row alone: rewriting a rejected draft position, or
+ * decoding with another block length, leaves every other row's codes and therefore every
+ * token as they were (a scale shared by several positions would have to follow each of them).
+ * No counterpart in the reference, whose KVCache holds bf16 (adapters.py:600-601).
+ * Quantising a row of hd values with a = max |x|: int8 codes are rint(x * (127 / a)) with
+ * scale a / 127, e4m3 codes e4m3(x * (448 / a)) (nearest even) with scale a / 448; a = 0 gives
+ * scale 0; a row that holds an infinity or a NaN gets scale NaN and codes 0.
+ * Codes are [seq][Hkv][cap][hd] bytes (or pages [page][Hkv][page_size][hd], page_table as in
+ * dfl_attention_paged), scales [seq][Hkv][cap] (or [page][Hkv][page_size]) floats: a head's
+ * positions follow one another without gaps, sequences (pages) and heads are strides apart;
+ * K and V have the same strides. Codes are 16-byte aligned, seq_stride and head_stride
+ * multiples of 16, hd in {64, 128, 256}, page_size a power of two >= 64. The e4m3 NaN codes
+ * 0x7f and 0xff are never written and must not occur where a position is read.
+ * The kernels check positions, sequences and page numbers against n_seqs, cap and n_pages:
+ * what is out of range is not accessed and sets the device error word (dfl_device_error):
+ * 340 a row's sequence (out of range, or two sequences in one run of seq_rows rows), 341 a
+ * position or key range beyond cap or max_kv, 342 a page number. */
+#define DFL_KV_INT8 0
+#define DFL_KV_E4M3 1
+typedef struct dfl_kv_q8 {
+  void* k;               /* codes */
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t seq_stride, head_stride;             /* codes: bytes between sequences (pages) and between heads */
+  int64_t scale_seq_stride, scale_head_stride; /* scales: floats */
+  const int32_t* page_table;                   /* NULL: contiguous slots */
+  int64_t pt_stride;
+  int page_size;
+  int n_seqs;  /* sequences a row may name */
+  int n_pages; /* pages in the pools (with page_table) */
+  int cap;     /* positions a sequence can hold: its slots, or page_size * the table's columns */
+  int n_kv_heads, head_dim, type;
+} dfl_kv_q8;
+
+/* q/k head norm + RoPE, as dfl_qkv_rope_append, into an 8-bit cache: q_out in bf16, the key
+ * and value rows quantised as they are written. fp32 throughout with one rounding at the end
+ * (no bf16 rounding between norm, rotation and quantiser), and rotary angles formed and
+ * reduced in fp64, so far positions keep their phase. Rows with pos < 0 are skipped; the rows of
+ * one call name distinct (sequence, position) pairs. qkv rows 16-byte aligned (ldqkv, q_stride
+ * % 8 == 0), rot_dim % 16 == 0. do_q = 0 leaves the q heads out (Hq may be 0). */
+int dfl_qkv_rope_append_q8(const void* qkv, int64_t ldqkv, int q_stride, const int32_t* pos, const int32_t* row_seq,
+                           const void* q_norm, const void* k_norm, const float* inv_freq, void* q_out,
+                           const dfl_kv_q8* cache, int M, int Hq, int rot_dim, float eps, int do_q, void* stream);
+/* Reads cache rows back: k_out / v_out[r] = bf16(code * scale) of position pos[r] of sequence
+ * row_seq[r] (NULL: sequence 0), for every kv head: dense [M][Hkv][hd], 16-byte aligned. Rows
+ * with pos < 0 are left as they are. */
+int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq, int M, void* k_out, void* v_out,
+                   void* stream);
+/* dfl_attention (same arguments and meanings) over an 8-bit cache, at most 16 query heads per
+ * kv head. Rows of one sequence share a tile: with row_seq, every run of seq_rows rows starting
+ * at a multiple of seq_rows belongs to one sequence (0 = any layout: each row is its own run);
+ * without it all rows are sequence 0's. key_chunk (multiple of 128; 0 = chosen from the number
+ * of runs, n_kv_heads and max_kv): keys per split; a row's result depends on it and on nothing
+ * else of the call but the row's own query and keys. A row with pos >= 0 that sees no key
+ * (kv_len <= 0) is zero; rows with pos < 0 are left as they are. max_kv bounds every row's
+ * keys. ldo % 4 == 0, q 16-byte and out 8-byte aligned. */
+size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq, int max_kv,
+                                        int key_chunk);
+int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq,
+                     const int32_t* kv_len, int seq_rows, int M, int Hq, int causal, float scale, int max_kv,
+                     int key_chunk, void* out, int64_t ldo, const void* gate, int64_t ldg, int gate_head_stride,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- speculative step control ---------------------------------------------
  * Greedy argmax from DFL_EPI_ARGMAX partials (runtime.py:22-29 at temperature 0). */
 int dfl_argmax_reduce(const void* partials, int M, int n_tiles, int32_t* out, void* stream);

@@ -1,0 +1,392 @@
+"""8-bit K/V cache: the quantising append, the attention over the codes and the read-back, each
+against a plain implementation in 64 bits; rows that do not depend on their neighbours, masked
+garbage, untouched rows, strides, streams and graphs.
+
+Tolerances count the roundings: half a step is eps / 2 relative to the value (bf16 2^-8, fp16 2^-11,
+e4m3 2^-4); fp32 work in between is given 2^-18 of the largest term (a few ulps of 2^-24 per step
+over sums of at most 256)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+TOP = {"int8": 127.0, "e4m3": 448.0}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need(lib):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def _quantise(x, t):
+    a = x.abs().amax(-1)
+    y = x * torch.where(a > 0, TOP[t] / a, torch.zeros_like(a))[..., None]
+    return (y.round() if t == "int8" else y).to(TYPES[t]), a / TOP[t]
+
+
+class Cache:
+    """Random codes for B sequences of the given lengths; everything behind a length is garbage
+    (NaN and huge scales, random codes without e4m3 NaNs)."""
+
+    def __init__(self, t, lens, Hkv, hd, page=0, seed=0, slack=5, wide=False):
+        from dflash_b200 import ops
+        g = torch.Generator().manual_seed(seed)
+        B, cap = len(lens), max(lens) + slack
+        x = torch.randn((2, B, Hkv, cap, hd), generator=g)
+        x[0, ..., ::16] *= 5
+        x *= torch.exp(2 * torch.randn((2, B, Hkv, cap, 1), generator=g)) if wide else 1 + torch.rand((2, B, Hkv, cap, 1), generator=g)
+        codes, scale = _quantise(x, t)
+        self.val = codes.double() * scale.double()[..., None]  # [2, B, Hkv, cap, hd]
+        for b, n in enumerate(lens):
+            scale[:, b, :, n:] = torch.tensor([math.nan, 3e30, math.inf, 1.0, -2.0])[torch.arange(cap - n) % 5]
+        table = None
+        if page:
+            need = [(n + page - 1) // page for n in lens]
+            order = torch.randperm(sum(need) + 1, generator=g)
+            table = torch.full((B, max(need) + 1), -7, dtype=torch.int32)
+            pc = torch.full((2, sum(need) + 1, Hkv, page, hd), 3, dtype=torch.uint8)
+            ps = torch.full((2, sum(need) + 1, Hkv, page), math.nan)
+            at = 0
+            for b, n in enumerate(need):
+                for i in range(n):
+                    pg = int(order[at])
+                    table[b, i] = pg
+                    m = min(page, cap - i * page)
+                    pc[:, pg, :, :m] = codes.view(torch.uint8)[:, b, :, i * page:i * page + m]
+                    ps[:, pg, :, :m] = scale[:, b, :, i * page:i * page + m]
+                    at += 1
+            codes, scale = pc.view(TYPES[t]), ps
+            table = table.to(DEV)
+        self.codes, self.scale = codes.to(DEV), scale.to(DEV)
+        self.kv = ops.QuantKV(self.codes[0], self.codes[1], self.scale[0], self.scale[1], page_table=table,
+                              page_size=page)
+
+
+def _attention64(val, q, lim, seq, scale, gate=None):
+    """(o, tolerance): attention in 64 bits; rows with lim 0 are zero."""
+    M, Hq, hd = q.shape
+    Hkv = val.shape[2]
+    G = Hq // Hkv
+    o, A, smax = torch.zeros(M, Hq, hd, dtype=torch.float64), torch.zeros(M, Hq, hd, dtype=torch.float64), 0.0
+    low = torch.zeros(M, Hq, hd, dtype=torch.float64)
+    for m in range(M):
+        n = int(lim[m])
+        if n <= 0:
+            continue
+        k, v = val[0, int(seq[m]), :, :n], val[1, int(seq[m]), :, :n]
+        qm = q[m].double().view(Hkv, G, hd)
+        p = torch.softmax(torch.einsum("hgd,hnd->hgn", qm, k) * scale, -1)
+        smax = max(smax, float((torch.einsum("hgd,hnd->hgn", qm.abs(), k.abs()) * abs(scale)).max()))
+        o[m] = torch.einsum("hgn,hnd->hgd", p, v).reshape(Hq, hd)
+        A[m] = torch.einsum("hgn,hnd->hgd", p, v.abs()).reshape(Hq, hd)
+        # fp16's lower end: a weight p_j vs_j is held in units in which the row's largest e_j times
+        # the largest vs lies in [2^14, 2^16), rounded there to a multiple of 2^-24 at worst: off by
+        # 2^-25 / 2^14 = 2^-39 of max p * max vs <= max vs. Summed over n codes of at most TOP, and
+        # max vs * TOP being the largest |v|: n 2^-39 max |v|
+        low[m] = (n * 2.0 ** -39 * v.abs().amax((1, 2)))[:, None, None].expand(Hkv, G, hd).reshape(Hq, hd)
+    o, A, low = o.reshape(M, Hq * hd), A.reshape(M, Hq * hd), low.reshape(M, Hq * hd)
+    if gate is not None:
+        s = torch.sigmoid(gate.double())
+        o, A, low = o * s, A * s, low * s
+    # weights: fp16 (2^-11) and their exponent's error: scores summed in fp32 over hd terms of at
+    # most smax in all, 2^-23 each step, in numerator and denominator
+    tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18 + 2 * hd * 2.0 ** -23 * smax) * A + low
+    return o, tol
+
+
+CASES = [
+    # type, lens, rows, Hkv, G, hd, page, causal, gate, key_chunk
+    ("int8", [1], 1, 1, 1, 64, 0, True, False, 0),
+    ("e4m3", [1], 1, 2, 4, 128, 64, True, False, 0),
+    ("int8", [33, 32, 31], 1, 2, 3, 128, 64, True, True, 0),
+    ("e4m3", [129, 640, 7], 1, 1, 8, 256, 128, True, False, 128),
+    ("int8", [1000, 517], 5, 2, 4, 128, 0, True, False, 256),
+    ("e4m3", [200, 130, 384], 16, 2, 4, 128, 64, True, False, 128),
+    ("int8", [700, 90], 16, 1, 6, 256, 0, True, True, 512),
+    ("e4m3", [150], 150, 2, 5, 64, 64, True, False, 128),
+    ("int8", [261], 37, 1, 16, 128, 128, True, True, 0),
+    ("int8", [300, 1, 64], 16, 2, 2, 64, 0, False, False, 128),
+    ("e4m3", [77, 513], 8, 2, 4, 128, 64, False, True, 0),
+    ("int8", [2100], 1, 2, 7, 128, 64, False, False, 128),
+]
+
+
+@pytest.mark.parametrize("t,lens,rows,Hkv,G,hd,page,causal,gated,chunk", CASES)
+def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gated, chunk):
+    from dflash_b200 import ops
+    c = Cache(t, lens, Hkv, hd, page, seed=hd + rows, wide=rows == 5)
+    g = torch.Generator().manual_seed(7)
+    B, Hq = len(lens), Hkv * G
+    q = (1.5 * torch.randn(B * rows, Hq, hd, generator=g)).bfloat16()
+    seq = torch.arange(B, dtype=torch.int32).repeat_interleave(rows)
+    # the run's last row sits at its sequence's last position (positions below 0: rows skipped)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32).clamp_min(-1)
+    kv_len = torch.tensor(lens, dtype=torch.int32)
+    gate = torch.randn(B * rows, Hq * hd, generator=g).bfloat16() if gated else None
+    out = torch.full((B * rows, Hq * hd), 9.0, dtype=torch.bfloat16, device=DEV)
+    ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), causal, max(lens), kv_len=kv_len.to(DEV),
+                     row_seq=seq.to(DEV) if B > 1 else None, seq_rows=rows, key_chunk=chunk, out=out,
+                     gate=gate.to(DEV) if gated else None)
+    lim = pos + 1 if causal else kv_len[seq.long()]
+    ref, tol = _attention64(c.val, q, lim, seq, hd ** -0.5, gate)
+    live = pos >= 0
+    err = (out.double().cpu() - ref).abs()[live]
+    assert ops.device_error() == 0
+    assert (err <= tol[live]).all(), float((err / tol[live]).max())
+    assert (out[~live.to(DEV)] == 9.0).all()  # rows with pos < 0 are left as they were
+
+
+@pytest.mark.parametrize("t", ["int8", "e4m3"])
+@pytest.mark.parametrize("G,hd", [(1, 128), (4, 128), (2, 64), (3, 256), (6, 128)])
+def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd):
+    """A verify block's rows equal single-token calls bit for bit, with later rows' keys (masked for
+    the earlier ones) NaN, infinite or huge; paged equals contiguous."""
+    from dflash_b200 import ops
+    lens, rows, Hkv = [300, 77], 16, 2
+    flat, paged = Cache(t, lens, Hkv, hd, 0, seed=3), Cache(t, lens, Hkv, hd, 64, seed=3)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(2 * rows, Hkv * G, hd, generator=g).bfloat16().to(DEV)
+    seq = torch.arange(2, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
+    kw = dict(causal=True, max_kv=300, key_chunk=128)
+    full = ops.attention_q8(q, flat.kv, pos, row_seq=seq, seq_rows=rows, **kw)
+    assert torch.equal(full, ops.attention_q8(q, paged.kv, pos, row_seq=seq, seq_rows=rows, **kw))
+    assert torch.equal(full, ops.attention_q8(q, flat.kv, pos, row_seq=seq, **kw))  # any layout
+    for b in range(2):
+        one = ops.attention_q8(q[b * rows:b * rows + 5].contiguous(), flat.kv, pos[b * rows:b * rows + 5],
+                               row_seq=seq[b * rows:b * rows + 5], seq_rows=1, **kw)
+        assert torch.equal(one, full[b * rows:b * rows + 5])
+    # later rows' keys and values poisoned: earlier rows keep their bits
+    for bad in (math.nan, math.inf, 1e30):
+        for b, n in enumerate(lens):
+            flat.scale[:, b, :, n - 6:n] = bad
+        got = ops.attention_q8(q, flat.kv, pos, row_seq=seq, seq_rows=rows, **kw)
+        for b in range(2):
+            assert torch.equal(got[b * rows:b * rows + 10], full[b * rows:b * rows + 10])
+        if bad != 1e30:  # and the rows that see them say so
+            assert got[10:16].isnan().all()
+    assert ops.device_error() == 0
+
+
+def test_rows_without_keys_are_zero_and_empty_calls_do_nothing():
+    from dflash_b200 import ops
+    c = Cache("int8", [40, 40, 40], 2, 128)
+    q = torch.randn(3, 4, 128).bfloat16().to(DEV)
+    seq = torch.arange(3, dtype=torch.int32, device=DEV)
+    pos = torch.tensor([0, 5, -1], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor([40, 0, 40], dtype=torch.int32, device=DEV)
+    for max_kv in (40, 1000):  # one chunk, several
+        c2 = c if max_kv == 40 else Cache("int8", [40, 40, 1000], 2, 128)
+        out = torch.full((3, 512), 5.0, dtype=torch.bfloat16, device=DEV)
+        ops.attention_q8(q, c2.kv, pos, False, max_kv, kv_len=kv_len, row_seq=seq, seq_rows=1, out=out, key_chunk=128)
+        assert (out[1] == 0).all() and (out[2] == 5).all() and out[0].isfinite().all() and (out[0] != 5).any()
+    assert ops.attention_q8(q[:0], c.kv, pos[:0], True, 40).shape == (0, 512)
+    assert ops.kv_read_q8(c.kv, pos[:0])[0].shape == (0, 2, 128)
+    assert ops.device_error() == 0
+
+
+def test_scales_and_queries_of_extreme_size():
+    """Values far from 1 keep their relative precision; a softmax scale of 0 averages the values."""
+    from dflash_b200 import ops
+    for ks, vs, qs in ((1e-20, 1e-20, 1e15), (1e12, 1e25, 1e-12), (1.0, 1e-30, 1.0)):
+        c = Cache("int8", [200], 2, 128, seed=9)
+        c.scale[0] *= ks
+        c.scale[1] *= vs
+        val = torch.stack([c.val[0] * ks, c.val[1] * vs])
+        q = (torch.randn(4, 8, 128, generator=torch.Generator().manual_seed(2)) * qs).bfloat16()
+        pos = torch.tensor([196, 197, 198, 199], dtype=torch.int32)
+        sc = 128 ** -0.5 / (ks * qs)
+        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, scale=sc)
+        ref, tol = _attention64(val, q, pos + 1, torch.zeros(4), sc)
+        assert ((out.double().cpu() - ref).abs() <= tol).all()
+        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, scale=0.0)
+        ref, tol = _attention64(val, q, pos + 1, torch.zeros(4), 0.0)
+        assert ((out.double().cpu() - ref).abs() <= tol).all()
+        neg = ops.attention_q8((-q).to(DEV), c.kv, pos.to(DEV), True, 200, scale=-sc)
+        assert torch.equal(neg, ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, scale=sc))
+
+
+def _append64(qkv, pos, qn, kn, inv, Hq, Hkv, hd, rot, qs, eps):
+    x = qkv.double()
+    M = x.shape[0]
+    q = x[:, :Hq * qs].reshape(M, Hq, qs)[..., :hd] if Hq else x.new_zeros(M, 0, hd)
+    k = x[:, Hq * qs:Hq * qs + Hkv * hd].reshape(M, Hkv, hd)
+    v = x[:, Hq * qs + Hkv * hd:Hq * qs + 2 * Hkv * hd].reshape(M, Hkv, hd)
+    out = []
+    for y, w in ((q, qn), (k, kn)):
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * w.double()
+        ang = pos.double()[:, None] * inv.double()
+        c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+        a, b = y[..., :rot // 2], y[..., rot // 2:rot]
+        out.append(torch.cat([a * c - b * s, b * c + a * s, y[..., rot:]], -1))
+    return out[0], out[1], v
+
+
+@pytest.mark.parametrize("t", ["int8", "e4m3"])
+@pytest.mark.parametrize("M,Hq,Hkv,hd,rot,gated,page,do_q", [
+    (1, 1, 1, 64, 64, False, 0, True), (16, 32, 8, 128, 128, False, 64, True), (7, 24, 4, 256, 64, True, 0, True),
+    (33, 0, 3, 128, 128, False, 128, False), (5, 3, 2, 64, 16, False, 64, True), (130, 5, 1, 256, 256, False, 64, True),
+    (400, 32, 8, 128, 128, False, 64, True), (3, 4, 2, 128, 0, False, 0, True), (600, 6, 2, 64, 32, True, 0, True),
+])
+def test_append_matches_64_bits_and_reads_back(t, M, Hq, Hkv, hd, rot, gated, page, do_q):
+    from dflash_b200 import ops
+    g = torch.Generator().manual_seed(M)
+    qs = 2 * hd if gated else hd
+    qkv = torch.randn(M, Hq * qs + 2 * Hkv * hd + 8, generator=g).bfloat16()
+    qkv[0, -8 - hd:-8] = 0  # a value row of zeros
+    qn, kn = [(1 + 0.2 * torch.randn(hd, generator=g)).bfloat16() for _ in range(2)]
+    inv = (1e6 ** (-torch.arange(0, max(rot, 2), 2, dtype=torch.float64) / max(rot, 2))).float()
+    cap = 131072 if page == 64 and M == 16 else 1024
+    pos = torch.randperm(cap - 100, generator=g)[:M].to(torch.int32)
+    seq = torch.randint(0, 3, (M,), generator=g).to(torch.int32)
+    if M > 4:
+        pos[2] = -1
+    n_pages = 3 * cap // page if page else 3
+    shape = (n_pages, Hkv, page) if page else (3, Hkv, cap)
+    table = torch.randperm(n_pages, generator=g).to(torch.int32).view(3, -1).to(DEV) if page else None
+    codes = torch.full((2, *shape, hd), 0x55, dtype=torch.uint8, device=DEV).view(TYPES[t])
+    scale = torch.full((2, *shape), 77.0, device=DEV)
+    kv = ops.QuantKV(codes[0], codes[1], scale[0], scale[1], page_table=table, page_size=page)
+    q = torch.full((M, Hq, hd), 9.0, dtype=torch.bfloat16, device=DEV) if do_q else None
+    d = lambda x: x.to(DEV)  # noqa: E731
+    ops.qkv_rope_append_q8(d(qkv), d(pos), d(qn), d(kn), d(inv), kv, Hq, rot, 1e-6, q_out=q, row_seq=d(seq),
+                           q_stride=qs, do_q=do_q)
+    k, v = ops.kv_read_q8(kv, d(pos), row_seq=d(seq))
+    assert ops.device_error() == 0
+    live = pos >= 0
+    rq, rk, rv = _append64(qkv[:, :Hq * qs + 2 * Hkv * hd], pos, qn, kn, inv[:rot // 2], Hq, Hkv, hd, rot, qs, 1e-6)
+    if do_q:
+        err = (q.double().cpu() - rq).abs()[live]
+        assert (err <= 2.0 ** -8 * rq.abs()[live] + 2.0 ** -18 * rq.abs().amax(-1, keepdim=True)[live]).all()
+        assert (q.cpu()[~live] == 9).all()
+    if page:
+        at = table.cpu()[seq.long(), (pos // page).clamp_min(0).long()].long(), (pos % page).long()
+    else:
+        at = seq.long(), pos.long().clamp_min(0)
+    for i, (ref, back) in enumerate(((rk, k), (rv, v))):
+        s = scale[i].cpu()[at[0], :, at[1]].double()
+        amax = ref.abs().amax(-1)
+        assert ((s - amax / TOP[t]).abs()[live] <= 2.0 ** -18 * (amax / TOP[t])[live]).all()
+        held = codes[i].cpu().view(torch.uint8)[at[0], :, at[1]].view(TYPES[t]).double() * s[..., None]
+        half = 0.5 * s[..., None] if t == "int8" else 2.0 ** -4 * ref.abs() + 2.0 ** -10 * s[..., None]
+        assert ((held - ref).abs() <= half + 2.0 ** -18 * amax[..., None])[live].all()
+        # read-back: the held value rounded once
+        f32 = codes[i].cpu().view(torch.uint8)[at[0], :, at[1]].view(TYPES[t]).float() * s.float()[..., None]
+        assert torch.equal(back.cpu()[live], f32.bfloat16()[live])
+    # nothing but the rows named was written
+    touched = torch.zeros(shape, dtype=torch.bool)
+    touched[at[0][live], :, at[1][live]] = True
+    assert (scale.cpu()[:, ~touched] == 77).all()
+    assert (codes.cpu().view(torch.uint8)[:, ~touched] == 0x55).all()
+
+
+def test_rows_that_hold_infinities_or_nans_are_held_as_nan():
+    from dflash_b200 import ops
+    for t in TYPES:
+        codes = torch.zeros((2, 1, 2, 64, 128), dtype=torch.uint8, device=DEV).view(TYPES[t])
+        scale = torch.zeros((2, 1, 2, 64), device=DEV)
+        kv = ops.QuantKV(codes[0], codes[1], scale[0], scale[1])
+        qkv = torch.randn(3, 6 * 128).bfloat16()
+        qkv[0, 4 * 128 + 5] = math.inf   # value head 0 of row 0
+        qkv[1, 5 * 128 + 7] = math.nan   # value head 1 of row 1
+        qkv[2, 4 * 128 + 5] = -math.inf
+        w = torch.ones(128).bfloat16().to(DEV)
+        ops.qkv_rope_append_q8(qkv.to(DEV), torch.arange(3, dtype=torch.int32, device=DEV), w, w,
+                               torch.ones(64, device=DEV), kv, 2, 128, 1e-6)
+        bad = scale[1, 0, :, :3].isnan().cpu()
+        assert bad.tolist() == [[True, False, True], [False, True, False]]
+        assert (codes[1, 0].view(torch.uint8).cpu()[:, :3][bad] == 0).all()
+        k, v = ops.kv_read_q8(kv, torch.arange(3, dtype=torch.int32, device=DEV))
+        assert v[0, 0].isnan().all() and v[0, 1].isfinite().all() and k.isfinite().all()
+
+
+@pytest.mark.parametrize("page", [0, 64])
+def test_out_of_range_rows_are_refused_on_the_device(page):
+    """Positions, sequences and pages out of range are not accessed and set the error word; the other
+    rows of the call are served."""
+    from dflash_b200 import ops
+    c = Cache("int8", [100, 100], 2, 128, page, slack=28)
+    cap = c.kv.cap
+    q = torch.randn(2, 4, 128).bfloat16().to(DEV)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    assert ops.device_error() == 0
+    good = ops.attention_q8(q, c.kv, i32(50, 60), True, 100, row_seq=i32(0, 1), seq_rows=1)
+    out = torch.zeros_like(good)
+    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, row_seq=i32(0, 2), seq_rows=1, out=out)  # no sequence 2
+    assert ops.device_error() == 340 and torch.equal(out[0], good[0]) and (out[1] == 0).all()
+    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, row_seq=i32(0, 1), seq_rows=2, out=out)  # two in one run
+    assert ops.device_error() == 340 and torch.equal(out[0], good[0]) and (out[1] == 0).all()
+    ops.attention_q8(q, c.kv, i32(50, 1 << 30), True, 100, row_seq=i32(0, 1), seq_rows=1, out=out)
+    assert ops.device_error() == 341 and torch.equal(out[0], good[0])
+    before = c.codes.view(torch.uint8).clone()
+    qkv = torch.randn(2, 8 * 128).bfloat16().to(DEV)
+    w = torch.ones(128).bfloat16().to(DEV)
+    for pos, seq, code in ((i32(cap, cap + 5), i32(0, 1), 341), (i32(3, 4), i32(-1, 2), 340)):
+        ops.qkv_rope_append_q8(qkv, pos, w, w, torch.ones(64, device=DEV), c.kv, 4, 128, 1e-6, row_seq=seq)
+        assert ops.device_error() == code
+        ops.kv_read_q8(c.kv, pos, row_seq=seq)
+        assert ops.device_error() == code
+    if page:  # a table entry that is no page (the tables' last column holds -7)
+        pos = i32(cap - 1, cap - 2)
+        ops.qkv_rope_append_q8(qkv, pos, w, w, torch.ones(64, device=DEV), c.kv, 4, 128, 1e-6, row_seq=i32(0, 1))
+        assert ops.device_error() == 342
+        ops.attention_q8(q, c.kv, pos, True, cap, row_seq=i32(0, 1), seq_rows=1)
+        assert ops.device_error() == 342
+    assert torch.equal(before, c.codes.view(torch.uint8))
+
+
+def test_views_streams_and_graphs():
+    """Strided caches (one layer of a [seq, layer, ...] pool), strided outputs and gates, another
+    stream, and two captured graphs replayed out of order."""
+    from dflash_b200 import ops
+    g = torch.Generator().manual_seed(4)
+    B, L, Hkv, cap, hd, G = 3, 2, 2, 700, 128, 4
+    x = torch.randn((2, B, L, Hkv, cap, hd), generator=g)
+    codes, scale = _quantise(x, "int8")
+    val = codes.double() * scale.double()[..., None]
+    codes, scale = codes.to(DEV), scale.to(DEV)
+    kvs = [ops.QuantKV(codes[0][:, l], codes[1][:, l], scale[0][:, l], scale[1][:, l]) for l in range(L)]
+    M, Hq = B * 2, Hkv * G
+    q = torch.randn(M, Hq, hd, generator=g).bfloat16()
+    qkvg = torch.randn(M, 2 * Hq * hd, generator=g).bfloat16()
+    pos = torch.tensor([699, 698, 10, 11, 300, 301], dtype=torch.int32)
+    seq = torch.arange(B, dtype=torch.int32).repeat_interleave(2)
+    gate = qkvg.view(M, Hq, 2, hd)[:, :, 1].reshape(M, Hq * hd)
+    dq, dg, dp, ds = q.to(DEV), qkvg.to(DEV), pos.to(DEV), seq.to(DEV)
+    refs = [_attention64(val[:, :, l], q, pos + 1, seq, hd ** -0.5, gate) for l in range(L)]
+    outs = [torch.zeros(M, Hq * hd + 4, dtype=torch.bfloat16, device=DEV) for _ in range(L)]
+
+    def call(l):
+        ops.attention_q8(dq, kvs[l], dp, True, cap, row_seq=ds, seq_rows=2, key_chunk=128, out=outs[l][:, :Hq * hd],
+                         gate=dg[:, hd:], gate_head_stride=2 * hd)
+
+    def check():
+        for l, (ref, tol) in enumerate(refs):
+            assert ((outs[l][:, :Hq * hd].double().cpu() - ref).abs() <= tol).all()
+            assert (outs[l][:, Hq * hd:] == 0).all()
+            outs[l].zero_()
+
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        call(0)
+        call(1)
+    s.synchronize()
+    check()
+    graphs = []
+    for l in range(L):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            call(l)
+        graphs.append(gr)
+    for _ in range(3):  # side by side on two streams: no scratch is shared
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graphs[1].replay()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        check()
