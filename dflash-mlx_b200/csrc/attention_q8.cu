@@ -27,7 +27,7 @@
 //    bits; the sum of e_j uses the same M, which cancels in the quotient.
 // Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales,
 // codes or query products may be anything), so infinities and NaN there do not reach the row.
-#include "kv_q8.cuh"
+#include "attention_q8.cuh"
 
 #include <type_traits>
 
@@ -36,28 +36,7 @@ namespace dfl {
 constexpr int Q8_KB = 32;       // keys per block
 constexpr int Q8_STRANDS = 4;   // blocks in flight per chunk, each a warp of every row group
 constexpr int Q8_CHUNK_UNIT = Q8_KB * Q8_STRANDS;
-
-struct AttnQ8Args {
-  const __nv_bfloat16* q;  // [M][Hq][hd]
-  Q8Cache c;
-  const int* pos;
-  const int* row_seq;
-  const int* kv_len;
-  float* part_o;    // [chunks][M][Hq][hd]
-  float2* part_ml;  // [chunks][M][Hq]: (M, sum)
-  __nv_bfloat16* out;
-  long long ldo;
-  const __nv_bfloat16* gate;
-  long long ldg;
-  int gate_hs;
-  int M, Hq, G, causal, max_kv, n_chunks, key_chunk;
-  int run_rows;   // rows per run
-  int tile_toks;  // tokens per tile
-  int run_tiles;  // tiles per run
-  float scale_log2;  // |softmax scale| * log2(e); 1 when the scale is 0
-  float q_sign;      // sign of the softmax scale (0 when it is 0): folded into q
-  int* err;
-};
+constexpr int Q8_TC_CHUNK = 512;  // keys per chunk from which the tcgen05 form runs
 
 // ---- fp16 fragments ------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -68,42 +47,11 @@ __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// Four codes b0..b3 to two half2: (b0, b1), (b2, b3) with PAIRED (K: consecutive dims) or
-// (b0, b2), (b1, b3) without (V: the same dim of two keys).
-template <bool E4M3, bool PAIRED>
-__device__ __forceinline__ void q8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (E4M3) {
-    if (!PAIRED) w = __byte_perm(w, 0, 0x3120);
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
-    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
-  } else {
-    // fp16 0x6400 | u is 1024 + u; the biased byte u = c + 128
-    w ^= 0x80808080u;
-    lo = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4140 : 0x4240), 0x64806480u);
-    hi = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4342 : 0x4341), 0x64806480u);
-  }
-}
-
 // byte offset of 16-byte chunk c of key row r in a stage's [32][HD]-byte tile: ldmatrix reads the
 // same chunk of eight consecutive rows, which then lie in eight different 16-byte bank groups
 template <int HD>
 __device__ __forceinline__ int q8_swz(int r, int c) {
   return r * HD + ((HD == 64 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4);
-}
-
-// keys row m sees: clamped to what the cache and the call allow (an excess sets the error word)
-__device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, int seq, int* err) {
-  const long long lim = a.causal ? (long long)p + 1 : a.kv_len[seq];
-  const int most = min(a.max_kv, a.c.cap);
-  if (lim > most) q8_error(err, Q8_ERR_POS);
-  return lim > most ? most : lim < 0 ? 0 : (int)lim;
 }
 
 template <int HD, int MT, int RG, int ST>
@@ -573,6 +521,25 @@ __global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constan
   for (int i = 0; i < VEC; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(y[i], y[i + 1]);
 }
 
+template <int HD>
+static int launch_attn_q8_merge(const AttnQ8Args& a, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((long long)a.M * a.Hq + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<HD>, a);
+  if (e != cudaSuccess) {
+    set_error("dfl_attention_q8: merge launch failed: %s", cudaGetErrorString(e));
+    return DFL_ERR_CUDA;
+  }
+  return DFL_OK;
+}
+
 template <int HD, int MT, int RG, int ST, bool E4M3>
 static int launch_attn_q8(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   using L = AttnQ8Layout<HD, MT, RG, ST>;
@@ -598,14 +565,7 @@ static int launch_attn_q8(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_kernel<HD, MT, RG, ST, E4M3>, a);
-  if (e == cudaSuccess && a.n_chunks > 1) {
-    const long long items = (long long)a.M * a.Hq;
-    cfg.gridDim = dim3((unsigned)((items + 7) / 8));
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, attn_q8_merge_kernel<HD>, a);
-  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_kernel<HD, MT, RG, ST, E4M3>, a);
   if (e != cudaSuccess) {
     set_error("dfl_attention_q8: launch failed: %s", cudaGetErrorString(e));
     return DFL_ERR_CUDA;
@@ -702,10 +662,13 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
     set_error("%s: workspace missing, misaligned or too small (%zu < %zu)", who, workspace_bytes, need);
     return DFL_ERR_WORKSPACE;
   }
-  // rows a CTA takes: 16, 32 or (head_dim <= 128) 64 rows of (token, head) pairs
-  const int most = hd == 256 ? 32 : 64;
+  // long chunks take the tcgen05 form (the chunk size alone decides, so that calls to be
+  // compared bit for bit, which use one chunk size, use one form)
+  const bool tc = a.key_chunk >= Q8_TC_CHUNK;
+  // rows a CTA takes: 16, 32 or (tcgen05 form, or head_dim <= 128) 64 (token, head) pairs
+  const int most = hd == 256 && !tc ? 32 : 64;
   const long long want = (long long)run_rows * G;
-  const int rows = want <= 16 ? 16 : want <= 32 ? 32 : most;
+  const int rows = tc ? 64 : want <= 16 ? 16 : want <= 32 ? 32 : most;
   a.run_rows = run_rows;
   a.run_tiles = (run_rows + rows / G - 1) / (rows / G);
   a.tile_toks = (run_rows + a.run_tiles - 1) / a.run_tiles;
@@ -736,9 +699,16 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
   a.err = device_error_word();
   cudaStream_t st = as_stream(stream);
   const bool e4 = cache->type == DFL_KV_E4M3;
-  switch (hd) {
-    case 64: return e4 ? launch_attn_q8_rows<64, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<64, false>(a, rows, (int)tiles, st);
-    case 128: return e4 ? launch_attn_q8_rows<128, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<128, false>(a, rows, (int)tiles, st);
-    default: return e4 ? launch_attn_q8_rows<256, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<256, false>(a, rows, (int)tiles, st);
+  int status;
+  if (tc) {
+    status = launch_attention_q8_tc(a, hd, e4, (int)tiles, st);
+  } else if (hd == 64) {
+    status = e4 ? launch_attn_q8_rows<64, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<64, false>(a, rows, (int)tiles, st);
+  } else if (hd == 128) {
+    status = e4 ? launch_attn_q8_rows<128, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<128, false>(a, rows, (int)tiles, st);
+  } else {
+    status = e4 ? launch_attn_q8_rows<256, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<256, false>(a, rows, (int)tiles, st);
   }
+  if (status != DFL_OK || a.n_chunks == 1) return status;
+  return hd == 64 ? launch_attn_q8_merge<64>(a, st) : hd == 128 ? launch_attn_q8_merge<128>(a, st) : launch_attn_q8_merge<256>(a, st);
 }

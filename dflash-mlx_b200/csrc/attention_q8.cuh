@@ -1,0 +1,64 @@
+// What the two forms of the attention over an 8-bit cache share (attention_q8.cu,
+// attention_q8_tc.cu): arguments, code conversion and row limits.
+#pragma once
+#include "kv_q8.cuh"
+
+namespace dfl {
+
+struct AttnQ8Args {
+  const __nv_bfloat16* q;  // [M][Hq][hd]
+  Q8Cache c;
+  const int* pos;
+  const int* row_seq;
+  const int* kv_len;
+  float* part_o;    // [chunks][M][Hq][hd]
+  float2* part_ml;  // [chunks][M][Hq]: (M, sum)
+  __nv_bfloat16* out;
+  long long ldo;
+  const __nv_bfloat16* gate;
+  long long ldg;
+  int gate_hs;
+  int M, Hq, G, causal, max_kv, n_chunks, key_chunk;
+  int run_rows;   // rows per run
+  int tile_toks;  // tokens per tile
+  int run_tiles;  // tiles per run
+  float scale_log2;  // |softmax scale| * log2(e); 1 when the scale is 0
+  float q_sign;      // sign of the softmax scale (0 when it is 0): folded into q
+  int* err;
+};
+
+__device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Four codes b0..b3 to two half2: (b0, b1), (b2, b3) with PAIRED (K: consecutive dims) or
+// (b0, b2), (b1, b3) without (V: the same dim of two keys).
+template <bool E4M3, bool PAIRED>
+__device__ __forceinline__ void q8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (E4M3) {
+    if (!PAIRED) w = __byte_perm(w, 0, 0x3120);
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
+    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
+  } else {
+    // fp16 0x6400 | u is 1024 + u; the biased byte u = c + 128
+    w ^= 0x80808080u;
+    lo = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4140 : 0x4240), 0x64806480u);
+    hi = hsub2_u32(__byte_perm(w, 0x64646464u, PAIRED ? 0x4342 : 0x4341), 0x64806480u);
+  }
+}
+
+// keys row m sees: clamped to what the cache and the call allow (an excess sets the error word)
+__device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, int seq, int* err) {
+  const long long lim = a.causal ? (long long)p + 1 : a.kv_len[seq];
+  const int most = min(a.max_kv, a.c.cap);
+  if (lim > most) q8_error(err, Q8_ERR_POS);
+  return lim > most ? most : lim < 0 ? 0 : (int)lim;
+}
+
+// The tcgen05 form (attention_q8_tc.cu): the chunk kernel alone.
+int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int tiles, cudaStream_t st);
+
+}  // namespace dfl
