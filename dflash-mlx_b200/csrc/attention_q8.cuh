@@ -38,10 +38,9 @@ template <bool E4M3, bool PAIRED>
 __device__ __forceinline__ void q8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (E4M3) {
     if (!PAIRED) w = __byte_perm(w, 0, 0x3120);
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    lo = (uint32_t)a.x | ((uint32_t)a.y << 16);
-    hi = (uint32_t)b.x | ((uint32_t)b.y << 16);
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   } else {
     // fp16 0x6400 | u is 1024 + u; the biased byte u = c + 128
     w ^= 0x80808080u;

@@ -16,8 +16,8 @@
 // bandwidth (fp16 tiles written once and read once by the MMA: 8 bytes per code) is what this form
 // is closest to.
 // A row's exponent base M follows its maximum lazily: sums, weights and O are rescaled only when
-// M would grow by more than 4 (log2), so weights stay below 2^15 in fp16 and those down to 2^-25 of the
-// largest keep all their bits (those below are rounded to multiples of 2^-35 of it).
+// M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to 2^-18 of
+// the largest keep all their bits (those below are rounded to multiples of 2^-28 of it).
 // Every wait is bounded (device error 350-359).
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
@@ -29,7 +29,7 @@ constexpr int QT_ROWS = 64;     // (token, head) rows per tile
 constexpr int QT_THREADS = 288;
 constexpr int QT_SCALES = 4;    // scale ring: block i's are read until its weights are written
 constexpr int QT_AHEAD = 4;     // blocks prefetched into L2
-constexpr float QT_BASE = 10.f, QT_LAZY = 4.f;
+constexpr float QT_BASE = 4.f, QT_LAZY = 10.f;
 
 template <int HD>
 struct QtLayout {
@@ -79,6 +79,56 @@ __device__ __forceinline__ void tc_st16_nowait(uint32_t taddr, const uint32_t (&
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
+// Bounded wait that sleeps in the barrier unit (1 ms a try) instead of spending issue slots
+__device__ __forceinline__ bool qt_wait(uint64_t* bar, uint32_t parity, int site, int* err) {
+  const uint32_t addr = smem_u32(bar);
+  for (int n = 0; n < 2000; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+  }
+  q8_error(err, site);
+  return false;
+}
+
+// 2^x, results below the normal range flushed to zero (fp16 weights and their sum lose nothing)
+__device__ __forceinline__ float qt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two fp32 operations an instruction
+__device__ __forceinline__ uint64_t qt_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 qt_unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t qt_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t qt_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t qt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // 16-byte chunk c of row r of a [rows][128 B] 128-byte-swizzled unit
 __device__ __forceinline__ uint32_t qt_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -98,9 +148,9 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + QT_ROWS;
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + QT_ROWS * 8);  // [128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* k_full = bars;        // [2] 128 converter arrivals
+  uint64_t* k_full = bars;        // [2] 64 converter arrivals
   uint64_t* k_empty = bars + 2;   // [2] MMA commit
-  uint64_t* v_full = bars + 4;    // [2] 128 converter arrivals
+  uint64_t* v_full = bars + 4;    // [2] 64 converter arrivals
   uint64_t* v_empty = bars + 6;   // [2] MMA commit
   uint64_t* s_full = bars + 8;    // [2] MMA commit
   uint64_t* p_full = bars + 10;   // [2] 128 softmax arrivals: weights written (and S consumed)
@@ -108,6 +158,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   uint64_t* sc_full = bars + 14;  // [QT_SCALES] 128 converter arrivals
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::N_BAR);
   __shared__ int s_tok_lim[QT_ROWS], s_tok_ok[QT_ROWS];
+  __shared__ int s_row[QT_ROWS];  // token * 16 + head in group of each tile row, -1 behind the last
 
   grid_dependency_wait();
   const int run = blockIdx.x / a.run_tiles, tile = blockIdx.x % a.run_tiles, kvh = blockIdx.y, chunk = blockIdx.z;
@@ -115,247 +166,290 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   const int m0 = run * a.run_rows + tile * a.tile_toks;
   const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
   if (ntok <= 0) return;
-  int seq = -1;  // of the tile's first row with a position
-  for (int i = 0; i < ntok && seq < 0; ++i)
-    if (a.pos[m0 + i] >= 0) seq = a.row_seq ? a.row_seq[m0 + i] : 0;
-  if (seq < 0 || seq >= a.c.n_seqs) {
-    if (seq >= 0 && threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
+  // the tile's rows, two a lane, by every warp alike: their positions and sequences, the run's sequence
+  // (that of the first row with a position), limits
+  int pos2[2], sq2[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = lane + 32 * k;
+    pos2[k] = i < ntok ? a.pos[m0 + i] : -1;
+    sq2[k] = i < ntok && a.row_seq ? a.row_seq[m0 + i] : 0;
+  }
+  const unsigned v0 = __ballot_sync(0xffffffffu, pos2[0] >= 0), v1 = __ballot_sync(0xffffffffu, pos2[1] >= 0);
+  if (!(v0 | v1)) return;
+  const int seq = __shfl_sync(0xffffffffu, v0 ? sq2[0] : sq2[1], __ffs(v0 ? v0 : v1) - 1);
+  if (seq < 0 || seq >= a.c.n_seqs) {  // a row that names no sequence of the cache is left as it is
+    if (threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
     return;
   }
-  if (threadIdx.x < ntok) {
-    const int m = m0 + threadIdx.x, p = a.pos[m];
-    int lim = 0, ok = p >= 0;
-    if (ok && a.row_seq && a.row_seq[m] != seq) {
-      q8_error(a.err, Q8_ERR_SEQ);
-      ok = 0;
-    }
-    if (ok) lim = q8_row_limit(a, m, p, seq, chunk == 0 && kvh == 0 ? a.err : nullptr);
-    s_tok_lim[threadIdx.x] = lim;
-    s_tok_ok[threadIdx.x] = ok;
-  }
-  __syncthreads();
   int lim_max = 0, lim_min = 0x7fffffff;
-  for (int i = 0; i < ntok; ++i) {
-    const int lim = s_tok_lim[i];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = lane + 32 * k;
+    const bool ok = pos2[k] >= 0 && sq2[k] == seq;
+    if (warp == 0 && pos2[k] >= 0 && !ok) q8_error(a.err, Q8_ERR_SEQ);
+    const int lim = ok ? q8_row_limit(a, m0 + i, pos2[k], seq, warp == 0 && chunk == 0 && kvh == 0 ? a.err : nullptr) : 0;
+    if (warp == 0) {
+      s_tok_lim[i] = lim;
+      s_tok_ok[i] = ok;
+    }
     lim_max = max(lim_max, lim);
     if (lim > 0) lim_min = min(lim_min, lim);
   }
+  lim_max = __reduce_max_sync(0xffffffffu, lim_max);
+  lim_min = __reduce_min_sync(0xffffffffu, lim_min);
   const int k_begin = chunk * a.key_chunk;
   if (k_begin >= lim_max && a.n_chunks > 1) return;
   const int k_end = min(k_begin + a.key_chunk, lim_max);
   const int n_blocks = (max(k_end - k_begin, 0) + QT_KB - 1) / QT_KB;
-
   if (threadIdx.x == 256) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 128);
+      mbar_init(&k_full[s], 64);
       mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 128);
+      mbar_init(&v_full[s], 64);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s], ntok * a.G > 32 ? 128 : 64);
       mbar_init(&pv_done[s], 1);
     }
     for (int s = 0; s < QT_SCALES; ++s) mbar_init(&sc_full[s], 128);
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (threadIdx.x >= 128 && threadIdx.x < 128 + QT_ROWS) {
+    const int r = threadIdx.x - 128, tok = r / a.G;
+    s_row[r] = tok < ntok ? tok * 16 + r - tok * a.G : -1;
+  }
+  __syncthreads();
+  const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+  if (warp >= 4 && warp < 8) {
+    // ---------------- converters: warps 4-5 K, 6-7 V ----------------
+    constexpr int NC = HD / 16;            // 16-code chunks per key
+    constexpr int PER = QT_KB * NC / 64;   // chunks per thread and block
+    const int ct = threadIdx.x & 63;
+    const bool is_v = warp >= 6;
+    const unsigned char* src = (is_v ? a.c.v : a.c.k) + kvh * a.c.head_stride;
+    const float* ssrc = (is_v ? a.c.vs : a.c.ks) + kvh * a.c.s_head_stride + ct;
+    unsigned char* dst = smem + (is_v ? L::OFF_V : L::OFF_K);
+    float* sdst = s_sc + (is_v ? QT_KB : 0) + ct;
+    uint64_t* full = is_v ? v_full : k_full;
+    uint64_t* empty = is_v ? v_empty : k_empty;
+    // A thread's chunk column c and rows r, r + STEP, ... Lane bits: two of the chunk, one of the row,
+    // the rest of the chunk, the rest of the row: the eight lanes of a 16-byte store phase write two
+    // rows' chunks of one unit, eight different bank groups. STEP is a multiple of 4; for head_dim 256
+    // odd multiples flip the swizzle's third bit.
+    constexpr int HI = NC / 4, STEP = 64 / NC;
+    const int c = (ct & 3) | (((ct >> 3) & (HI - 1)) << 2);
+    const int r = ((ct >> 2) & 1) | ((ct / (8 * HI)) << 1);
+    const uint32_t dst0 = (uint32_t)(c >> 2) * (QT_KB * 128) + qt_sw(r, (c & 3) * 2);
+    src += c * 16;
+    // Places of 32 blocks, one a lane, read together: a table lookup per block would stand in front of
+    // the block's loads.
+    int win = 0, win_page = -1;
+    auto window = [&](int i) {
+      long long page = -1;
+      int row;
+      win = i;
+      if (i + lane < n_blocks && !q8_place(a.c, seq, k_begin + (i + lane) * QT_KB, warp == 4 ? a.err : nullptr, page, row))
+        page = -1;
+      win_page = (int)page;
+    };
+    // block i's codes and scale offsets and keys (0 behind the last block, or when its place is refused)
+    auto where = [&](int i, long long& off, long long& soff) -> int {
+      const long long page = __shfl_sync(0xffffffffu, win_page, i - win);
+      const int kb = k_begin + i * QT_KB;
+      const int row = a.c.page_table ? kb & ((1 << a.c.page_shift) - 1) : kb;
+      off = soff = 0;
+      if (page < 0) return 0;
+      off = page * a.c.seq_stride + (long long)row * HD;
+      soff = page * a.c.s_seq_stride + row;
+      return min(QT_KB, k_end - kb);
+    };
+    uint4 b[PER];
+    // The thread's chunks of a block of n keys at p: volatile, so that the loads are issued here, most of
+    // a block's time ahead of their use. Rows behind the last key repeat it: their scores are masked,
+    // their weights 0, and a code is a finite number.
+    auto fetch = [&](const unsigned char* p, int n) {
+      if (n == QT_KB) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+          asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(b[u].x), "=r"(b[u].y), "=r"(b[u].z), "=r"(b[u].w)
+                       : "l"(p + (r + u * STEP) * HD));
+      } else if (n > 0) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+          asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(b[u].x), "=r"(b[u].y), "=r"(b[u].z), "=r"(b[u].w)
+                       : "l"(p + min(r + u * STEP, n - 1) * HD));
+      } else {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) b[u] = make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto prefetch = [&](int i) {  // a block into L2, by the thread whose src is the matrix's start
+      long long o, so;
+      const int n = where(i, o, so);
+      if (ct == 0 && n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(src + o), "r"(n * HD) : "memory");
+    };
+    long long off, soff;
+    window(0);
+    int n = where(0, off, soff);
+    fetch(src + off, n);
+    float scale = ct < n ? __ldg(ssrc + soff) : 0.f;
+    for (int i = 1; i < QT_AHEAD; ++i) prefetch(i);
+    for (int i = 0; i < n_blocks; ++i) {
+      const int s = i & 1;
+      if (i + QT_AHEAD - win >= 32) window(i + 1);
+      n = where(i + 1, off, soff);
+      prefetch(i + QT_AHEAD);
+      if (!qt_wait(&empty[s], ((i >> 1) & 1) ^ 1, 350, a.err)) break;
+      sdst[(i & (QT_SCALES - 1)) * 2 * QT_KB] = scale;
+      mbar_arrive(&sc_full[i & (QT_SCALES - 1)]);
+      unsigned char* d = dst + s * L::TILE + dst0;
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        uint4 h0, h1;
+        q8_to_half<E4M3, true>(b[u].x, h0.x, h0.y);
+        q8_to_half<E4M3, true>(b[u].y, h0.z, h0.w);
+        q8_to_half<E4M3, true>(b[u].z, h1.x, h1.y);
+        q8_to_half<E4M3, true>(b[u].w, h1.z, h1.w);
+        // the chunk's second half lies at its first's address with bit 4 flipped
+        const uint32_t flip = STEP % 8 ? (u & 1) << 6 : 0;
+        unsigned char* du = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(d) ^ flip) + u * STEP * 128;
+        *reinterpret_cast<uint4*>(du) = h0;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(du) ^ 16) = h1;
+      }
+      fetch(src + off, n);
+      scale = ct < n ? __ldg(ssrc + soff) : 0.f;
+      fence_proxy_async_smem();
+      mbar_arrive(&full[s]);
+    }
+  } else if (warp == 8) {
+    // ---------------- MMA issuer ----------------
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
                  "n"(L::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
-  }
-  // Q rows to scaled fp16, twice (softmax warps); a row's factor undoes its power of two
-  if (warp < 4) {
-    constexpr int VEC = HD / 32;
-    for (int r = warp; r < QT_ROWS; r += 4) {
-      const int tok = r / a.G, hg = r % a.G;
-      const bool ok = tok < ntok && s_tok_lim[min(tok, ntok - 1)] > 0;
-      const __nv_bfloat16* src = a.q + ((long long)(ok ? m0 + tok : m0) * a.Hq + kvh * a.G + (ok ? hg : 0)) * HD;
-      uint32_t u[VEC / 2];
-      if constexpr (VEC == 2) {
-        u[0] = reinterpret_cast<const uint32_t*>(src)[lane];
-      } else if constexpr (VEC == 4) {
-        const uint2 w = reinterpret_cast<const uint2*>(src)[lane];
-        u[0] = w.x, u[1] = w.y;
-      } else {
-        const uint4 w = reinterpret_cast<const uint4*>(src)[lane];
-        u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
-      }
-      float x[VEC], mx = 0.f;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        x[j] = !ok ? 0.f : __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
-        mx = fmaxf(mx, fabsf(x[j]));
-      }
-      mx = warp_max(mx);
-      int sh = 0;
-      if (mx > 0.f && mx < INFINITY) sh = min(14 - ((int)(__float_as_uint(mx) >> 23) - 127), 120);
-      const float f = __uint_as_float((uint32_t)(sh + 127) << 23) * a.q_sign;
-#pragma unroll
-      for (int j = 0; j < VEC; j += 2) {
-        const int d = lane * VEC + j;
-        const __half2 h = __floats2half2_rn(x[j] * f, x[j + 1] * f);
-        unsigned char* dst = smem + L::OFF_Q + (d >> 6) * 16384 + ((d & 7) << 1);
-        *reinterpret_cast<__half2*>(dst + qt_sw(r, (d & 63) >> 3)) = h;
-        *reinterpret_cast<__half2*>(dst + qt_sw(r + QT_ROWS, (d & 63) >> 3)) = h;
-      }
-      if (lane == 0) {
-        s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
-        s_lim[r] = ok ? s_tok_lim[tok] : 0;
-      }
-    }
-  }
-  fence_proxy_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  grid_dependency_launch_dependents();  // after the TMEM allocation: a dependent's must not come before it
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t t_o = tmem + 128;  // S / weights: columns 0-63, 64-127
-
-  if (warp >= 4 && warp < 8) {
-    // ---------------- converters ----------------
-    constexpr int NC = HD / 16;                 // 16-code chunks per key
-    constexpr int PER = QT_KB * NC / 128;       // chunks per thread and matrix
-    const int ct = threadIdx.x - 128;
-    const unsigned char* Kh = a.c.k + kvh * a.c.head_stride;
-    const unsigned char* Vh = a.c.v + kvh * a.c.head_stride;
-    const float* Sh = (ct < QT_KB ? a.c.ks : a.c.vs) + kvh * a.c.s_head_stride;
-    // Lane bits: two of the chunk, one of the row, the rest of the chunk, the rest of the row: the eight
-    // lanes of a 16-byte store phase write two rows' chunks of one unit, eight different bank groups.
-    auto place = [&](int u, int& r, int& c) {
-      const int idx = ct + u * 128;
-      constexpr int HI = NC / 4;  // units
-      c = (idx & 3) | (((idx >> 3) & (HI - 1)) << 2);
-      r = ((idx >> 2) & 1) | ((idx / (8 * HI)) << 1);
-    };
-    struct Block {
-      uint4 k[PER], v[PER];
-      float s;
-    };
-    auto locate = [&](int i, long long& page, int& row) -> bool {
-      return q8_place(a.c, seq, k_begin + i * QT_KB, ct == 0 ? a.err : nullptr, page, row);
-    };
-    auto prefetch = [&](int i) {  // both matrices' rows of block i, one bulk prefetch each
-      long long page;
-      int row;
-      if (i >= n_blocks || ct >= 2 || !locate(i, page, row)) return;
-      const int n = min(QT_KB, k_end - (k_begin + i * QT_KB));
-      const unsigned char* p = (ct ? Vh : Kh) + page * a.c.seq_stride + (long long)row * HD;
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(p), "r"(n * HD) : "memory");
-    };
-    auto fetch = [&](int i, Block& b) {
-      long long page;
-      int row;
-      const bool ok = locate(i, page, row);
-      const int n = ok ? min(QT_KB, k_end - (k_begin + i * QT_KB)) : 0;
-      const long long off = ok ? page * a.c.seq_stride + (long long)row * HD : 0;
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        int r, c;
-        place(u, r, c);
-        b.k[u] = b.v[u] = make_uint4(0, 0, 0, 0);
-        if (r < n) {
-          b.k[u] = __ldg(reinterpret_cast<const uint4*>(Kh + off + r * HD + c * 16));
-          b.v[u] = __ldg(reinterpret_cast<const uint4*>(Vh + off + r * HD + c * 16));
-        }
-      }
-      b.s = (ct & 63) < n ? __ldg(Sh + page * a.c.s_seq_stride + row + (ct & 63)) : 0.f;
-    };
-    auto convert = [&](const uint4& w, unsigned char* dst, int r, int c) {
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-      uint32_t h[8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) q8_to_half<E4M3, true>(x[q], h[2 * q], h[2 * q + 1]);
-      unsigned char* d = dst + (c >> 2) * (QT_KB * 128);
-      *reinterpret_cast<uint4*>(d + qt_sw(r, (c & 3) * 2)) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(d + qt_sw(r, (c & 3) * 2 + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-    };
-    Block nxt;
-    for (int i = 1; i <= QT_AHEAD; ++i) prefetch(i);
-    if (n_blocks > 0) fetch(0, nxt);
-    for (int i = 0; i < n_blocks; ++i) {
-      const int s = i & 1;
-      const Block cur = nxt;
-      if (i + 1 < n_blocks) {
-        prefetch(i + 1 + QT_AHEAD);
-        fetch(i + 1, nxt);
-      }
-      if (!mbar_wait(&k_empty[s], ((i >> 1) & 1) ^ 1, 350, a.err)) break;
-      s_sc[(i & (QT_SCALES - 1)) * 2 * QT_KB + ct] = cur.s;
-      mbar_arrive(&sc_full[i & (QT_SCALES - 1)]);
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        int r, c;
-        place(u, r, c);
-        convert(cur.k[u], smem + L::OFF_K + s * L::TILE, r, c);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&k_full[s]);
-      if (!mbar_wait(&v_empty[s], ((i >> 1) & 1) ^ 1, 351, a.err)) break;
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        int r, c;
-        place(u, r, c);
-        convert(cur.v[u], smem + L::OFF_V + s * L::TILE, r, c);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&v_full[s]);
-    }
-  } else if (warp == 8) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      const uint32_t q0 = smem_u32(smem + L::OFF_Q);
-      auto pv = [&](int j) -> bool {
-        const int s = j & 1;
-        if (!mbar_wait(&p_full[s], (j >> 1) & 1, 352, a.err)) return false;
-        if (!mbar_wait(&v_full[s], (j >> 1) & 1, 353, a.err)) return false;
-        tc_fence_after();
-        const uint32_t vb = smem_u32(smem + L::OFF_V + s * L::TILE);
+    tc_fence_before();
+    asm volatile("bar.sync 2, 160;\n" ::: "memory");  // Q written, TMEM allocated
+    tc_fence_after();
+    grid_dependency_launch_dependents();  // not before the allocation: a dependent's must not come first
+    const uint32_t tmem = *tmem_slot, t_o = tmem + 128;  // S / weights: columns 0-63, 64-127
+    // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
+    const bool leader = lane == 0;
+    const uint64_t qd = sw128_desc(smem_u32(smem + L::OFF_Q));
+    const uint64_t kd0 = sw128_desc(smem_u32(smem + L::OFF_K));
+    const uint64_t vd0 = sw128_mn_desc(smem_u32(smem + L::OFF_V), QT_KB * 128, 1024);
+    auto pv = [&](int j) -> bool {
+      const int s = j & 1;
+      if (!qt_wait(&p_full[s], (j >> 1) & 1, 352, a.err)) return false;
+      if (!qt_wait(&v_full[s], (j >> 1) & 1, 353, a.err)) return false;
+      tc_fence_after();
+      if (leader) {
+        const uint64_t vd = vd0 + s * (L::TILE >> 4);
+        const uint32_t tw = tmem + s * 64;
 #pragma unroll
         for (int kk = 0; kk < QT_KB / 16; ++kk)
-          tc_mma_ts(t_o, tmem + s * 64 + kk * 8, sw128_mn_desc(vb + kk * 2048, QT_KB * 128, 1024), qt_idesc(HD, true),
-                    j > 0 || kk > 0 ? 1u : 0u);
+          tc_mma_ts(t_o, tw + kk * 8, vd + kk * (2048 >> 4), qt_idesc(HD, true), j > 0 || kk > 0 ? 1u : 0u);
         tc_commit(&v_empty[s]);
         tc_commit(&pv_done[s]);
-        return true;
-      };
-      bool ok = true;
-      for (int i = 0; i < n_blocks && ok; ++i) {
-        const int s = i & 1;
-        if (!mbar_wait(&k_full[s], (i >> 1) & 1, 354, a.err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        // S of block i overwrites the weights of block i - 2, whose product was issued before it
-        const uint32_t kt = smem_u32(smem + L::OFF_K + s * L::TILE);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          tc_mma(tmem + s * 64, sw128_desc(q0 + (kk >> 2) * 16384) + 2 * (kk & 3),
-                 sw128_desc(kt + (kk >> 2) * (QT_KB * 128)) + 2 * (kk & 3), qt_idesc(QT_KB, false), kk > 0 ? 1u : 0u);
-        tc_commit(&k_empty[s]);
-        tc_commit(&s_full[s]);
-        if (i > 0) ok = pv(i - 1);
       }
-      if (ok && n_blocks > 0) pv(n_blocks - 1);
-    }
-    __syncwarp();
-  } else if (warp < 4) {
-    // ---------------- softmax: thread = (row, copy) ----------------
-    const int row = threadIdx.x & 63, half = threadIdx.x >> 6;
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    const int lim = s_lim[row];
-    const float rowf = s_rowf[row];
-    float m = -INFINITY, mu_used = -INFINITY, l = 0.f;
-    int er = -90;
+      __syncwarp();
+      return true;
+    };
     bool ok = true;
     for (int i = 0; i < n_blocks && ok; ++i) {
       const int s = i & 1;
+      if (!qt_wait(&k_full[s], (i >> 1) & 1, 354, a.err)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (leader) {
+        // S of block i overwrites the weights of block i - 2, whose product was issued before it
+        const uint64_t kd = kd0 + s * (L::TILE >> 4);
+        const uint32_t ts = tmem + s * 64;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+          tc_mma(ts, qd + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (QT_KB * 128 >> 4) + 2 * (kk & 3),
+                 qt_idesc(QT_KB, false), kk > 0 ? 1u : 0u);
+        tc_commit(&k_empty[s]);
+        tc_commit(&s_full[s]);
+      }
+      __syncwarp();
+      if (i > 0) ok = pv(i - 1);
+    }
+    if (ok && n_blocks > 0) pv(n_blocks - 1);
+  } else if (warp < 4) {
+    // ---------------- softmax: thread = (row, copy) ----------------
+    // Q rows to scaled fp16, twice; a row's factor undoes its power of two. hd / 16 lanes a row, 16
+    // dims each; a rolled loop, since code that runs once a CTA comes from a cold instruction cache.
+    {
+      constexpr int LPR = HD / 16, RPW = 32 / LPR;
+      const int ql = lane % LPR;
+      uint4 nx[2];
+      auto qload = [&](int r) {
+        const int th = r < QT_ROWS ? s_row[r] : -1;
+        nx[0] = nx[1] = make_uint4(0, 0, 0, 0);
+        if (th >= 0 && s_tok_lim[th >> 4] > 0) {
+          const uint4* q = reinterpret_cast<const uint4*>(
+              a.q + ((long long)(m0 + (th >> 4)) * a.Hq + kvh * a.G + (th & 15)) * HD + ql * 16);
+          nx[0] = q[0];
+          nx[1] = q[1];
+        }
+      };
+      qload(warp * RPW + lane / LPR);
+#pragma unroll 1
+      for (int r = warp * RPW + lane / LPR; r < QT_ROWS; r += 4 * RPW) {
+        const uint32_t u[8] = {nx[0].x, nx[0].y, nx[0].z, nx[0].w, nx[1].x, nx[1].y, nx[1].z, nx[1].w};
+        qload(r + 4 * RPW);
+        // magnitudes compare as integers; one that is not finite leaves the row unscaled
+        uint32_t mx = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = max(mx, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int sh = mx > 0 && mx < 0x7f800000u ? min(14 - ((int)(mx >> 23) - 127), 120) : 0;
+        const float f = __uint_as_float((uint32_t)(sh + 127) << 23) * a.q_sign;
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __half2 y = __floats2half2_rn(__uint_as_float(u[j] << 16) * f, __uint_as_float(u[j] & 0xffff0000u) * f);
+          h[j] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        unsigned char* d = smem + L::OFF_Q + (ql >> 2) * 16384 + qt_sw(r, (ql & 3) * 2);
+#pragma unroll
+        for (int copy = 0; copy < 2; ++copy, d += QT_ROWS * 128) {
+          *reinterpret_cast<uint4*>(d) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d) ^ 16) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+        if (ql == 0) {
+          s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
+          s_lim[r] = s_row[r] < 0 ? 0 : s_tok_lim[s_row[r] >> 4];
+        }
+      }
+    }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    asm volatile("bar.sync 2, 160;\n" ::: "memory");
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot, t_o = tmem + 128;
+    const int row = threadIdx.x & 63, half = threadIdx.x >> 6;
+    const int lim = s_lim[row];
+    const float rowf = s_rowf[row];
+    float m = -INFINITY, mu_used = -INFINITY;
+    uint64_t l = 0;  // two partial sums
+    int er = -90;
+    bool ok = true;
+    // a warp whose 32 rows all lie behind the tile's does nothing: what its lanes hold goes to its own
+    // rows of O, which nobody reads
+    const int my_blocks = (row & 32) < ntok * a.G ? n_blocks : 0;
+    for (int i = 0; i < my_blocks && ok; ++i) {
+      const int s = i & 1;
       const float* sc = s_sc + (i & (QT_SCALES - 1)) * 2 * QT_KB + half * 32;
       const int kb = k_begin + i * QT_KB + half * 32;
-      ok = mbar_wait(&sc_full[i & (QT_SCALES - 1)], (i / QT_SCALES) & 1, 355, a.err) &&
-           mbar_wait(&s_full[s], (i >> 1) & 1, 356, a.err);
+      ok = qt_wait(&sc_full[i & (QT_SCALES - 1)], (i / QT_SCALES) & 1, 355, a.err) &&
+           qt_wait(&s_full[s], (i >> 1) & 1, 356, a.err);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -364,77 +458,82 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       float sv[32];
       tc_ld32(tmem + lane_base + (uint32_t)(s * 64 + half * 32), sv);
       const bool full = kb + 32 <= lim_min;
-      float mx = -INFINITY;
-      uint32_t vm = 0;
+      uint64_t x[16];
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 ks = *reinterpret_cast<const float4*>(sc + c);
-        sv[c] *= ks.x;
-        sv[c + 1] *= ks.y;
-        sv[c + 2] *= ks.z;
-        sv[c + 3] *= ks.w;
+      for (int c = 0; c < 16; c += 2) {
+        const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + 2 * c);
+        x[c] = qt_mul2(qt_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
+        x[c + 1] = qt_mul2(qt_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
       }
+      uint32_t vm = __float_as_uint(sc[QT_KB + lane]) & 0x7fffffffu;
       if (full) {
-        const uint32_t b = __float_as_uint(sc[QT_KB + lane]) & 0x7fffffffu;
-        vm = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
+        vm = __reduce_max_sync(0xffffffffu, vm < 0x7f800000u ? vm : 0u);
       } else {
+        vm = 0;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const bool seen = kb + c < lim;
-          sv[c] = seen ? sv[c] : -INFINITY;
-          const uint32_t b = __float_as_uint(sc[QT_KB + c]) & 0x7fffffffu;
-          if (seen && b < 0x7f800000u) vm = max(vm, b);
+        for (int c = 0; c < 16; ++c) {
+          const float2 y = qt_unpack(x[c]);
+          const bool seen0 = kb + 2 * c < lim, seen1 = kb + 2 * c + 1 < lim;
+          x[c] = qt_pack(seen0 ? y.x : -INFINITY, seen1 ? y.y : -INFINITY);
+          const uint2 v = *reinterpret_cast<const uint2*>(sc + QT_KB + 2 * c);
+          const uint32_t v0 = v.x & 0x7fffffffu, v1 = v.y & 0x7fffffffu;
+          if (seen0 && v0 < 0x7f800000u) vm = max(vm, v0);
+          if (seen1 && v1 < 0x7f800000u) vm = max(vm, v1);
         }
       }
+      float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 32; ++c) mx = fmaxf(mx, sv[c]);
-      m = fmaxf(m, mx * rowf);
+      for (int c = 0; c < 16; c += 2) {
+        const float2 y = qt_unpack(x[c]), z = qt_unpack(x[c + 1]);
+        mx0 = fmaxf(fmaxf(mx0, y.x), y.y);
+        mx1 = fmaxf(fmaxf(mx1, z.x), z.y);
+      }
+      m = fmaxf(m, fmaxf(mx0, mx1) * rowf);
       er = max(er, (int)(vm >> 23) - 127);
       const float M = m + ((float)er - QT_BASE);
       const bool grow = M > mu_used + QT_LAZY || (mu_used == -INFINITY && M > -INFINITY);
-      const float fac = grow ? exp2f(mu_used - M) : 1.f;
-      if (grow) {
-        mu_used = M;
-        l *= fac;
-      }
-      if (i > 0 && __any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
-        ok = mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 357, a.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      if (__any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
+        const float fac = grow ? qt_exp2(mu_used - M) : 1.f;
+        if (grow) mu_used = M;
+        l = qt_mul2(l, qt_pack(fac, fac));
+        if (i > 0) {
+          ok = qt_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 357, a.err);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
-          float ov[16];
-          tc_ld16(t_o + lane_base + (uint32_t)c, ov);
+          for (int c = 0; c < HD; c += 16) {
+            float ov[16];
+            tc_ld16(t_o + lane_base + (uint32_t)c, ov);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ov[e] *= fac;
-          tc_st16(t_o + lane_base + (uint32_t)c, ov);
+            for (int e = 0; e < 16; ++e) ov[e] *= fac;
+            tc_st16(t_o + lane_base + (uint32_t)c, ov);
+          }
         }
       }
       const float mu = mu_used == -INFINITY ? 0.f : mu_used;
-      float ps0 = 0.f, ps1 = 0.f;
+      const uint64_t rf2 = qt_pack(rowf, rowf), mu2 = qt_pack(-mu, -mu);
       uint32_t w[16];
 #pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 vs = *reinterpret_cast<const float4*>(sc + QT_KB + c);
-        const float e0 = exp2f(__fmaf_rn(sv[c], rowf, -mu)), e1 = exp2f(__fmaf_rn(sv[c + 1], rowf, -mu));
-        const float e2 = exp2f(__fmaf_rn(sv[c + 2], rowf, -mu)), e3 = exp2f(__fmaf_rn(sv[c + 3], rowf, -mu));
-        ps0 += e0 + e1;
-        ps1 += e2 + e3;
-        float w0 = e0 * vs.x, w1 = e1 * vs.y, w2 = e2 * vs.z, w3 = e3 * vs.w;
-        if (!full) {
-          w0 = kb + c < lim ? w0 : 0.f;
-          w1 = kb + c + 1 < lim ? w1 : 0.f;
-          w2 = kb + c + 2 < lim ? w2 : 0.f;
-          w3 = kb + c + 3 < lim ? w3 : 0.f;
+      for (int c = 0; c < 16; c += 2) {
+        const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + QT_KB + 2 * c);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const float2 y = qt_unpack(qt_fma2(x[c + d], rf2, mu2));
+          const uint64_t e = qt_pack(qt_exp2(y.x), qt_exp2(y.y));
+          l = qt_add2(l, e);
+          const float2 ww = qt_unpack(qt_mul2(e, d ? vs.y : vs.x));
+          const __half2 h = __floats2half2_rn(ww.x, ww.y);
+          w[c + d] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        const __half2 h0 = __floats2half2_rn(w0, w1), h1 = __floats2half2_rn(w2, w3);
-        w[c / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-        w[c / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
       }
-      l += ps0 + ps1;
+      if (!full) {  // 0 * scale of a key that is not seen may be NaN
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          w[c] &= (kb + 2 * c < lim ? 0xffffu : 0u) | (kb + 2 * c + 1 < lim ? 0xffff0000u : 0u);
+      }
       const uint32_t t_w = tmem + lane_base + (uint32_t)(s * 64);
       tc_st16_nowait(t_w + half * 16, w);
 #pragma unroll
@@ -446,37 +545,37 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     }
     // ---- O of both copies through shared memory, then merged, row by row ----
     const int nb1 = n_blocks - 1;
-    if (ok && n_blocks > 0) ok = mbar_wait(&pv_done[nb1 & 1], (nb1 >> 1) & 1, 358, a.err);
+    if (ok && n_blocks > 0) ok = qt_wait(&pv_done[nb1 & 1], (nb1 >> 1) & 1, 358, a.err);
     ok = __all_sync(0xffffffffu, ok);
     constexpr int CH = HD / 4;  // float4 chunks per row
     float4* s_o = reinterpret_cast<float4*>(smem);
-    if (ok && n_blocks > 0) {
+    if (ok && my_blocks > 0) {
       tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 16) {
-        float ov[16];
-        tc_ld16(t_o + lane_base + (uint32_t)c, ov);
+      for (int c = 0; c < HD; c += 32) {
+        float ov[32];
+        tc_ld32(t_o + lane_base + (uint32_t)c, ov);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 8; ++e)
           s_o[threadIdx.x * CH + ((c / 4 + e) ^ (threadIdx.x & 7))] =
               make_float4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
       }
       tc_fence_before();
     }
-    s_ml[threadIdx.x] = make_float2(mu_used, l);
+    s_ml[threadIdx.x] = make_float2(mu_used, qt_unpack(l).x + qt_unpack(l).y);
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
     constexpr int RPW = CH >= 32 ? 1 : 32 / CH;  // rows a warp writes at a time
-    for (int r0 = warp * RPW; r0 < ntok * a.G && ok; r0 += 4 * RPW) {
+#pragma unroll 2
+    for (int r0 = warp * RPW; r0 < ntok * a.G; r0 += 4 * RPW) {
       const int r = r0 + lane / (32 / RPW), c0 = lane % (32 / RPW);
-      const int tok = r / a.G, hg = r % a.G;
-      if (tok >= ntok || !s_tok_ok[tok]) continue;
+      const int th = s_row[r], tok = th >> 4, head = kvh * a.G + (th & 15);
       const int lm = s_lim[r];
-      if (a.n_chunks > 1 && lm <= k_begin) continue;
       const float2 x0 = s_ml[r], x1 = s_ml[r + QT_ROWS];
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
-      const float w0 = exp2f(x0.x - mu), w1 = exp2f(x1.x - mu);
+      const float w0 = qt_exp2(x0.x - mu), w1 = qt_exp2(x1.x - mu);
       const float den = w0 * x0.y + w1 * x1.y;
-      const int mrow = m0 + tok, head = kvh * a.G + hg;
+      if (!ok || th < 0 || !s_tok_ok[tok] || (a.n_chunks > 1 && lm <= k_begin)) continue;
+      const int mrow = m0 + tok;
       const long long base = ((long long)chunk * a.M + mrow) * a.Hq + head;
 #pragma unroll
       for (int c = c0; c < CH; c += 32) {
@@ -506,7 +605,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "n"(L::COLS));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(*tmem_slot), "n"(L::COLS));
   }
 }
 

@@ -84,10 +84,10 @@ def _attention64(val, q, lim, seq, scale, gate=None):
         o[m] = torch.einsum("hgn,hnd->hgd", p, v).reshape(Hq, hd)
         A[m] = torch.einsum("hgn,hnd->hgd", p, v.abs()).reshape(Hq, hd)
         # fp16's lower end: a weight p_j vs_j is held in units in which the row's largest e_j times
-        # the largest vs is at least 2^10, rounded there to a multiple of 2^-24 at worst: off by at
-        # most 2^-25 / 2^10 = 2^-35 of max p * max vs <= max vs. Summed over n codes of at most TOP,
-        # and max vs * TOP being the largest |v|: n 2^-35 max |v|
-        low[m] = (n * 2.0 ** -35 * v.abs().amax((1, 2)))[:, None, None].expand(Hkv, G, hd).reshape(Hq, hd)
+        # the largest vs is at least 2^3, rounded there to a multiple of 2^-24 at worst: off by at
+        # most 2^-25 / 2^3 = 2^-28 of max p * max vs <= max vs. Summed over n codes of at most TOP,
+        # and max vs * TOP being the largest |v|: n 2^-28 max |v|
+        low[m] = (n * 2.0 ** -28 * v.abs().amax((1, 2)))[:, None, None].expand(Hkv, G, hd).reshape(Hq, hd)
     o, A, low = o.reshape(M, Hq * hd), A.reshape(M, Hq * hd), low.reshape(M, Hq * hd)
     if gate is not None:
         s = torch.sigmoid(gate.double())
