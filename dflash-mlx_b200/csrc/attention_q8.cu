@@ -36,7 +36,6 @@ namespace dfl {
 constexpr int Q8_KB = 32;       // keys per block
 constexpr int Q8_STRANDS = 4;   // blocks in flight per chunk, each a warp of every row group
 constexpr int Q8_CHUNK_UNIT = Q8_KB * Q8_STRANDS;
-constexpr int Q8_TC_CHUNK = 512;  // keys per chunk from which the tcgen05 form runs
 
 // ---- fp16 fragments ------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
       lim[mt][h] = s_lim[r0 + mt * 16 + g + 8 * h];
       mrow[mt][h] = Mr[mt][h] = -INFINITY;
       lrow[mt][h] = 0.f;
-      er[mt][h] = -90;
+      er[mt][h] = Q8_ER_MIN;
     }
   float o[MT][2 * NC][4];
 #pragma unroll
@@ -337,7 +336,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
             const __half2 w = __floats2half2_rn(w0, w1);
             pf[mt][j >> 1][(j & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&w);
           }
-          lrow[mt][h] = lrow[mt][h] * fac[h] + ps;
+          lrow[mt][h] = __fmaf_rn(ps, Q8_SUM_UNIT, lrow[mt][h] * fac[h]);
         }
         if (__any_sync(0xffffffffu, fac[0] != 1.f || fac[1] != 1.f)) {  // a factor of 1 is exact
 #pragma unroll
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
         if (a.n_chunks > 1) {
           *reinterpret_cast<float4*>(a.part_o + base * HD + d) = y;
         } else {
-          const float inv = lm > 0 ? 1.f / den : 0.f;
+          const float inv = lm > 0 ? Q8_SUM_UNIT / den : 0.f;
           float f[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
           if (a.gate) {
             const __nv_bfloat16* gr = a.gate + (long long)m * a.ldg + (long long)head * a.gate_hs + d;
@@ -475,7 +474,7 @@ __global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constan
     if (a.row_seq[first] != seq) return;
   }
   const int lim = q8_row_limit(a, m, p, seq, nullptr);
-  const int nch = min((lim + a.key_chunk - 1) / a.key_chunk, a.n_chunks);
+  const int nch = lim > 0 ? min((lim - 1) / a.key_chunk + 1, a.n_chunks) : 0;
   const long long cstride = (long long)a.M * a.Hq;
   const float2* ml = a.part_ml + item;
   const float* po = a.part_o + item * HD + lane * VEC;
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constan
       }
     }
   }
-  const float inv = lim > 0 ? 1.f / den : 0.f;
+  const float inv = lim > 0 ? Q8_SUM_UNIT / den : 0.f;
   __nv_bfloat16* dst = a.out + (long long)m * a.ldo + (long long)h * HD + lane * VEC;
   float y[VEC];
 #pragma unroll
@@ -588,18 +587,32 @@ static int launch_attn_q8_rows(const AttnQ8Args& a, int rows, int tiles, cudaStr
 
 using namespace dfl;
 
-// Keys per chunk for a call of `runs` sequences: enough chunks for about eight CTAs per SM at
-// one tile a run, between one block per strand and 2048 keys. Runs, not rows, so that decode
-// and verify of the same sequences split alike.
-static int q8_key_chunk(int key_chunk, long long runs, int Hkv, int max_kv) {
-  if (key_chunk > 0) return key_chunk;
-  const long long c = (long long)max_kv * runs * Hkv / (148 * 8);
-  const long long r = (c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT;
-  return (int)(r < Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : r > 2048 ? 2048 : r);
-}
-
 static int q8_run_rows(int M, int seq_rows, bool one_seq) {
   return one_seq ? M : seq_rows > 0 ? (seq_rows < M ? seq_rows : M) : 1;
+}
+
+// The form and the keys per chunk of a call. Up to 16 (token, head) rows a run take the warp form, more the
+// tcgen05 form, whose tile of 64 rows they fill better (one token of 64 sequences 105 against
+// 123 us, 16 tokens 280 against 168).
+struct Q8Plan {
+  int form, key_chunk, n_chunks;
+};
+static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int G, int Hkv, int hd, int max_kv) {
+  Q8Plan p;
+  const long long want = (long long)run_rows * G;
+  p.form = form != DFL_Q8_AUTO ? form : want <= 16 ? DFL_Q8_WARP : DFL_Q8_TC;
+  if (key_chunk <= 0) {
+    // about as many CTAs as the SMs hold at a time (warp form: eight an SM, its CTAs are short-lived;
+    // tcgen05 form: one wave, since a CTA's start and end cost it some ten blocks)
+    const long long units = runs * Hkv * ((want + 63) / 64);
+    const long long slots = 148 * (p.form == DFL_Q8_TC ? (hd == 256 ? 1 : 2) : 8);
+    const long long lo = p.form == DFL_Q8_TC ? 512 : Q8_CHUNK_UNIT, hi = p.form == DFL_Q8_TC ? 8192 : 4096;
+    const long long r = (max_kv * units / slots + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT;
+    key_chunk = (int)(r < lo ? lo : r > hi ? hi : r);
+  }
+  p.key_chunk = key_chunk;
+  p.n_chunks = (int)(((long long)max_kv + key_chunk - 1) / key_chunk);
+  return p;
 }
 
 static size_t q8_workspace(int M, int Hq, int hd, int n_chunks) {
@@ -609,17 +622,19 @@ static size_t q8_workspace(int M, int Hq, int hd, int n_chunks) {
 }
 
 extern "C" size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq,
-                                                   int max_kv, int key_chunk) {
-  if (!cache || M <= 0 || Hq <= 0 || max_kv <= 0 || key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT || cache->n_kv_heads <= 0)
+                                                   int max_kv, int form, int key_chunk) {
+  if (!cache || M <= 0 || Hq <= 0 || max_kv <= 0 || key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT ||
+      cache->n_kv_heads <= 0 || form < DFL_Q8_AUTO || form > DFL_Q8_TC)
     return 0;
   const int rr = q8_run_rows(M, seq_rows, one_seq != 0);
-  const int kc = q8_key_chunk(key_chunk, (M + rr - 1) / rr, cache->n_kv_heads, max_kv);
-  return q8_workspace(M, Hq, cache->head_dim, (max_kv + kc - 1) / kc);
+  return q8_workspace(M, Hq, cache->head_dim,
+                      q8_plan(form, key_chunk, (M + rr - 1) / rr, rr, Hq / cache->n_kv_heads, cache->n_kv_heads,
+                              cache->head_dim, max_kv).n_chunks);
 }
 
 extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq,
                                 const int32_t* kv_len, int seq_rows, int M, int Hq, int causal, float scale,
-                                int max_kv, int key_chunk, void* out, int64_t ldo, const void* gate, int64_t ldg,
+                                int max_kv, int form, int key_chunk, void* out, int64_t ldo, const void* gate, int64_t ldg,
                                 int gate_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "dfl_attention_q8";
   if (M == 0) return DFL_OK;
@@ -634,6 +649,10 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
   if (G > 16) {
     set_error("%s: query heads per kv head must be 1..16 (got %d)", who, G);
     return DFL_ERR_UNSUPPORTED;
+  }
+  if (form < DFL_Q8_AUTO || form > DFL_Q8_TC) {
+    set_error("%s: unknown form %d", who, form);
+    return DFL_ERR_INVALID;
   }
   if (key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT) {
     set_error("%s: key_chunk %d must be a multiple of %d", who, key_chunk, Q8_CHUNK_UNIT);
@@ -651,8 +670,9 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
   }
   const int run_rows = q8_run_rows(M, seq_rows, row_seq == nullptr);
   const int runs = (M + run_rows - 1) / run_rows;
-  a.key_chunk = q8_key_chunk(key_chunk, runs, Hkv, max_kv);
-  a.n_chunks = (int)(((long long)max_kv + a.key_chunk - 1) / a.key_chunk);
+  const Q8Plan plan = q8_plan(form, key_chunk, runs, run_rows, G, Hkv, hd, max_kv);
+  a.key_chunk = plan.key_chunk;
+  a.n_chunks = plan.n_chunks;
   if (a.n_chunks > 65535) {
     set_error("%s: %d key chunks; a larger key_chunk is needed", who, a.n_chunks);
     return DFL_ERR_UNSUPPORTED;
@@ -662,9 +682,7 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
     set_error("%s: workspace missing, misaligned or too small (%zu < %zu)", who, workspace_bytes, need);
     return DFL_ERR_WORKSPACE;
   }
-  // long chunks take the tcgen05 form (the chunk size alone decides, so that calls to be
-  // compared bit for bit, which use one chunk size, use one form)
-  const bool tc = a.key_chunk >= Q8_TC_CHUNK;
+  const bool tc = plan.form == DFL_Q8_TC;
   // rows a CTA takes: 16, 32 or (tcgen05 form, or head_dim <= 128) 64 (token, head) pairs
   const int most = hd == 256 && !tc ? 32 : 64;
   const long long want = (long long)run_rows * G;

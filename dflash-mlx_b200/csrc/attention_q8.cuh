@@ -5,6 +5,13 @@
 
 namespace dfl {
 
+// A row's exponentials e_j carry the factor 2^-er, er the exponent of the largest V scale it has seen,
+// so that the weights e_j vs_j fit fp16. er starts at Q8_ER_MIN (V scales below 2^-104 are the first to
+// lose bits), and the sums of e_j are kept in units of 2^16: with er between -104 and 90 neither they
+// nor the weights leave fp32's normal range, over 2^20 keys and more.
+constexpr int Q8_ER_MIN = -104;
+constexpr float Q8_SUM_UNIT = 1.f / 65536.f;
+
 struct AttnQ8Args {
   const __nv_bfloat16* q;  // [M][Hq][hd]
   Q8Cache c;

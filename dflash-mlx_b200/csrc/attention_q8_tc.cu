@@ -28,7 +28,6 @@ constexpr int QT_KB = 64;       // keys per block
 constexpr int QT_ROWS = 64;     // (token, head) rows per tile
 constexpr int QT_THREADS = 288;
 constexpr int QT_SCALES = 4;    // scale ring: block i's are read until its weights are written
-constexpr int QT_AHEAD = 4;     // blocks prefetched into L2
 constexpr float QT_BASE = 4.f, QT_LAZY = 10.f;
 
 template <int HD>
@@ -38,8 +37,8 @@ struct QtLayout {
   static constexpr int OFF_K = 0;               // 2 stages
   static constexpr int OFF_V = 2 * TILE;        // 2 stages; the epilogue reuses K and V for O
   static constexpr int OFF_Q = 4 * TILE;        // [units][128 rows][128 B]
-  static constexpr int OFF_S = OFF_Q + 128 * HD * 2;  // scales [4][2][64]
-  static constexpr int OFF_R = OFF_S + QT_SCALES * 2 * QT_KB * 4;  // row factor, limit, (M, l) of both copies
+  static constexpr int OFF_S = OFF_Q + 128 * HD * 2;  // scales [4][2][64], largest V scales [4][2]
+  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of both copies
   static constexpr int OFF_BAR = OFF_R + QT_ROWS * 8 + 128 * 8;
   static constexpr int N_BAR = 2 * 4 + 2 * 3 + QT_SCALES;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
@@ -118,11 +117,6 @@ __device__ __forceinline__ uint64_t qt_mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t qt_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t qt_fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -144,6 +138,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* s_sc = reinterpret_cast<float*>(smem + L::OFF_S);  // [ring][K, V][64]
+  uint32_t* s_vmax = reinterpret_cast<uint32_t*>(s_sc + QT_SCALES * 2 * QT_KB);  // [ring][half], finite scales' bits
   float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_R);
   int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + QT_ROWS;
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + QT_ROWS * 8);  // [128]
@@ -242,27 +237,25 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     const int r = ((ct >> 2) & 1) | ((ct / (8 * HI)) << 1);
     const uint32_t dst0 = (uint32_t)(c >> 2) * (QT_KB * 128) + qt_sw(r, (c & 3) * 2);
     src += c * 16;
-    // Places of 32 blocks, one a lane, read together: a table lookup per block would stand in front of
-    // the block's loads.
-    int win = 0, win_page = -1;
+    // Codes and scale offsets of 32 blocks, one a lane, made together: a table lookup per block would
+    // stand in front of the block's loads. A place that is refused is -1: its keys have scale 0.
+    int win = 0;
+    long long win_off = -1, win_soff = 0;
     auto window = [&](int i) {
-      long long page = -1;
-      int row;
+      long long page = 0;
+      int row = 0;
       win = i;
-      if (i + lane < n_blocks && !q8_place(a.c, seq, k_begin + (i + lane) * QT_KB, warp == 4 ? a.err : nullptr, page, row))
-        page = -1;
-      win_page = (int)page;
+      win_off = -1;
+      if (i + lane < n_blocks && q8_place(a.c, seq, k_begin + (i + lane) * QT_KB, warp == 4 ? a.err : nullptr, page, row)) {
+        win_off = page * a.c.seq_stride + (long long)row * HD;
+        win_soff = page * a.c.s_seq_stride + row;
+      }
     };
-    // block i's codes and scale offsets and keys (0 behind the last block, or when its place is refused)
+    // block i's codes and scale offsets; its keys, 0 behind the last block
     auto where = [&](int i, long long& off, long long& soff) -> int {
-      const long long page = __shfl_sync(0xffffffffu, win_page, i - win);
-      const int kb = k_begin + i * QT_KB;
-      const int row = a.c.page_table ? kb & ((1 << a.c.page_shift) - 1) : kb;
-      off = soff = 0;
-      if (page < 0) return 0;
-      off = page * a.c.seq_stride + (long long)row * HD;
-      soff = page * a.c.s_seq_stride + row;
-      return min(QT_KB, k_end - kb);
+      off = __shfl_sync(0xffffffffu, win_off, i - win);
+      soff = __shfl_sync(0xffffffffu, win_soff, i - win);
+      return off < 0 ? 0 : min(QT_KB, k_end - (k_begin + i * QT_KB));
     };
     uint4 b[PER];
     // The thread's chunks of a block of n keys at p: volatile, so that the loads are issued here, most of
@@ -286,24 +279,22 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         for (int u = 0; u < PER; ++u) b[u] = make_uint4(0, 0, 0, 0);
       }
     };
-    auto prefetch = [&](int i) {  // a block into L2, by the thread whose src is the matrix's start
-      long long o, so;
-      const int n = where(i, o, so);
-      if (ct == 0 && n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(src + o), "r"(n * HD) : "memory");
-    };
     long long off, soff;
     window(0);
     int n = where(0, off, soff);
     fetch(src + off, n);
     float scale = ct < n ? __ldg(ssrc + soff) : 0.f;
-    for (int i = 1; i < QT_AHEAD; ++i) prefetch(i);
     for (int i = 0; i < n_blocks; ++i) {
       const int s = i & 1;
-      if (i + QT_AHEAD - win >= 32) window(i + 1);
+      if (i + 1 - win >= 32) window(i + 1);
       n = where(i + 1, off, soff);
-      prefetch(i + QT_AHEAD);
       if (!qt_wait(&empty[s], ((i >> 1) & 1) ^ 1, 350, a.err)) break;
       sdst[(i & (QT_SCALES - 1)) * 2 * QT_KB] = scale;
+      if (is_v) {  // a warp holds the 32 keys of one copy
+        const uint32_t v = __float_as_uint(scale) & 0x7fffffffu;
+        const uint32_t vm = __reduce_max_sync(0xffffffffu, v < 0x7f800000u ? v : 0u);
+        if (lane == 0) s_vmax[(i & (QT_SCALES - 1)) * 2 + (ct >> 5)] = vm;
+      }
       mbar_arrive(&sc_full[i & (QT_SCALES - 1)]);
       unsigned char* d = dst + s * L::TILE + dst0;
 #pragma unroll
@@ -404,9 +395,10 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         const uint32_t u[8] = {nx[0].x, nx[0].y, nx[0].z, nx[0].w, nx[1].x, nx[1].y, nx[1].z, nx[1].w};
         qload(r + 4 * RPW);
         // magnitudes compare as integers; one that is not finite leaves the row unscaled
-        uint32_t mx = 0;
+        uint32_t mx2 = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mx = max(mx, max((u[j] << 16) & 0x7fffffffu, u[j] & 0x7fff0000u));
+        for (int j = 0; j < 8; ++j) mx2 = __vmaxu2(mx2, u[j] & 0x7fff7fffu);
+        uint32_t mx = max(mx2 << 16, mx2 & 0xffff0000u);
 #pragma unroll
         for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const int sh = mx > 0 && mx < 0x7f800000u ? min(14 - ((int)(mx >> 23) - 127), 120) : 0;
@@ -439,7 +431,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     const float rowf = s_rowf[row];
     float m = -INFINITY, mu_used = -INFINITY;
     uint64_t l = 0;  // two partial sums
-    int er = -90;
+    int er = Q8_ER_MIN;
     bool ok = true;
     // a warp whose 32 rows all lie behind the tile's does nothing: what its lanes hold goes to its own
     // rows of O, which nobody reads
@@ -465,10 +457,8 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         x[c] = qt_mul2(qt_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
         x[c + 1] = qt_mul2(qt_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
       }
-      uint32_t vm = __float_as_uint(sc[QT_KB + lane]) & 0x7fffffffu;
-      if (full) {
-        vm = __reduce_max_sync(0xffffffffu, vm < 0x7f800000u ? vm : 0u);
-      } else {
+      uint32_t vm = s_vmax[(i & (QT_SCALES - 1)) * 2 + half];
+      if (!full) {
         vm = 0;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -514,7 +504,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         }
       }
       const float mu = mu_used == -INFINITY ? 0.f : mu_used;
-      const uint64_t rf2 = qt_pack(rowf, rowf), mu2 = qt_pack(-mu, -mu);
+      const uint64_t rf2 = qt_pack(rowf, rowf), mu2 = qt_pack(-mu, -mu), unit2 = qt_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
       uint32_t w[16];
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {
@@ -523,7 +513,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         for (int d = 0; d < 2; ++d) {
           const float2 y = qt_unpack(qt_fma2(x[c + d], rf2, mu2));
           const uint64_t e = qt_pack(qt_exp2(y.x), qt_exp2(y.y));
-          l = qt_add2(l, e);
+          l = qt_fma2(e, unit2, l);
           const float2 ww = qt_unpack(qt_mul2(e, d ? vs.y : vs.x));
           const __half2 h = __floats2half2_rn(ww.x, ww.y);
           w[c + d] = *reinterpret_cast<const uint32_t*>(&h);
@@ -587,7 +577,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         if (a.n_chunks > 1) {
           *reinterpret_cast<float4*>(a.part_o + base * HD + c * 4) = y;
         } else {
-          const float inv = lm > 0 ? 1.f / den : 0.f;
+          const float inv = lm > 0 ? Q8_SUM_UNIT / den : 0.f;
           float f[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
           if (a.gate) {
             const __nv_bfloat16* gr = a.gate + (long long)mrow * a.ldg + (long long)head * a.gate_hs + c * 4;

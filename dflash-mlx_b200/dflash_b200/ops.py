@@ -458,6 +458,7 @@ class KvQ8(ctypes.Structure):
                 ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("type", ctypes.c_int)]
 
 
+Q8_FORMS = {"auto": 0, "warp": 1, "tc": 2}  # DFL_Q8_AUTO, DFL_Q8_WARP, DFL_Q8_TC
 KV_Q8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # DFL_KV_INT8, DFL_KV_E4M3
 
 
@@ -578,11 +579,12 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
                  kv_len: torch.Tensor | None = None, row_seq: torch.Tensor | None = None,
                  scale: float | None = None, out: torch.Tensor | None = None, ws: Workspace | None = None,
                  gate: torch.Tensor | None = None, gate_head_stride: int = 0, seq_rows: int = 0,
-                 key_chunk: int = 0) -> torch.Tensor:
+                 key_chunk: int = 0, form: str = "auto") -> torch.Tensor:
     """attention() over an 8-bit cache (dfl_attention_q8): q [M, Hq, hd] bf16 against ``kv``;
     returns [M, Hq*hd] bf16. seq_rows: rows per sequence when row_seq groups contiguous runs (0 =
-    any layout). key_chunk (a multiple of 128; 0 = chosen from the sequences, heads and max_kv):
-    results depend on it. Rows with pos < 0 are left as they are; rows that see no key are zero.
+    any layout). ``form``: "warp" (mma.sync, few rows), "tc" (tcgen05, verify blocks and prefill) or
+    "auto"; key_chunk: keys per split, a multiple of 128, 0 = chosen by the call's sizes. A row's
+    result depends on these two and its own query and keys only. Rows with pos < 0 are left as they are; rows that see no key are zero.
     ``ws``: partial results live in its attention scratch (one workspace per stream and captured
     graph, as for attention()); without it each call allocates its own."""
     dev, hd = kv.device, kv.head_dim
@@ -592,6 +594,9 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
     _index_rows("pos", pos, M, dev)
     _index_rows("row_seq", row_seq, M, dev)
     _index_rows("kv_len", kv_len, kv.n_seqs, dev)
+    fcode = Q8_FORMS.get(form)
+    if fcode is None:
+        raise ValueError(f"form must be one of {tuple(Q8_FORMS)}, not {form!r}")
     if scale is None:
         scale = 1.0 / math.sqrt(hd)
     if out is None:
@@ -604,14 +609,14 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
                 or gate.shape[1] < (Hq - 1) * ghs + hd:
             raise ValueError(f"gate must be bf16 rows covering {Hq} heads on {dev}")
     need = int(_lib.query("dfl_attention_q8_workspace_bytes", kv._ref, M, Hq, int(seq_rows), int(row_seq is None),
-                          int(max_kv), int(key_chunk)))
+                          int(max_kv), fcode, int(key_chunk)))
     if ws is not None:
         ws.ensure_attn(need)
         scratch = ws.attn
     else:
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _call_on(dev, "dfl_attention_q8", q.data_ptr(), kv._ref, pos.data_ptr(), _ptr(row_seq), _ptr(kv_len),
-             int(seq_rows), M, Hq, int(causal), float(scale), int(max_kv), int(key_chunk), out.data_ptr(),
+             int(seq_rows), M, Hq, int(causal), float(scale), int(max_kv), fcode, int(key_chunk), out.data_ptr(),
              _row_stride(out), _ptr(gate), _row_stride(gate) if gate is not None else 0, int(gate_head_stride),
              _ptr(scratch), scratch.numel() if scratch is not None else 0)
     return out

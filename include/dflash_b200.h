@@ -338,6 +338,9 @@ int dfl_attention_qkv(const void* qkv, int64_t ldqkv, const void* q_norm, const 
  * position or key range beyond cap or max_kv, 342 a page number. */
 #define DFL_KV_INT8 0
 #define DFL_KV_E4M3 1
+#define DFL_Q8_AUTO 0
+#define DFL_Q8_WARP 1
+#define DFL_Q8_TC 2
 typedef struct dfl_kv_q8 {
   void* k;               /* codes */
   void* v;
@@ -371,15 +374,17 @@ int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* ro
 /* dfl_attention (same arguments and meanings) over an 8-bit cache, at most 16 query heads per
  * kv head. Rows of one sequence share a tile: with row_seq, every run of seq_rows rows starting
  * at a multiple of seq_rows belongs to one sequence (0 = any layout: each row is its own run);
- * without it all rows are sequence 0's. key_chunk (multiple of 128; 0 = chosen from the number
- * of runs, n_kv_heads and max_kv): keys per split; a row's result depends on it and on nothing
- * else of the call but the row's own query and keys. A row with pos >= 0 that sees no key
+ * without it all rows are sequence 0's. form: DFL_Q8_WARP (mma.sync, keys split over a CTA's
+ * warps: few rows) or DFL_Q8_TC (tcgen05, 64 rows a CTA: verify blocks and prefill); key_chunk:
+ * keys per split, a multiple of 128. A row's result depends on these two and on nothing else
+ * of the call but the row's own query and keys, so calls to be compared bit for bit name
+ * both; DFL_Q8_AUTO and key_chunk 0 choose by the call's sizes. A row with pos >= 0 that sees no key
  * (kv_len <= 0) is zero; rows with pos < 0 are left as they are. max_kv bounds every row's
  * keys. ldo % 4 == 0, q 16-byte and out 8-byte aligned. */
 size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq, int max_kv,
-                                        int key_chunk);
+                                        int form, int key_chunk);
 int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq,
-                     const int32_t* kv_len, int seq_rows, int M, int Hq, int causal, float scale, int max_kv,
+                     const int32_t* kv_len, int seq_rows, int M, int Hq, int causal, float scale, int max_kv, int form,
                      int key_chunk, void* out, int64_t ldo, const void* gate, int64_t ldg, int gate_head_stride,
                      void* workspace, size_t workspace_bytes, void* stream);
 

@@ -23,11 +23,11 @@ def _append(desc, **kw):
 
 
 def _attn(desc, **kw):
-    a = dict(q=64, pos=64, row_seq=None, kv_len=None, seq_rows=0, M=2, Hq=4, causal=1, scale=0.1, max_kv=512, chunk=0,
+    a = dict(q=64, pos=64, row_seq=None, kv_len=None, seq_rows=0, M=2, Hq=4, causal=1, scale=0.1, max_kv=512, form=0, chunk=0,
              out=64, ldo=512, ws=None, ws_bytes=0)
     a.update(kw)
     return ("dfl_attention_q8", a["q"], desc, a["pos"], a["row_seq"], a["kv_len"], a["seq_rows"], a["M"], a["Hq"],
-            a["causal"], a["scale"], a["max_kv"], a["chunk"], a["out"], a["ldo"], None, 0, 0, a["ws"], a["ws_bytes"],
+            a["causal"], a["scale"], a["max_kv"], a["form"], a["chunk"], a["out"], a["ldo"], None, 0, 0, a["ws"], a["ws_bytes"],
             None)
 
 
@@ -64,7 +64,7 @@ def test_bad_caches_are_refused_by_every_entry_point(lib, bad, status):
     (_attn(_desc(), scale=float("nan")), 1), (_attn(_desc(), scale=float("inf")), 1), (_attn(_desc(), ldo=510), 2),
     (_attn(_desc(), ldo=256), 2), (_attn(_desc(), out=68), 2), (_attn(_desc(), q=72), 2),
     (_attn(_desc(), chunk=128), 4), (_attn(_desc(), chunk=128, ws=64, ws_bytes=100), 4),
-    (_attn(_desc(), seq_rows=-1), 1), (_attn(_desc(cap=1 << 30), max_kv=1 << 30, chunk=128, ws=64, ws_bytes=1 << 62), 2),
+    (_attn(_desc(), seq_rows=-1), 1), (_attn(_desc(), form=3), 1), (_attn(_desc(), form=-1), 1), (_attn(_desc(cap=1 << 30), max_kv=1 << 30, chunk=128, ws=64, ws_bytes=1 << 62), 2),
 ])
 def test_bad_arguments_are_refused_before_any_launch(lib, call, status):
     from dflash_b200 import _lib
@@ -78,13 +78,12 @@ def test_empty_calls_succeed_and_scratch_follows_the_chunks(lib):
     for make in (_append, _attn, _read):
         _lib.call(*make(_desc(), M=0))
     size = lambda *a: _lib.query("dfl_attention_q8_workspace_bytes", _desc(), *a)  # noqa: E731
-    assert size(2, 4, 1, 0, 512, 512) == 0  # one chunk
-    assert size(2, 4, 1, 0, 512, 128) == 4 * 2 * 4 * 128 * 4 + 4 * 2 * 4 * 8
-    assert size(2, 4, 1, 0, 513, 128) > size(2, 4, 1, 0, 512, 128)
-    assert size(0, 4, 1, 0, 512, 128) == 0 and size(2, 4, 1, 0, 512, 100) == 0
-    # the split depends on the sequences, not on their rows: decode and verify of a batch agree
-    rows1, rows16 = size(4, 4, 1, 0, 100000, 0) // 4, size(64, 4, 16, 0, 100000, 0) // 64
-    assert rows1 == rows16
+    for form in (1, 2):
+        assert size(2, 4, 1, 0, 512, form, 512) == 0  # one chunk
+        assert size(2, 4, 1, 0, 512, form, 128) == 4 * 2 * 4 * 128 * 4 + 4 * 2 * 4 * 8
+        assert size(2, 4, 1, 0, 513, form, 128) > size(2, 4, 1, 0, 512, form, 128)
+        assert size(0, 4, 1, 0, 512, form, 128) == 0 and size(2, 4, 1, 0, 512, form, 100) == 0
+    assert size(2, 4, 1, 0, 512, 3, 128) == 0
 
 
 def test_wrappers_take_cuda_tensors_only():

@@ -99,33 +99,33 @@ def _attention64(val, q, lim, seq, scale, gate=None):
 
 
 CASES = [
-    # type, lens, rows, Hkv, G, hd, page, causal, gate, key_chunk
-    ("int8", [1], 1, 1, 1, 64, 0, True, False, 0),
-    ("e4m3", [1], 1, 2, 4, 128, 64, True, False, 0),
-    ("int8", [33, 32, 31], 1, 2, 3, 128, 64, True, True, 0),
-    ("e4m3", [129, 640, 7], 1, 1, 8, 256, 128, True, False, 128),
-    ("int8", [1000, 517], 5, 2, 4, 128, 0, True, False, 256),
-    ("e4m3", [200, 130, 384], 16, 2, 4, 128, 64, True, False, 128),
-    ("int8", [700, 90], 16, 1, 6, 256, 0, True, True, 512),
-    ("e4m3", [150], 150, 2, 5, 64, 64, True, False, 128),
-    ("int8", [261], 37, 1, 16, 128, 128, True, True, 0),
-    ("int8", [300, 1, 64], 16, 2, 2, 64, 0, False, False, 128),
-    ("e4m3", [77, 513], 8, 2, 4, 128, 64, False, True, 0),
-    ("int8", [2100], 1, 2, 7, 128, 64, False, False, 128),
-    # chunks of 512 and more: the tcgen05 form
-    ("int8", [1], 1, 1, 1, 128, 64, True, False, 512),
-    ("e4m3", [1025, 33, 511], 1, 2, 4, 128, 64, True, True, 512),
-    ("int8", [1100, 97, 640], 16, 2, 4, 128, 0, True, False, 512),
-    ("e4m3", [640, 130], 16, 1, 6, 256, 128, True, True, 512),
-    ("int8", [700, 5], 5, 2, 3, 256, 0, False, False, 1024),
-    ("e4m3", [900, 64], 16, 2, 2, 64, 64, False, True, 512),
-    ("int8", [2500], 100, 1, 8, 64, 64, True, False, 1024),
-    ("int8", [1300, 514], 5, 2, 4, 128, 64, True, False, 1024),
+    # type, lens, rows, Hkv, G, hd, page, causal, gate, form, key_chunk
+    ("int8", [1], 1, 1, 1, 64, 0, True, False, "auto", 0),
+    ("e4m3", [1], 1, 2, 4, 128, 64, True, False, "auto", 0),
+    ("int8", [33, 32, 31], 1, 2, 3, 128, 64, True, True, "auto", 0),
+    ("e4m3", [129, 640, 7], 1, 1, 8, 256, 128, True, False, "warp", 128),
+    ("int8", [1000, 517], 5, 2, 4, 128, 0, True, False, "warp", 256),
+    ("e4m3", [200, 130, 384], 16, 2, 4, 128, 64, True, False, "warp", 128),
+    ("int8", [700, 90], 16, 1, 6, 256, 0, True, True, "warp", 512),
+    ("e4m3", [150], 150, 2, 5, 64, 64, True, False, "warp", 128),
+    ("int8", [261], 37, 1, 16, 128, 128, True, True, "auto", 0),
+    ("int8", [300, 1, 64], 16, 2, 2, 64, 0, False, False, "warp", 128),
+    ("e4m3", [77, 513], 8, 2, 4, 128, 64, False, True, "auto", 0),
+    ("int8", [2100], 1, 2, 7, 128, 64, False, False, "warp", 128),
+    # the tcgen05 form
+    ("int8", [1], 1, 1, 1, 128, 64, True, False, "tc", 512),
+    ("e4m3", [1025, 33, 511], 1, 2, 4, 128, 64, True, True, "tc", 512),
+    ("int8", [1100, 97, 640], 16, 2, 4, 128, 0, True, False, "tc", 512),
+    ("e4m3", [640, 130], 16, 1, 6, 256, 128, True, True, "tc", 512),
+    ("int8", [700, 5], 5, 2, 3, 256, 0, False, False, "tc", 1024),
+    ("e4m3", [900, 64], 16, 2, 2, 64, 64, False, True, "tc", 512),
+    ("int8", [2500], 100, 1, 8, 64, 64, True, False, "tc", 1024),
+    ("int8", [1300, 514], 5, 2, 4, 128, 64, True, False, "tc", 1024),
 ]
 
 
-@pytest.mark.parametrize("t,lens,rows,Hkv,G,hd,page,causal,gated,chunk", CASES)
-def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gated, chunk):
+@pytest.mark.parametrize("t,lens,rows,Hkv,G,hd,page,causal,gated,form,chunk", CASES)
+def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gated, form, chunk):
     from dflash_b200 import ops
     c = Cache(t, lens, Hkv, hd, page, seed=hd + rows, wide=rows == 5)
     g = torch.Generator().manual_seed(7)
@@ -138,7 +138,7 @@ def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gate
     gate = torch.randn(B * rows, Hq * hd, generator=g).bfloat16() if gated else None
     out = torch.full((B * rows, Hq * hd), 9.0, dtype=torch.bfloat16, device=DEV)
     ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), causal, max(lens), kv_len=kv_len.to(DEV),
-                     row_seq=seq.to(DEV) if B > 1 else None, seq_rows=rows, key_chunk=chunk, out=out,
+                     row_seq=seq.to(DEV) if B > 1 else None, seq_rows=rows, form=form, key_chunk=chunk, out=out,
                      gate=gate.to(DEV) if gated else None)
     lim = pos + 1 if causal else kv_len[seq.long()]
     ref, tol = _attention64(c.val, q, lim, seq, hd ** -0.5, gate)
@@ -150,9 +150,9 @@ def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gate
 
 
 @pytest.mark.parametrize("t", ["int8", "e4m3"])
-@pytest.mark.parametrize("chunk", [128, 512])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
 @pytest.mark.parametrize("G,hd", [(1, 128), (4, 128), (2, 64), (3, 256), (6, 128)])
-def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, chunk):
+def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, form, chunk):
     """A verify block's rows equal single-token calls bit for bit, with later rows' keys (masked for
     the earlier ones) NaN, infinite or huge; paged equals contiguous."""
     from dflash_b200 import ops
@@ -162,7 +162,7 @@ def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, chunk):
     q = torch.randn(2 * rows, Hkv * G, hd, generator=g).bfloat16().to(DEV)
     seq = torch.arange(2, dtype=torch.int32, device=DEV).repeat_interleave(rows)
     pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
-    kw = dict(causal=True, max_kv=700, key_chunk=chunk)
+    kw = dict(causal=True, max_kv=700, form=form, key_chunk=chunk)
     full = ops.attention_q8(q, flat.kv, pos, row_seq=seq, seq_rows=rows, **kw)
     assert torch.equal(full, ops.attention_q8(q, paged.kv, pos, row_seq=seq, seq_rows=rows, **kw))
     assert torch.equal(full, ops.attention_q8(q, flat.kv, pos, row_seq=seq, **kw))  # any layout
@@ -182,8 +182,8 @@ def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, chunk):
     assert ops.device_error() == 0
 
 
-@pytest.mark.parametrize("chunk", [128, 512])
-def test_rows_without_keys_are_zero_and_empty_calls_do_nothing(chunk):
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+def test_rows_without_keys_are_zero_and_empty_calls_do_nothing(form, chunk):
     from dflash_b200 import ops
     c = Cache("int8", [40, 40, 40], 2, 128)
     q = torch.randn(3, 4, 128).bfloat16().to(DEV)
@@ -193,15 +193,15 @@ def test_rows_without_keys_are_zero_and_empty_calls_do_nothing(chunk):
     for max_kv in (40, 1000):  # one chunk, several
         c2 = c if max_kv == 40 else Cache("int8", [40, 40, 1000], 2, 128)
         out = torch.full((3, 512), 5.0, dtype=torch.bfloat16, device=DEV)
-        ops.attention_q8(q, c2.kv, pos, False, max_kv, kv_len=kv_len, row_seq=seq, seq_rows=1, out=out, key_chunk=chunk)
+        ops.attention_q8(q, c2.kv, pos, False, max_kv, kv_len=kv_len, row_seq=seq, seq_rows=1, out=out, form=form, key_chunk=chunk)
         assert (out[1] == 0).all() and (out[2] == 5).all() and out[0].isfinite().all() and (out[0] != 5).any()
     assert ops.attention_q8(q[:0], c.kv, pos[:0], True, 40).shape == (0, 512)
     assert ops.kv_read_q8(c.kv, pos[:0])[0].shape == (0, 2, 128)
     assert ops.device_error() == 0
 
 
-@pytest.mark.parametrize("chunk", [128, 512])
-def test_scales_and_queries_of_extreme_size(chunk):
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+def test_scales_and_queries_of_extreme_size(form, chunk):
     """Values far from 1 keep their relative precision; a softmax scale of 0 averages the values."""
     from dflash_b200 import ops
     for ks, vs, qs in ((1e-20, 1e-20, 1e15), (1e12, 1e25, 1e-12), (1.0, 1e-30, 1.0)):
@@ -212,14 +212,14 @@ def test_scales_and_queries_of_extreme_size(chunk):
         q = (torch.randn(4, 8, 128, generator=torch.Generator().manual_seed(2)) * qs).bfloat16()
         pos = torch.tensor([196, 197, 198, 199], dtype=torch.int32)
         sc = 128 ** -0.5 / (ks * qs)
-        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, key_chunk=chunk, scale=sc)
+        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, form=form, key_chunk=chunk, scale=sc)
         ref, tol = _attention64(val, q, pos + 1, torch.zeros(4), sc)
         assert ((out.double().cpu() - ref).abs() <= tol).all()
-        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, key_chunk=chunk, scale=0.0)
+        out = ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, form=form, key_chunk=chunk, scale=0.0)
         ref, tol = _attention64(val, q, pos + 1, torch.zeros(4), 0.0)
         assert ((out.double().cpu() - ref).abs() <= tol).all()
-        neg = ops.attention_q8((-q).to(DEV), c.kv, pos.to(DEV), True, 200, key_chunk=chunk, scale=-sc)
-        assert torch.equal(neg, ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, key_chunk=chunk, scale=sc))
+        neg = ops.attention_q8((-q).to(DEV), c.kv, pos.to(DEV), True, 200, form=form, key_chunk=chunk, scale=-sc)
+        assert torch.equal(neg, ops.attention_q8(q.to(DEV), c.kv, pos.to(DEV), True, 200, form=form, key_chunk=chunk, scale=sc))
 
 
 def _append64(qkv, pos, qn, kn, inv, Hq, Hkv, hd, rot, qs, eps):
@@ -316,9 +316,9 @@ def test_rows_that_hold_infinities_or_nans_are_held_as_nan():
         assert v[0, 0].isnan().all() and v[0, 1].isfinite().all() and k.isfinite().all()
 
 
-@pytest.mark.parametrize("chunk", [128, 512])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
 @pytest.mark.parametrize("page", [0, 64])
-def test_out_of_range_rows_are_refused_on_the_device(page, chunk):
+def test_out_of_range_rows_are_refused_on_the_device(page, form, chunk):
     """Positions, sequences and pages out of range are not accessed and set the error word; the other
     rows of the call are served."""
     from dflash_b200 import ops
@@ -327,13 +327,13 @@ def test_out_of_range_rows_are_refused_on_the_device(page, chunk):
     q = torch.randn(2, 4, 128).bfloat16().to(DEV)
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
     assert ops.device_error() == 0
-    good = ops.attention_q8(q, c.kv, i32(50, 60), True, 100, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=1)
+    good = ops.attention_q8(q, c.kv, i32(50, 60), True, 100, form=form, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=1)
     out = torch.zeros_like(good)
-    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, key_chunk=chunk, row_seq=i32(0, 2), seq_rows=1, out=out)  # no sequence 2
+    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, form=form, key_chunk=chunk, row_seq=i32(0, 2), seq_rows=1, out=out)  # no sequence 2
     assert ops.device_error() == 340 and torch.equal(out[0], good[0]) and (out[1] == 0).all()
-    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=2, out=out)  # two in one run
+    ops.attention_q8(q, c.kv, i32(50, 60), True, 100, form=form, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=2, out=out)  # two in one run
     assert ops.device_error() == 340 and torch.equal(out[0], good[0]) and (out[1] == 0).all()
-    ops.attention_q8(q, c.kv, i32(50, 1 << 30), True, 100, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=1, out=out)
+    ops.attention_q8(q, c.kv, i32(50, 1 << 30), True, 100, form=form, key_chunk=chunk, row_seq=i32(0, 1), seq_rows=1, out=out)
     assert ops.device_error() == 341 and torch.equal(out[0], good[0])
     before = c.codes.view(torch.uint8).clone()
     qkv = torch.randn(2, 8 * 128).bfloat16().to(DEV)
@@ -347,13 +347,13 @@ def test_out_of_range_rows_are_refused_on_the_device(page, chunk):
         pos = i32(cap - 1, cap - 2)
         ops.qkv_rope_append_q8(qkv, pos, w, w, torch.ones(64, device=DEV), c.kv, 4, 128, 1e-6, row_seq=i32(0, 1))
         assert ops.device_error() == 342
-        ops.attention_q8(q, c.kv, pos, True, cap, row_seq=i32(0, 1), seq_rows=1, key_chunk=chunk)
+        ops.attention_q8(q, c.kv, pos, True, cap, row_seq=i32(0, 1), seq_rows=1, form=form, key_chunk=chunk)
         assert ops.device_error() == 342
     assert torch.equal(before, c.codes.view(torch.uint8))
 
 
-@pytest.mark.parametrize("chunk", [128, 512])
-def test_views_streams_and_graphs(chunk):
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+def test_views_streams_and_graphs(form, chunk):
     """Strided caches (one layer of a [seq, layer, ...] pool), strided outputs and gates, another
     stream, and two captured graphs replayed out of order."""
     from dflash_b200 import ops
@@ -375,7 +375,7 @@ def test_views_streams_and_graphs(chunk):
     outs = [torch.zeros(M, Hq * hd + 4, dtype=torch.bfloat16, device=DEV) for _ in range(L)]
 
     def call(l):
-        ops.attention_q8(dq, kvs[l], dp, True, cap, row_seq=ds, seq_rows=2, key_chunk=chunk, out=outs[l][:, :Hq * hd],
+        ops.attention_q8(dq, kvs[l], dp, True, cap, row_seq=ds, seq_rows=2, form=form, key_chunk=chunk, out=outs[l][:, :Hq * hd],
                          gate=dg[:, hd:], gate_head_stride=2 * hd)
 
     def check():
