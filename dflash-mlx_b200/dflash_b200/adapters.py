@@ -75,8 +75,8 @@ class TargetAdapter:
         eos = tokenizer.eos_token_ids
         return {eos} if isinstance(eos, int) else set(eos)
 
-    def make_cache(self, model, cap: int = 8192) -> TargetCache:
-        return TargetCache(model.make_cache(1, cap))
+    def make_cache(self, model, cap: int = 8192, kv_dtype: str = "bf16") -> TargetCache:
+        return TargetCache(model.make_cache(1, cap, dtype=kv_dtype))
 
     def embed_tokens(self, model: TargetModel, tokens: torch.Tensor) -> torch.Tensor:
         t = tokens.reshape(-1).to(model.device, torch.int32).contiguous()
@@ -160,8 +160,8 @@ class Qwen35TargetAdapter(TargetAdapter):
 
     family = "qwen3_5"
 
-    def make_cache(self, model, cap: int = 8192, block: int = 16) -> TargetCache:
-        return TargetCache(model.make_cache(1, cap, block=block))
+    def make_cache(self, model, cap: int = 8192, block: int = 16, kv_dtype: str = "bf16") -> TargetCache:
+        return TargetCache(model.make_cache(1, cap, block=block, dtype=kv_dtype))
 
     def _forward_states(self, model, inputs: torch.Tensor, cache: TargetCache, layer_ids, records: bool):
         toks = inputs.reshape(-1).to(model.device, torch.int32).contiguous()
@@ -271,8 +271,8 @@ class LoadedTargetModel:
     def stop_token_ids(self) -> set[int]:
         return self.adapter.stop_token_ids(self.tokenizer)
 
-    def make_cache(self, cap: int = 8192):
-        return self.adapter.make_cache(self.model, cap)
+    def make_cache(self, cap: int = 8192, kv_dtype: str = "bf16"):
+        return self.adapter.make_cache(self.model, cap, kv_dtype=kv_dtype)
 
     def embed_tokens(self, tokens):
         return self.adapter.embed_tokens(self.model, tokens)

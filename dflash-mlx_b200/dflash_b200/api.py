@@ -10,7 +10,7 @@ import torch
 
 from .adapters import LoadedTargetModel, load_target_model
 from .config import PRESETS
-from .model import DraftModel
+from .model import DraftModel, kv_dtype as _kv_dtype
 from .runtime import dflash_generate, dflash_generate_stream
 from .weights import random_draft_weights
 
@@ -128,7 +128,10 @@ def maybe_quantize_draft_model(draft: DraftCheckpoint, bits: int | None, group_s
 class DFlashGenerator:
     def __init__(self, target_model=DEFAULT_TARGET_MODEL, draft_model=DEFAULT_DRAFT_MODEL,
                  draft_attention_mask: str = "auto", draft_quant_bits: int | None = None,
-                 draft_quant_group_size: int = 64, seed: int = 0, device: str = "cuda"):
+                 draft_quant_group_size: int = 64, seed: int = 0, device: str = "cuda", kv_dtype: str = "bf16"):
+        """kv_dtype: "bf16", or "int8" / "e4m3" to hold the K/V caches in 8 bits."""
+        _kv_dtype(kv_dtype)
+        self.kv_dtype = kv_dtype
         torch.manual_seed(seed)
         self.seed = int(seed)  # default sampling seed of generate / stream
         self.requested_target_model = target_model
@@ -169,7 +172,7 @@ class DFlashGenerator:
             temperature=temperature, stop_token_ids=self.target.stop_token_ids(),
             layer_ids=self.draft.target_layer_ids, speculative_tokens=speculative_tokens, verify_mode=verify_mode,
             verify_chunk_size=verify_chunk_size, profile=profile,
-            seed=self.seed if seed is None else seed)
+            seed=self.seed if seed is None else seed, kv_dtype=self.kv_dtype)
         generated = output_tokens[metrics["num_input_tokens"]:]
         text = self.target.tokenizer.decode(generated, skip_special_tokens=skip_special_tokens)
         return DFlashResult(text=text, output_tokens=output_tokens, generated_tokens=generated, metrics=metrics)
@@ -188,7 +191,8 @@ class DFlashGenerator:
                 target=self.target.model, draft=self.draft, prompt_tokens=prompt_tokens,
                 max_new_tokens=max_new_tokens, temperature=temperature, stop_token_ids=self.target.stop_token_ids(),
                 layer_ids=self.draft.target_layer_ids, speculative_tokens=speculative_tokens, verify_mode=verify_mode,
-                verify_chunk_size=verify_chunk_size, profile=profile, seed=self.seed if seed is None else seed):
+                verify_chunk_size=verify_chunk_size, profile=profile, seed=self.seed if seed is None else seed,
+                kv_dtype=self.kv_dtype):
             generated = event.output_tokens[prompt_len:]
             text = self.target.tokenizer.decode(generated, skip_special_tokens=skip_special_tokens)
             delta = text[len(decoded):] if text.startswith(decoded) else text

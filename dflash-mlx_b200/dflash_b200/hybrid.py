@@ -28,7 +28,7 @@ import torch
 
 from . import ops
 from .config import TargetConfig
-from .model import KVCache, alloc_kv
+from .model import KVCache, alloc_kv, kv_dtype
 from .weights import pack_gate_up, rope_inv_freq
 
 
@@ -119,16 +119,17 @@ class HybridTargetModel:
 
     # ------------------------------------------------------------------
     def make_cache(self, batch: int, cap: int, block: int = 16, window_rows: int = 128,
-                   rollback: str = "snapshot") -> HybridCache:
+                   rollback: str = "snapshot", dtype: str = "bf16") -> HybridCache:
         """rollback="snapshot": the verify forward writes the state after every token
         (a rollback is a copy; the adapter contract's "advance the whole block, then roll
         back" needs it). rollback="replay": the verify forward keeps the block's k, v, g,
         beta and the rollback re-advances the state over each sequence's accepted prefix
-        (the reference's own method, adapters.py:505-560): T-fold less state traffic."""
+        (the reference's own method, adapters.py:505-560): T-fold less state traffic.
+        dtype: "bf16", "int8" or "e4m3" K/V of the attention layers."""
         if rollback not in ("snapshot", "replay"):
             raise ValueError(f"rollback must be 'snapshot' or 'replay', not {rollback!r}")
         c, dev = self.cfg, self.device
-        kv = alloc_kv(max(1, len(self.attn_index)), batch, c.num_key_value_heads, cap, c.head_dim, dev)
+        kv = alloc_kv(max(1, len(self.attn_index)), batch, c.num_key_value_heads, cap, c.head_dim, dev, kv_dtype(dtype))
         n = len(self.gdn_index)
         S = (self.Hv, self.Dv, self.Dk)
         Tw = max(block, window_rows)
@@ -249,7 +250,7 @@ class HybridTargetModel:
                 layer_ids: list[int] | None = None, taps_out: torch.Tensor | None = None,
                 row_seq: torch.Tensor | None = None, head: str = "argmax", ws: ops.Workspace | None = None,
                 seqs: slice | None = None, verify: bool = True, T: int | None = None, seq_rows: int = 0,
-                key_chunk: int = 0):
+                key_chunk: int = 0, form: str | None = None):
         """Block forward over M = B_s * T rows of sequences ``seqs`` (default: all, T = M / B).
         verify=True writes per-token snapshots + the conv window (a later dfl_gdn_rollback
         picks the accepted prefix); verify=False advances the GDN state in place (prefill)
@@ -272,14 +273,13 @@ class HybridTargetModel:
                 xn = self._gdn_layer(lw, h, ss, b, cache, self.gdn_index[l], seqs, T, verify, ws, xn=xn,
                                      next_norm=lw["post_norm"])
             else:
-                kc, vc = cache.kv.layer(self.attn_index[l])
+                ai = self.attn_index[l]
                 self._normed_gemm(h, xn, lw["w_qkv"], lw["in_norm"], ss, ws, out=b["qkv"])
                 qkv = b["qkv"][:, :(2 * Hq + 2 * Hkv) * hd]
-                ops.qkv_rope_append(qkv, pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, Hq, Hkv, hd,
-                                    c.rope_dim, eps, q_out=b["q"], row_seq=row_seq, q_stride=2 * hd)
-                ops.attention(b["q"], kc, vc, pos, causal=True, max_kv=max_kv, row_seq=row_seq, out=b["attn"],
-                              seq_rows=seq_rows or T, key_chunk=key_chunk,
-                              ws=ws, gate=qkv[:, hd:], gate_head_stride=2 * hd)
+                cache.kv.append(ai, qkv, pos, lw, self.inv_freq, Hq, Hkv, hd, c.rope_dim, eps, q_out=b["q"],
+                                row_seq=row_seq, q_stride=2 * hd)
+                cache.kv.attend(ai, b["q"], pos, True, max_kv, row_seq=row_seq, out=b["attn"], seq_rows=seq_rows or T,
+                                key_chunk=key_chunk, form=form, ws=ws, gate=qkv[:, hd:], gate_head_stride=2 * hd)
                 xn = self._row_parallel(b["attn"], lw["w_o"], h, ss, None, ws, parity=0, next_norm=lw["post_norm"],
                                         xn_out=b["xtp"])
             self._normed_gemm(h, xn, lw["w_gu"], lw["post_norm"], ss, ws, ops.EPI_SILU_MUL, out=b["act"])

@@ -35,13 +35,27 @@ class KVCache:
     position p of sequence b in slot p) or, with a page table, page pools
     [L, n_pages, Hkv, page_size, hd] and ``page_table`` [B, pages] int32 (position p of
     sequence b in page page_table[b, p // page_size], row p % page_size), so that each
-    sequence holds pages for its own length only."""
+    sequence holds pages for its own length only. With ``k_scale`` / ``v_scale`` (fp32, the
+    codes' shape without hd) K and V are held in 8 bits, int8 or float8_e4m3fn codes with one
+    scale per position and head (ops.QuantKV)."""
 
     k: torch.Tensor
     v: torch.Tensor
     page_table: torch.Tensor | None = None
     page_size: int = 0
     cap_tokens: int = 0
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+
+    def __post_init__(self):
+        # one handle per layer, checked once
+        self._q8 = [] if self.k_scale is None else [
+            ops.QuantKV(self.k[l], self.v[l], self.k_scale[l], self.v_scale[l], page_table=self.page_table,
+                        page_size=self.page_size) for l in range(self.k.shape[0])]
+
+    @property
+    def quantized(self) -> bool:
+        return self.k_scale is not None
 
     @property
     def cap(self) -> int:
@@ -58,7 +72,11 @@ class KVCache:
         return {"page_table": self.page_table, "page_size": self.page_size}
 
     def gather(self, l: int, b: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values of positions [0, n) of sequence b in layer l, as [Hkv, n, hd]."""
+        """Keys and values of positions [0, n) of sequence b in layer l, as [Hkv, n, hd] (bf16)."""
+        if self.quantized:
+            pos = torch.arange(n, dtype=torch.int32, device=self.k.device)
+            k, v = ops.kv_read_q8(self._q8[l], pos, row_seq=torch.full_like(pos, b))
+            return k.transpose(0, 1), v.transpose(0, 1)
         if self.page_table is None:
             return self.k[l, b, :, :n], self.v[l, b, :, :n]
         ps = self.page_size
@@ -68,10 +86,68 @@ class KVCache:
         return k, v
 
 
-def alloc_kv(n_layers: int, batch: int, n_kv: int, cap: int, hd: int, device) -> KVCache:
-    shape = (n_layers, batch, n_kv, cap, hd)
-    return KVCache(torch.zeros(shape, dtype=torch.bfloat16, device=device),
-                   torch.zeros(shape, dtype=torch.bfloat16, device=device))
+    def append(self, l: int, qkv, pos, lw: dict, inv_freq, Hq: int, Hkv: int, hd: int, rot_dim: int, eps: float,
+               q_out=None, row_seq=None, q_stride: int | None = None, do_q: bool = True) -> None:
+        """q/k head norm + RoPE of projection rows and their append to layer l, in the cache's type."""
+        if self.quantized:
+            ops.qkv_rope_append_q8(qkv, pos, lw["q_norm"], lw["k_norm"], inv_freq, self._q8[l], Hq, rot_dim, eps,
+                                   q_out=q_out, row_seq=row_seq, q_stride=q_stride, do_q=do_q)
+        else:
+            ops.qkv_rope_append(qkv, pos, lw["q_norm"], lw["k_norm"], inv_freq, self.k[l], self.v[l], Hq, Hkv, hd,
+                                rot_dim, eps, q_out=q_out, row_seq=row_seq, q_stride=q_stride, do_q=do_q,
+                                **self.paging)
+
+    def attend(self, l: int, q, pos, causal: bool, max_kv: int, kv_len=None, row_seq=None, out=None, ws=None,
+               gate=None, gate_head_stride: int = 0, seq_rows: int = 0, key_chunk: int = 0,
+               form: str | None = None) -> torch.Tensor:
+        """Attention over layer l. An 8-bit cache without a ``form`` splits as (warp, 128 keys),
+        whatever the rows are, as the bf16 attention does by default."""
+        if self.quantized:
+            if form is None:
+                form, key_chunk = "warp", key_chunk or ops.Q8_CHUNK
+            return ops.attention_q8(q, self._q8[l], pos, causal, max_kv, kv_len=kv_len, row_seq=row_seq, out=out,
+                                    ws=ws, gate=gate, gate_head_stride=gate_head_stride, seq_rows=seq_rows,
+                                    key_chunk=key_chunk, form=form)
+        return ops.attention(q, self.k[l], self.v[l], pos, causal=causal, max_kv=max_kv, kv_len=kv_len,
+                             row_seq=row_seq, out=out, ws=ws, gate=gate, gate_head_stride=gate_head_stride,
+                             seq_rows=seq_rows, key_chunk=key_chunk, **self.paging)
+
+
+KV_DTYPES = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+
+
+def kv_dtype(name: str) -> torch.dtype:
+    """The K/V cache type of a kv_dtype argument ("bf16", "int8" or "e4m3")."""
+    if name not in KV_DTYPES:
+        raise ValueError(f"kv_dtype must be one of {tuple(KV_DTYPES)}, not {name!r}")
+    return KV_DTYPES[name]
+
+
+def _zero_kv(shape: tuple, dtype: torch.dtype, device) -> dict:
+    """Zeroed K/V (and, in 8 bits, scales) of the given shape, as KVCache fields."""
+    if dtype == torch.bfloat16:
+        return {n: torch.zeros(shape, dtype=dtype, device=device) for n in ("k", "v")}
+    out = {n: torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for n in ("k", "v")}
+    out.update({n: torch.zeros(shape[:-1], dtype=torch.float32, device=device) for n in ("k_scale", "v_scale")})
+    return out
+
+
+def alloc_kv(n_layers: int, batch: int, n_kv: int, cap: int, hd: int, device,
+             dtype: torch.dtype = torch.bfloat16) -> KVCache:
+    return KVCache(**_zero_kv((n_layers, batch, n_kv, cap, hd), dtype, device))
+
+
+def q8_split(batch: int, n_kv: int, max_total: int) -> tuple[str, int]:
+    """(form, keys per split) of a session's attention over an 8-bit cache. It depends on what a
+    session's plain and speculative decode share (sequences, kv heads, total length), so that
+    their rows agree bit for bit. One short stream: 128 keys a CTA on as many SMs as there are; else
+    the tcgen05 form, in splits that give each SM about two CTAs, a power of two."""
+    if batch < 4 and max_total * batch * n_kv <= 65536:
+        return "warp", ops.Q8_CHUNK
+    chunk = 512
+    while chunk < 8192 and chunk * 296 < max_total * batch * n_kv:
+        chunk *= 2
+    return "tc", chunk
 
 
 PAGE_SIZE = 64
@@ -116,16 +192,15 @@ def page_plan(lengths: list[int], page_size: int = PAGE_SIZE) -> tuple[torch.Ten
 
 
 def alloc_kv_paged(n_layers: int, lengths: list[int], n_kv: int, hd: int, device,
-                   page_table: torch.Tensor | None = None, page_size: int = PAGE_SIZE) -> KVCache:
+                   page_table: torch.Tensor | None = None, page_size: int = PAGE_SIZE,
+                   dtype: torch.dtype = torch.bfloat16) -> KVCache:
     """Paged K/V for sequences of the given lengths (one shared page table may serve
     several caches: pass the device table of a previous call)."""
     table, n_pages = page_plan(lengths, page_size)
     if page_table is None:
         page_table = table.to(device)
-    shape = (n_layers, n_pages, n_kv, page_size, hd)
-    return KVCache(torch.zeros(shape, dtype=torch.bfloat16, device=device),
-                   torch.zeros(shape, dtype=torch.bfloat16, device=device), page_table, page_size,
-                   max(lengths) if lengths else 0)
+    return KVCache(**_zero_kv((n_layers, n_pages, n_kv, page_size, hd), dtype, device), page_table=page_table,
+                   page_size=page_size, cap_tokens=max(lengths) if lengths else 0)
 
 
 class TargetModel:
@@ -166,14 +241,16 @@ class TargetModel:
 
     # ------------------------------------------------------------------
     def make_cache(self, batch: int, cap: int, block: int = 16, lengths: list[int] | None = None,
-                   page_table: torch.Tensor | None = None) -> KVCache:
+                   page_table: torch.Tensor | None = None, dtype: str = "bf16") -> KVCache:
         """Contiguous [L, batch, Hkv, cap, hd] slots, or, given each sequence's length,
-        a paged cache holding pages for those lengths only."""
+        a paged cache holding pages for those lengths only; in bf16 or 8 bits (``dtype``: "bf16",
+        "int8", "e4m3")."""
         c = self.cfg
         if lengths is not None:
             return alloc_kv_paged(c.num_hidden_layers, lengths, c.num_key_value_heads, c.head_dim, self.device,
-                                  page_table)
-        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device)
+                                  page_table, dtype=kv_dtype(dtype))
+        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device,
+                        kv_dtype(dtype))
 
     def buffers(self, M: int) -> dict[str, torch.Tensor]:
         b = self._bufs.get(M)
@@ -198,7 +275,7 @@ class TargetModel:
     def forward(self, tokens: torch.Tensor, pos: torch.Tensor, cache: KVCache, max_kv: int,
                 layer_ids: list[int] | None = None, taps_out: torch.Tensor | None = None,
                 row_seq: torch.Tensor | None = None, head: str = "argmax", ws: ops.Workspace | None = None,
-                seq_rows: int = 0, key_chunk: int = 0):
+                seq_rows: int = 0, key_chunk: int = 0, form: str | None = None):
         """Block forward over M rows (tokens int32 [M] at positions pos [M]).
 
         Appends K/V at each row's position, writes the residual stream after each
@@ -220,13 +297,13 @@ class TargetModel:
         h, ss = b["h"], b["ss"]
         eps = c.rms_norm_eps
         ops.embed(tokens, self.embed_w, out=h, sumsq_out=ss)
-        fused = (self.fuse_attention and cache.page_table is None
+        fused = (self.fuse_attention and cache.page_table is None and not cache.quantized
                  and ops.fused_attention_ok(M, row_seq, seq_rows, hd, c.rope_dim))
         pg = cache.paging
         if self.use_chain and chain_ok(M, ws):
             return self._forward_chain(pos, cache, max_kv, tap_col, taps_out, row_seq, head, ws, seq_rows, key_chunk,
-                                       fused, b)
-        qkv_rope = not fused and qkv_rope_ok(ws, hd, c.rope_dim)
+                                       fused, b, form)
+        qkv_rope = not fused and not cache.quantized and qkv_rope_ok(ws, hd, c.rope_dim)
         for l, lw in enumerate(self.layers):
             kc, vc = cache.layer(l)
             if qkv_rope:  # input_layernorm, QKV projection, q/k norm + RoPE + append: one call
@@ -241,10 +318,10 @@ class TargetModel:
                                   key_chunk=key_chunk)
             else:
                 if not qkv_rope:
-                    ops.qkv_rope_append(b["qkv"], pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, Hq, Hkv,
-                                        hd, c.rope_dim, eps, q_out=b["q"], row_seq=row_seq, **pg)
-                ops.attention(b["q"], kc, vc, pos, causal=True, max_kv=max_kv, row_seq=row_seq, out=b["attn"],
-                              ws=ws, seq_rows=seq_rows, key_chunk=key_chunk, **pg)
+                    cache.append(l, b["qkv"], pos, lw, self.inv_freq, Hq, Hkv, hd, c.rope_dim, eps, q_out=b["q"],
+                                 row_seq=row_seq)
+                cache.attend(l, b["q"], pos, True, max_kv, row_seq=row_seq, out=b["attn"], ws=ws, seq_rows=seq_rows,
+                             key_chunk=key_chunk, form=form)
             ops.gemm(b["attn"], lw["w_o"], ops.EPI_RESIDUAL, residual=h, out=h, ws=ws, sumsq_out=ss)
             # post_attention_layernorm fused into the gate/up projection
             ops.gemm(h, lw["w_gu"], ops.EPI_SILU_MUL, out=b["act"], ws=ws, norm_w=lw["post_norm"], sumsq_in=ss,
@@ -261,7 +338,8 @@ class TargetModel:
         return ops.gemm(h, self.lm_head_w, ops.EPI_ARGMAX, argmax_partials=b["argmax"], ws=ws, norm_w=self.norm_w,
                         sumsq_in=ss, eps=eps)
 
-    def _forward_chain(self, pos, cache, max_kv, tap_col, taps_out, row_seq, head, ws, seq_rows, key_chunk, fused, b):
+    def _forward_chain(self, pos, cache, max_kv, tap_col, taps_out, row_seq, head, ws, seq_rows, key_chunk, fused, b,
+                       form=None):
         """forward() with every run of projections between two attention calls as one
         GEMM-chain launch: [qkv_0], then per layer [o, gate/up, down, next qkv or lm_head]."""
         c = self.cfg
@@ -279,10 +357,10 @@ class TargetModel:
                                   max_kv, row_seq=row_seq, out=b["attn"], ws=ws, seq_rows=seq_rows,
                                   key_chunk=key_chunk)
             else:
-                ops.qkv_rope_append(b["qkv"], pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, Hq, Hkv, hd,
-                                    c.rope_dim, eps, q_out=b["q"], row_seq=row_seq, **pg)
-                ops.attention(b["q"], kc, vc, pos, causal=True, max_kv=max_kv, row_seq=row_seq, out=b["attn"],
-                              ws=ws, seq_rows=seq_rows, key_chunk=key_chunk, **pg)
+                cache.append(l, b["qkv"], pos, lw, self.inv_freq, Hq, Hkv, hd, c.rope_dim, eps, q_out=b["q"],
+                             row_seq=row_seq)
+                cache.attend(l, b["q"], pos, True, max_kv, row_seq=row_seq, out=b["attn"], ws=ws, seq_rows=seq_rows,
+                             key_chunk=key_chunk, form=form)
             tap = None
             if l in tap_col and taps_out is not None:
                 tap = taps_out[:, tap_col[l] * H:(tap_col[l] + 1) * H]
@@ -434,12 +512,13 @@ class DraftModel:
         return list(self.cfg.target_layer_ids)
 
     def make_cache(self, batch: int, cap: int, lengths: list[int] | None = None,
-                   page_table: torch.Tensor | None = None) -> KVCache:
+                   page_table: torch.Tensor | None = None, dtype: str = "bf16") -> KVCache:
         c = self.cfg
         if lengths is not None:
             return alloc_kv_paged(c.num_hidden_layers, lengths, c.num_key_value_heads, c.head_dim, self.device,
-                                  page_table)
-        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device)
+                                  page_table, dtype=kv_dtype(dtype))
+        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device,
+                        kv_dtype(dtype))
 
     def buffers(self, M: int, kind: str) -> dict[str, torch.Tensor]:
         key = (M, kind)
@@ -484,7 +563,7 @@ class DraftModel:
                                          sumsq_in=b["ss"], eps=c.rms_norm_eps)], ws)
         else:
             ops.gemm(taps, self.fc, out=b["fc"], ws=ws, sumsq_out=b["ss"])
-            if qkv_rope_ok(ws, hd, hd) and len(self.layers) <= ops.KV_LAYERS_MAX:
+            if qkv_rope_ok(ws, hd, hd) and len(self.layers) <= ops.KV_LAYERS_MAX and not cache.quantized:
                 # hidden_norm, the stacked k/v projection of every layer and each layer's
                 # k_norm + RoPE + append: one call (the same bits as the calls below)
                 ops.gemm_kv_append_layers(b["fc"], self.w_ctx_kv, b["kv"], pos, [lw["k_norm"] for lw in self.layers],
@@ -497,14 +576,13 @@ class DraftModel:
                      eps=c.rms_norm_eps)
         per = 2 * Hkv * hd
         for l, lw in enumerate(self.layers):
-            kc, vc = cache.layer(l)
-            view = b["kv"][:, l * per:(l + 1) * per]
-            ops.qkv_rope_append(view, pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, 0, Hkv, hd, hd,
-                                c.rms_norm_eps, row_seq=row_seq, do_q=False, **cache.paging)
+            cache.append(l, b["kv"][:, l * per:(l + 1) * per], pos, lw, self.inv_freq, 0, Hkv, hd, hd, c.rms_norm_eps,
+                         row_seq=row_seq, do_q=False)
 
     def forward_block(self, tokens: torch.Tensor, pos: torch.Tensor, cache: KVCache, kv_len: torch.Tensor,
                       max_kv: int, row_seq: torch.Tensor | None = None, head: str = "argmax",
-                      ws: ops.Workspace | None = None, seq_rows: int = 0, key_chunk: int = 0):
+                      ws: ops.Workspace | None = None, seq_rows: int = 0, key_chunk: int = 0,
+                      form: str | None = None):
         """Block rows (the target embedding of [last, mask, ...] = the noise embedding,
         runtime.py:408-410) attend to the draft cache (context rows already ingested)
         plus the block itself; returns the lm_head argmax partials of the final-normed
@@ -523,11 +601,9 @@ class DraftModel:
             pending = [qkv_op(self.layers[0])] if self.layers else []
             for l, lw in enumerate(self.layers):
                 ops.gemm_chain(pending, ws)
-                kc, vc = cache.layer(l)
-                ops.qkv_rope_append(b["qkv"], pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, Hq, Hkv, hd,
-                                    hd, eps, q_out=b["q"], row_seq=row_seq, **cache.paging)
-                ops.attention(b["q"], kc, vc, pos, causal=causal, max_kv=max_kv, kv_len=kv_len, row_seq=row_seq,
-                              seq_rows=seq_rows, key_chunk=key_chunk, out=b["attn"], ws=ws, **cache.paging)
+                cache.append(l, b["qkv"], pos, lw, self.inv_freq, Hq, Hkv, hd, hd, eps, q_out=b["q"], row_seq=row_seq)
+                cache.attend(l, b["q"], pos, causal, max_kv, kv_len=kv_len, row_seq=row_seq, seq_rows=seq_rows,
+                             key_chunk=key_chunk, form=form, out=b["attn"], ws=ws)
                 pending = [ops.chain_op(b["attn"], lw["w_o"], ops.EPI_RESIDUAL, residual=h, out=h, sumsq_out=ss),
                            ops.chain_op(h, lw["w_gu"], ops.EPI_SILU_MUL, out=b["act"], norm_w=lw["post_norm"],
                                         sumsq_in=ss, eps=eps),
@@ -535,7 +611,7 @@ class DraftModel:
                 if l + 1 < len(self.layers):
                     pending.append(qkv_op(self.layers[l + 1]))
             return chain_head(pending, h, ss, self.target.lm_head_w, self.norm_w, eps, head, b, ws)
-        qkv_rope = qkv_rope_ok(ws, hd, hd)
+        qkv_rope = qkv_rope_ok(ws, hd, hd) and not cache.quantized
         for l, lw in enumerate(self.layers):
             kc, vc = cache.layer(l)
             if qkv_rope:  # QKV projection + q/k norm + RoPE + append in one call (same bits)
@@ -544,10 +620,9 @@ class DraftModel:
                                   ws=ws, **cache.paging)
             else:
                 ops.gemm(h, lw["w_qkv"], out=b["qkv"], ws=ws, norm_w=lw["in_norm"], sumsq_in=ss, eps=eps)
-                ops.qkv_rope_append(b["qkv"], pos, lw["q_norm"], lw["k_norm"], self.inv_freq, kc, vc, Hq, Hkv, hd,
-                                    hd, eps, q_out=b["q"], row_seq=row_seq, **cache.paging)
-            ops.attention(b["q"], kc, vc, pos, causal=causal, max_kv=max_kv, kv_len=kv_len, row_seq=row_seq,
-                          seq_rows=seq_rows, key_chunk=key_chunk, out=b["attn"], ws=ws, **cache.paging)
+                cache.append(l, b["qkv"], pos, lw, self.inv_freq, Hq, Hkv, hd, hd, eps, q_out=b["q"], row_seq=row_seq)
+            cache.attend(l, b["q"], pos, causal, max_kv, kv_len=kv_len, row_seq=row_seq, seq_rows=seq_rows,
+                         key_chunk=key_chunk, form=form, out=b["attn"], ws=ws)
             ops.gemm(b["attn"], lw["w_o"], ops.EPI_RESIDUAL, residual=h, out=h, ws=ws, sumsq_out=ss)
             ops.gemm(h, lw["w_gu"], ops.EPI_SILU_MUL, out=b["act"], ws=ws, norm_w=lw["post_norm"], sumsq_in=ss,
                      eps=eps)

@@ -151,10 +151,12 @@ class DFlashRunner(RunnerProtocol):
     """One request at a time through ``DFlashGenerator`` (openai_server.py:170-265)."""
 
     def __init__(self, *, target_model: str = "", draft_model: str = "", speculative_tokens: int | None = None,
-                 verify_mode: str = "parallel-replay", verify_chunk_size: int = 4, seed: int = 0, generator=None):
+                 verify_mode: str = "parallel-replay", verify_chunk_size: int = 4, seed: int = 0, generator=None,
+                 kv_dtype: str = "bf16"):
         if generator is None:
             from .api import DFlashGenerator
-            generator = DFlashGenerator(target_model=target_model, draft_model=draft_model, seed=seed)
+            generator = DFlashGenerator(target_model=target_model, draft_model=draft_model, seed=seed,
+                                        kv_dtype=kv_dtype)
         self.generator = generator
         self.speculative_tokens = speculative_tokens
         self.verify_mode = verify_mode
@@ -212,7 +214,8 @@ class BatchingRunner(RunnerProtocol):
                 g = self.generator
                 return dflash_generate_batch_stream(g.target.model, g.draft, prompts, max_new, temperature,
                                                     g.target.stop_token_ids(), self.speculative_tokens,
-                                                    seed=getattr(g, "seed", 0))
+                                                    seed=getattr(g, "seed", 0),
+                                                    kv_dtype=getattr(g, "kv_dtype", "bf16"))
         self._decode = decode_fn
         self._queue: queue.Queue = queue.Queue()
         self._stop = threading.Event()
@@ -428,6 +431,8 @@ def parse_args(argv: list[str] | None = None) -> argparse.Namespace:
                     choices=["stream", "chunked", "parallel-replay", "parallel-lazy-logits", "parallel-greedy-argmax"])
     ap.add_argument("--verify-chunk-size", type=int, default=4)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--kv-dtype", default="bf16", choices=["bf16", "int8", "e4m3"],
+                    help="type of the K/V caches; 8 bits halve their memory and attention traffic")
     ap.add_argument("--max-batch", type=int, default=16,
                     help="requests decoded together (1 = one request at a time, as the reference)")
     ap.add_argument("--batch-window-ms", type=float, default=5.0,
@@ -439,13 +444,14 @@ def main(argv: list[str] | None = None) -> None:
     args = parse_args(argv)
     if args.max_batch > 1:
         from .api import DFlashGenerator
-        gen = DFlashGenerator(target_model=args.target_model, draft_model=args.draft_model, seed=args.seed)
+        gen = DFlashGenerator(target_model=args.target_model, draft_model=args.draft_model, seed=args.seed,
+                              kv_dtype=args.kv_dtype)
         runner: RunnerProtocol = BatchingRunner(gen, max_batch=args.max_batch, window_s=args.batch_window_ms / 1e3,
                                                 speculative_tokens=args.max_speculative_tokens)
     else:
         runner = DFlashRunner(target_model=args.target_model, draft_model=args.draft_model,
                               speculative_tokens=args.max_speculative_tokens, verify_mode=args.verify_mode,
-                              verify_chunk_size=args.verify_chunk_size, seed=args.seed)
+                              verify_chunk_size=args.verify_chunk_size, seed=args.seed, kv_dtype=args.kv_dtype)
     config = ServerConfig(host=args.host, port=args.port, model_id=args.model_id, runner=runner)
     server = make_server(config)
     print(f"Serving DFlash OpenAI-compatible API on http://{config.host}:{config.port}")

@@ -458,6 +458,7 @@ class KvQ8(ctypes.Structure):
                 ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("type", ctypes.c_int)]
 
 
+Q8_CHUNK = 128  # the unit of attention_q8's key_chunk
 Q8_FORMS = {"auto": 0, "warp": 1, "tc": 2}  # DFL_Q8_AUTO, DFL_Q8_WARP, DFL_Q8_TC
 KV_Q8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # DFL_KV_INT8, DFL_KV_E4M3
 

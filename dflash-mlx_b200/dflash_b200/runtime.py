@@ -24,7 +24,7 @@ from typing import Any
 import torch
 
 from . import ops
-from .model import DraftModel, TargetModel
+from .model import DraftModel, TargetModel, kv_dtype as _kv_dtype, q8_split
 
 STATE_INTS = 16  # sizeof(dfl_seq_state) / 4
 S_START, S_PENDING, S_DRAFT_LEN, S_ACCEPTED, S_BONUS, S_FINISHED, S_STOP, S_STEPS, S_TOTAL, S_PROMPT = range(10)
@@ -83,8 +83,12 @@ class SpecSession:
     def __init__(self, target: TargetModel, draft: DraftModel | None, batch: int, max_total: int,
                  block_size: int, stop_token_ids: set[int] | None = None, use_graph: bool = True,
                  max_steps: int | None = None, prefill_chunk: int = 128, temperature: float = 0.0,
-                 seed: int = 0, profile: bool = False, paged: bool = True):
-        """temperature >= 1e-5 samples (Gumbel-max on the bf16 logits, keyed by sequence and
+                 seed: int = 0, profile: bool = False, paged: bool = True, kv_dtype: str = "bf16"):
+        """kv_dtype: "bf16", or "int8" / "e4m3" to hold the target's and the draft's K/V in 8 bits
+        (half the cache memory and attention traffic; tokens then follow the rounded cache, and
+        speculative and plain decode of one kv_dtype still agree token for token).
+
+        temperature >= 1e-5 samples (Gumbel-max on the bf16 logits, keyed by sequence and
         absolute position: the speculative decode reproduces the plain sampled decode of the
         same seed token for token); below it decoding is greedy (fused lm_head argmax)."""
         self.sampled = temperature >= 1e-5
@@ -115,6 +119,14 @@ class SpecSession:
         self.batched = batch >= 4
         self.key_chunk = 1024 if self.batched else 64
         self.out_cap = self.cap
+        _kv_dtype(kv_dtype)  # refuses an unknown name before anything is allocated
+        self.kv_dtype = kv_dtype
+        # an 8-bit cache's attention: form and keys per split of the steps and of the prefill chunks
+        self.step_split, self.prefill_split = {"key_chunk": self.key_chunk}, {"key_chunk": self.key_chunk}
+        if kv_dtype != "bf16":
+            form, chunk = q8_split(batch, tc.num_key_value_heads, max_total)
+            self.step_split = {"form": form, "key_chunk": chunk}
+            self.prefill_split = {"form": "tc", "key_chunk": 1024}
         self.max_steps = max_steps or (max_total + 1)
         # under 16 sequences, weights with few 128-row tiles also split K (fixed ranges)
         self.ws = ops.Workspace(self.dev, wide=self.batched, wide_split=4 if batch < 16 else 1)
@@ -139,15 +151,15 @@ class SpecSession:
         self.paged = paged and not self.hybrid
         self.tcache = None
         if self.hybrid:
-            self.tcache = target.make_cache(B, self.cap, block=bs, rollback="replay")
+            self.tcache = target.make_cache(B, self.cap, block=bs, rollback="replay", dtype=kv_dtype)
         elif not self.paged:
-            self.tcache = target.make_cache(B, self.cap, block=bs)
+            self.tcache = target.make_cache(B, self.cap, block=bs, dtype=kv_dtype)
         self.layer_ids = sorted(draft.target_layer_ids) if draft is not None else []
         ntaps = max(1, len(self.layer_ids))
         self.taps = torch.zeros((B * bs, ntaps * tc.hidden_size), dtype=torch.bfloat16, device=dev)
         self.dcache = None
         if draft is not None and not self.paged:
-            self.dcache = draft.make_cache(B, self.cap)
+            self.dcache = draft.make_cache(B, self.cap, dtype=kv_dtype)
         self.inject_tokens = self.inject_len = self.inject_noise = None
         self.graph: torch.cuda.CUDAGraph | None = None
         self.host_state = torch.zeros((B, STATE_INTS), dtype=torch.int32, pin_memory=True)
@@ -175,6 +187,14 @@ class SpecSession:
                                                    ops.wide_split(N, K, self.ws))))
             attn_need = max(attn_need, int(q("dfl_attention_workspace_bytes", M, tc.num_attention_heads,
                                                tc.head_dim, self.cap, self.key_chunk)))
+        if self.kv_dtype != "bf16":
+            for cfg in [tc] + ([self.draft.cfg] if self.draft is not None else []):
+                desc = ops.KvQ8(n_kv_heads=cfg.num_key_value_heads, head_dim=cfg.head_dim)
+                for M, rows, split in ((shapes[0], self.bs, self.step_split),
+                                       (shapes[1], shapes[1], self.prefill_split)):
+                    attn_need = max(attn_need, int(q("dfl_attention_q8_workspace_bytes", ops.ctypes.byref(desc), M,
+                                                     cfg.num_attention_heads, rows, int(M == rows), self.cap,
+                                                     ops.Q8_FORMS[split["form"]], split["key_chunk"])))
         self.ws.ensure_gemm(gemm_need)
         self.ws.ensure_attn(attn_need)
         if self.ws.wide:
@@ -202,9 +222,10 @@ class SpecSession:
             # pages for each sequence's own length (prompt + new tokens + two blocks of slack:
             # the bound the capacity check below applies)
             lengths = [min(self.cap, len(p) + m + 2 * self.bs + 1) for p, m in zip(prompts, max_new_tokens)]
-            self.tcache = self.target.make_cache(B, self.cap, block=self.bs, lengths=lengths)
+            self.tcache = self.target.make_cache(B, self.cap, block=self.bs, lengths=lengths, dtype=self.kv_dtype)
             if self.draft is not None:
-                self.dcache = self.draft.make_cache(B, self.cap, lengths=lengths, page_table=self.tcache.page_table)
+                self.dcache = self.draft.make_cache(B, self.cap, lengths=lengths, page_table=self.tcache.page_table,
+                                                    dtype=self.kv_dtype)
             self.graph = None  # a recorded step holds the previous caches' pointers
         firsts = []
         st = torch.zeros((B, STATE_INTS), dtype=torch.int32)
@@ -228,14 +249,13 @@ class SpecSession:
                     # recurrent layers advance in place over the chunk; conv state from the window
                     part = self.target.forward(toks[c0:c1], pos, self.tcache, max_kv=c1, layer_ids=self.layer_ids,
                                                taps_out=taps, row_seq=rs, ws=self.ws, seqs=slice(b, b + 1),
-                                               verify=False, T=n, seq_rows=n, key_chunk=self.key_chunk,
-                                               head=head)
+                                               verify=False, T=n, seq_rows=n, head=head, **self.prefill_split)
                     self.target.commit_prefill(self.tcache, slice(b, b + 1),
                                                torch.full((1,), n, dtype=torch.int32, device=dev), n)
                 else:
                     part = self.target.forward(toks[c0:c1], pos, self.tcache, max_kv=c1, layer_ids=self.layer_ids,
-                                               taps_out=taps, row_seq=rs, ws=self.ws, seq_rows=n,
-                                               key_chunk=self.key_chunk, head=head)
+                                               taps_out=taps, row_seq=rs, ws=self.ws, seq_rows=n, head=head,
+                                               **self.prefill_split)
                 if self.sampled:  # part holds logits: sample the token at position P
                     key = ops.keys_tensor([ops.sample_key(self.seed, ops.SAMPLE_TAG_TARGET, b, P)], dev)
                     last_part = ops.sample_partials(part[n - 1:n], key, self.temperature)
@@ -274,8 +294,8 @@ class SpecSession:
             d = self.draft
             d.ingest_context(self.taps, self.dpos_ctx, self.dcache, row_seq=self.row_seq, ws=self.ws)
             part = d.forward_block(self.block, self.dpos_blk, self.dcache, self.dkv_len, self.cap,
-                                   row_seq=self.row_seq, ws=self.ws, seq_rows=bs, key_chunk=self.key_chunk,
-                                   head="logits" if self.sampled else "argmax")
+                                   row_seq=self.row_seq, ws=self.ws, seq_rows=bs,
+                                   head="logits" if self.sampled else "argmax", **self.step_split)
             if self.sampled:  # draft row i proposes the token at position start + i
                 ops.sample_keys(self.state, B, bs, self.seed, ops.SAMPLE_TAG_DRAFT, 0, self.keys)
                 part = ops.sample_partials(part, self.keys, self.temperature, out=self.spart)
@@ -291,7 +311,7 @@ class SpecSession:
     def _verify_forward(self) -> None:
         part = self.target.forward(self.block, self.tpos, self.tcache, max_kv=self.cap, layer_ids=self.layer_ids,
                                    taps_out=self.taps, row_seq=self.row_seq, ws=self.ws, seq_rows=self.bs,
-                                   key_chunk=self.key_chunk, head="logits" if self.sampled else "argmax")
+                                   head="logits" if self.sampled else "argmax", **self.step_split)
         if self.sampled:  # verify row i predicts the token at position start + i + 1
             ops.sample_keys(self.state, self.B, self.bs, self.seed, ops.SAMPLE_TAG_TARGET, 1, self.keys)
             part = ops.sample_partials(part, self.keys, self.temperature, out=self.spart)
@@ -438,7 +458,8 @@ def dflash_generate_stream(target: TargetModel, draft: DraftModel, prompt_tokens
                            temperature: float, stop_token_ids: set[int], layer_ids: list[int] | None,
                            speculative_tokens: int | None, verify_mode: str = "parallel-replay",
                            verify_chunk_size: int = 4, profile: bool = False,
-                           use_graph: bool = True, seed: int = 0) -> Iterator[DFlashRuntimeEvent]:
+                           use_graph: bool = True, seed: int = 0,
+                           kv_dtype: str = "bf16") -> Iterator[DFlashRuntimeEvent]:
     """Single-sequence generator with the reference's event and metrics shape (runtime.py:360-555).
     temperature >= 1e-5 samples (sample_tokens, runtime.py:22-29) with noise keyed by
     ``seed`` and absolute position, so the output equals the plain sampled decode."""
@@ -454,7 +475,7 @@ def dflash_generate_stream(target: TargetModel, draft: DraftModel, prompt_tokens
     use_draft = draft if block_size > 1 else None
     total_max = prompt_len + max_new_tokens
     sess = SpecSession(target, use_draft, 1, total_max, block_size, stop_token_ids, use_graph=use_graph,
-                       temperature=temperature, seed=seed, profile=profile)
+                       temperature=temperature, seed=seed, profile=profile, kv_dtype=kv_dtype)
 
     torch.cuda.synchronize(target.device)
     t0 = time.perf_counter()
@@ -538,7 +559,7 @@ class BatchStreamEvent:
 def dflash_generate_batch_stream(target: TargetModel, draft: DraftModel | None, prompts: list[list[int]],
                                  max_new_tokens: list[int], temperature: float, stop_token_ids: set[int],
                                  speculative_tokens: int | None = None, use_graph: bool = True,
-                                 seed: int = 0) -> Iterator[list[BatchStreamEvent]]:
+                                 seed: int = 0, kv_dtype: str = "bf16") -> Iterator[list[BatchStreamEvent]]:
     """Decodes several prompts together in one batched session (per-sequence acceptance,
     stop and length rules of runtime.py:405-518 applied to every row) and yields, after
     each step, the events of the sequences that committed tokens or finished in it."""
@@ -553,7 +574,7 @@ def dflash_generate_batch_stream(target: TargetModel, draft: DraftModel | None, 
     use_draft = draft if block_size > 1 else None
     totals = [len(p) + m for p, m in zip(prompts, max_new_tokens)]
     sess = SpecSession(target, use_draft, B, max(totals), block_size, stop_token_ids, use_graph=use_graph,
-                       temperature=temperature, seed=seed)
+                       temperature=temperature, seed=seed, kv_dtype=kv_dtype)
     firsts = sess.prefill(prompts, max_new_tokens)
     streamed = [len(p) for p in prompts]
     done = [False] * B
@@ -600,11 +621,12 @@ def dflash_generate_batch_stream(target: TargetModel, draft: DraftModel | None, 
 def dflash_generate(target: TargetModel, draft: DraftModel, prompt_tokens, max_new_tokens: int, temperature: float,
                     stop_token_ids: set[int], layer_ids: list[int] | None, speculative_tokens: int | None,
                     verify_mode: str = "parallel-replay", verify_chunk_size: int = 4, profile: bool = False,
-                    use_graph: bool = True, seed: int = 0) -> tuple[list[int], dict[str, Any]]:
+                    use_graph: bool = True, seed: int = 0,
+                    kv_dtype: str = "bf16") -> tuple[list[int], dict[str, Any]]:
     final = None
     for event in dflash_generate_stream(target, draft, prompt_tokens, max_new_tokens, temperature, stop_token_ids,
                                         layer_ids, speculative_tokens, verify_mode, verify_chunk_size, profile,
-                                        use_graph, seed):
+                                        use_graph, seed, kv_dtype):
         if event.finished:
             final = event
     if final is None or final.metrics is None:
