@@ -62,9 +62,11 @@ int q8_cache(const dfl_kv_q8* c, const char* who, Q8Cache* out) {
 }
 
 // ---------------------------------------------------------------------------
-// Append. One CTA per (row, group of head slots); hd / 8 lanes per head, eight consecutive
-// values each (one 16-byte load), so a warp holds 256 / hd heads at a time and a head's sums
-// take log2(hd / 8) shuffles. The row's (cos, sin) table is made once per CTA.
+// Append. hd / 8 lanes per head, eight consecutive values each (one 16-byte load), so a warp holds
+// 256 / hd heads (a slot) at a time and a head's sums take log2(hd / 8) shuffles. A CTA takes ROWS
+// rows: its threads make the rows' (cos, sin) tables together, then 8 / ROWS warps walk each row's slots, a
+// slot's load in flight while the one before it is worked on. Few rows: one row a CTA and its
+// slots spread over CTAs (a slot a warp, for latency); many: four rows a CTA.
 // ---------------------------------------------------------------------------
 struct AppendQ8Args {
   const __nv_bfloat16* qkv;
@@ -77,8 +79,9 @@ struct AppendQ8Args {
   const float* inv_freq;
   __nv_bfloat16* q_out;
   Q8Cache c;
-  int M, Hq, rot_dim, do_q;
-  int slots_per_cta;  // head slots (256 / hd heads each) one CTA covers
+  int M, Hq, rot_dim;
+  int first_head;  // 0, or Hq when the q heads are left out
+  int slots_per_cta;
   float eps;
   int* err;
 };
@@ -95,77 +98,107 @@ __device__ __forceinline__ float2 rope_cos_sin(int p, float f) {
   return make_float2(c, s);
 }
 
-template <int HD, bool E4M3>
+// Codes of four values x * up, rounded to nearest even: int8 by an addition of 1.5 * 2^23, whose sum's low
+// byte is the integer (|x * up| <= 127 up to rounding, so none is out of range).
+template <bool E4M3>
+__device__ __forceinline__ uint32_t q8_codes4(const float* x, float up) {
+  if constexpr (E4M3) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * up, x[1] * up), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * up, x[3] * up), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  } else {
+    uint32_t b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[j], up), 12582912.f));
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  }
+}
+
+template <int HD, bool E4M3, int ROWS>
 __global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __grid_constant__ AppendQ8Args a) {
   grid_dependency_launch_dependents();
   grid_dependency_wait();
-  constexpr int LPH = HD / 8;   // lanes per head
-  constexpr int HPW = 32 / LPH;  // heads per warp
-  __shared__ float2 cs[HD / 2];
-  const int m = blockIdx.x;
-  const int p = a.pos[m];
-  if (p < 0) return;
-  const int seq = a.row_seq ? a.row_seq[m] : 0;
-  long long page;
-  int prow;
-  const bool placed = q8_place(a.c, seq, p, threadIdx.x == 0 ? a.err : nullptr, page, prow);
+  constexpr int LPH = HD / 8;               // lanes per head
+  constexpr int HPW = 32 / LPH;             // heads per slot
+  constexpr int WPR = APPEND_WARPS / ROWS;  // warps per row
+  __shared__ float2 cs[ROWS][HD / 2];
+  const int m0 = blockIdx.x * ROWS;
   const int half = a.rot_dim >> 1;
-  for (int i = threadIdx.x; i < half; i += blockDim.x) cs[i] = rope_cos_sin(p, a.inv_freq[i]);
-  __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane / LPH, l = lane % LPH;  // head within the warp, lane within the head
+  const int m = m0 + warp / WPR;
+  const int p = m < a.M ? a.pos[m] : -1;
+  const int sub = lane / LPH, l = lane % LPH;  // head within the slot, lane within the head
   const int Hkv = a.c.Hkv;
   const int n_heads = a.Hq + 2 * Hkv;
+  const __nv_bfloat16* row = a.qkv + (long long)m * a.ldqkv + l * 8;
+  const long long kv0 = (long long)a.Hq * a.q_stride;
+  auto load = [&](int slot) -> uint4 {
+    const int h = slot * HPW + sub;
+    if (p < 0 || h < a.first_head || h >= n_heads) return make_uint4(0, 0, 0, 0);
+    return *reinterpret_cast<const uint4*>(row + (h < a.Hq ? (long long)h * a.q_stride : kv0 + (long long)(h - a.Hq) * HD));
+  };
+  const int slots = (n_heads + HPW - 1) / HPW;
+  const int slot0 = a.first_head / HPW + blockIdx.y * a.slots_per_cta;
+  const int slot_end = min(slots, slot0 + a.slots_per_cta);
+  int slot = slot0 + warp % WPR;
+  uint4 nx = make_uint4(0, 0, 0, 0);
+  if (slot < slot_end) nx = load(slot);
+  // tables: thread t makes entries t, t + 256, ... of the CTA's rows
+  for (int i = threadIdx.x; i < ROWS * half; i += 32 * APPEND_WARPS) {
+    const int r = ROWS == 1 ? 0 : i / half, k = ROWS == 1 ? i : i - r * half;
+    const int pr = m0 + r < a.M ? a.pos[m0 + r] : -1;
+    if (pr >= 0) cs[r][k] = rope_cos_sin(pr, a.inv_freq[k]);
+  }
+  __syncthreads();
+  if (p < 0 || slot >= slot_end) return;
+  const int seq = a.row_seq ? a.row_seq[m] : 0;
+  long long page = 0;
+  int prow = 0;
+  const bool placed = q8_place(a.c, seq, p, lane == 0 ? a.err : nullptr, page, prow);
   // this lane's rotation: its eight values are i .. i + 7 of the first half (partner half / 8
-  // lanes up), of the second (down), or behind the rotated dims
+  // lanes up), of the second (down), or behind the rotated dims (turned by 0)
   const int hl = half / 8;
   const bool first = l < hl, second = l >= hl && l < 2 * hl;
   const int src = sub * LPH + (first ? l + hl : second ? l - hl : l);
   float cr[8], sr[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float2 t = first ? cs[l * 8 + j] : second ? cs[(l - hl) * 8 + j] : make_float2(1.f, 0.f);
+    const float2 t = first || second ? cs[warp / WPR][(first ? l : l - hl) * 8 + j] : make_float2(1.f, 0.f);
     cr[j] = t.x;
     sr[j] = first ? -t.y : t.y;  // x' = x cos -/+ partner sin
   }
-  const __nv_bfloat16* row = a.qkv + (long long)m * a.ldqkv;
-  const int slot0 = blockIdx.y * a.slots_per_cta;
-  for (int slot = slot0 + warp; slot < slot0 + a.slots_per_cta && slot * HPW < n_heads; slot += APPEND_WARPS) {
+  const uint4 qw = *reinterpret_cast<const uint4*>(a.q_norm + l * 8);
+  const uint4 kw = *reinterpret_cast<const uint4*>(a.k_norm + l * 8);
+  const long long code0 = page * a.c.seq_stride + (long long)prow * HD + l * 8;
+  const long long scale0 = page * a.c.s_seq_stride + prow;
+#pragma unroll 1
+  for (; slot < slot_end; slot += WPR) {
+    const uint32_t u[4] = {nx.x, nx.y, nx.z, nx.w};
+    if (slot + WPR < slot_end) nx = load(slot + WPR);
     const int h = slot * HPW + sub;
     const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + Hkv;
-    const bool live = h < n_heads && (is_q ? a.do_q : placed);
+    const bool live = h >= a.first_head && h < n_heads && (is_q || placed);
     float x[8];
-    if (live) {
-      const __nv_bfloat16* s = is_q ? row + (long long)h * a.q_stride
-                                    : row + (long long)a.Hq * a.q_stride + (long long)(h - a.Hq) * HD;
-      const uint4 w = *reinterpret_cast<const uint4*>(s + l * 8);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = __uint_as_float(u[j] << 16);
-        x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(u[j] << 16);
+      x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
     }
-    if (slot * HPW < a.Hq + Hkv) {  // some head of the warp is a q or k head: norm and rotation
+    if (slot * HPW < a.Hq + Hkv) {  // some head of the slot is a q or k head: norm and rotation
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = sq_acc(ss, x[j]);
 #pragma unroll
       for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss / (float)HD + a.eps);
-      const __nv_bfloat16* nw = is_q ? a.q_norm : a.k_norm;
-      const uint4 wv = *reinterpret_cast<const uint4*>(nw + l * 8);
-      const uint32_t wu[4] = {wv.x, wv.y, wv.z, wv.w};
+      const float inv = rsqrtf(ss * (1.f / (float)HD) + a.eps);
+      const uint32_t wu[4] = {is_q ? qw.x : kw.x, is_q ? qw.y : kw.y, is_q ? qw.z : kw.z, is_q ? qw.w : kw.w};
       const bool turn = is_q || is_k;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float wj = __uint_as_float(j & 1 ? wu[j >> 1] & 0xffff0000u : wu[j >> 1] << 16);
         const float y = wj * (x[j] * inv);
         const float z = __shfl_sync(0xffffffffu, y, src);
-        const float r = first || second ? __fmaf_rn(y, cr[j], z * sr[j]) : y;
+        const float r = __fmaf_rn(y, cr[j], z * sr[j]);
         x[j] = turn ? r : x[j];
       }
     }
@@ -177,7 +210,7 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __gr
       o.w = pack_bf16x2(x[6], x[7]);
       *reinterpret_cast<uint4*>(a.q_out + ((long long)m * a.Hq + h) * HD + l * 8) = o;
     }
-    if (slot * HPW + HPW > a.Hq) {  // some head of the warp is a k or v head: quantise
+    if (slot * HPW + HPW > a.Hq) {  // some head of the slot is a k or v head: quantise
       // the maximum magnitude as an unsigned comparison of the bits, in which a NaN or an
       // infinity is larger than every finite value
       unsigned am = 0;
@@ -193,25 +226,10 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __gr
         const bool some = finite && amax >= 1.5046328e-36f;
         const float up = some ? __fdiv_rn(TOP, amax) : 0.f;
         const float scale = finite ? (some ? __fdiv_rn(amax, TOP) : 0.f) : __uint_as_float(0x7fc00000u);
-        uint32_t code[2];
-#pragma unroll
-        for (int q4 = 0; q4 < 2; ++q4) {
-          uint32_t c = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float y = some ? x[q4 * 4 + j] * up : 0.f;
-            uint32_t b;
-            if (E4M3) b = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-            else b = (uint32_t)max(-127, min(127, __float2int_rn(y))) & 0xffu;
-            c |= b << (8 * j);
-          }
-          code[q4] = c;
-        }
+        const uint32_t c0 = some ? q8_codes4<E4M3>(x, up) : 0u, c1 = some ? q8_codes4<E4M3>(x + 4, up) : 0u;
         const int kh = h - a.Hq - (is_k ? 0 : Hkv);
-        unsigned char* dst = (is_k ? a.c.k : a.c.v) + page * a.c.seq_stride + kh * a.c.head_stride +
-                             (long long)prow * HD + l * 8;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
-        if (l == 0) (is_k ? a.c.ks : a.c.vs)[page * a.c.s_seq_stride + kh * a.c.s_head_stride + prow] = scale;
+        *reinterpret_cast<uint2*>((is_k ? a.c.k : a.c.v) + code0 + kh * a.c.head_stride) = make_uint2(c0, c1);
+        if (l == 0) (is_k ? a.c.ks : a.c.vs)[scale0 + kh * a.c.s_head_stride] = scale;
       }
     }
   }
@@ -347,25 +365,29 @@ extern "C" int dfl_qkv_rope_append_q8(const void* qkv, int64_t ldqkv, int q_stri
   a.M = M;
   a.Hq = Hq;
   a.rot_dim = rot_dim;
-  a.do_q = do_q;
+  a.first_head = do_q ? 0 : Hq;
   a.eps = eps;
   a.err = device_error_word();
-  const int per_warp = 256 / hd;
-  const int slots = (Hq + 2 * cache->n_kv_heads + per_warp - 1) / per_warp;
-  // few rows: one head slot per warp, the most CTAs; many: a CTA takes the whole row, so that
-  // its rotary table and lane constants serve every head
-  const int groups = (slots + APPEND_WARPS - 1) / APPEND_WARPS;
-  const bool few = (long long)M * groups <= 148 * 8;
+  const int per_slot = 256 / hd;
+  const int slots = (Hq + 2 * cache->n_kv_heads + per_slot - 1) / per_slot;
+  // Up to about four CTAs an SM: one row each, its slots over CTAs of eight. Beyond: four rows a CTA
+  // (16384 rows of 48 heads of 128: APPEND_TIMES).
+  const int groups = (slots - a.first_head / per_slot + APPEND_WARPS - 1) / APPEND_WARPS;
+  const bool few = (long long)M * groups <= 148 * 4;
   a.slots_per_cta = few ? APPEND_WARPS : slots;
-  const dim3 grid(M, few ? groups : 1);
+  const dim3 grid(few ? M : (M + 3) / 4, few ? groups : 1);
   cudaStream_t st = as_stream(stream);
-  const bool e4 = cache->type == DFL_KV_E4M3;
   const int thr = 32 * APPEND_WARPS;
+  const bool e4 = cache->type == DFL_KV_E4M3;
+#define APPEND_Q8(HD)                                                                                              \
+  return few ? launch_q8(e4 ? append_q8_kernel<HD, true, 1> : append_q8_kernel<HD, false, 1>, a, grid, thr, who, st) \
+             : launch_q8(e4 ? append_q8_kernel<HD, true, 4> : append_q8_kernel<HD, false, 4>, a, grid, thr, who, st)
   switch (hd) {
-    case 64: return launch_q8(e4 ? append_q8_kernel<64, true> : append_q8_kernel<64, false>, a, grid, thr, who, st);
-    case 128: return launch_q8(e4 ? append_q8_kernel<128, true> : append_q8_kernel<128, false>, a, grid, thr, who, st);
-    default: return launch_q8(e4 ? append_q8_kernel<256, true> : append_q8_kernel<256, false>, a, grid, thr, who, st);
+    case 64: APPEND_Q8(64);
+    case 128: APPEND_Q8(128);
+    default: APPEND_Q8(256);
   }
+#undef APPEND_Q8
 }
 
 extern "C" int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq, int M, void* k_out,

@@ -494,7 +494,7 @@ class QuantKV:
         elif page_size:
             raise ValueError("page_size given without a page_table")
         self.tensors = (k, v, k_scale, v_scale, page_table)  # keeps the memory alive
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.index, self.dtype = k.device, k.get_device(), k.dtype
         self.n_kv_heads, self.head_dim = k.shape[1], hd
         self.n_seqs = page_table.shape[0] if page_table is not None else k.shape[0]
         self.cap = page_table.shape[1] * page_size if page_table is not None else k.shape[2]
@@ -505,21 +505,25 @@ class QuantKV:
                          k.shape[0] if page_table is not None else 0, self.cap, self.n_kv_heads, hd,
                          KV_Q8_TYPES[k.dtype])
         self._ref = ctypes.byref(self.desc)
+        self._scratch: dict[tuple, int] = {}  # attention scratch bytes by a call's sizes
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """An entry point on ``device``'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+def _call_on(index: int, name: str, *args) -> None:
+    """An entry point on device ``index``'s current stream, whichever device is current (the raw
+    stream: a torch.cuda.Stream object costs 2 us, as much as the launch)."""
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _index_rows(what: str, t: torch.Tensor | None, n: int, device: torch.device) -> None:
-    if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or t.device != device
-                          or (n > 1 and t.stride(0) != 1)):
-        raise ValueError(f"{what} must be contiguous int32 with at least {n} entries on {device}")
+def _index_rows(what: str, t: torch.Tensor, n: int, index: int) -> int:
+    """Address of int32 row data with at least n entries on device ``index``."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] < n or t.get_device() != index \
+            or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what} must be contiguous int32 with at least {n} entries on cuda:{index}")
+    return t.data_ptr()
 
 
 def qkv_rope_append_q8(qkv: torch.Tensor, pos: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor,
@@ -530,29 +534,30 @@ def qkv_rope_append_q8(qkv: torch.Tensor, pos: torch.Tensor, q_norm: torch.Tenso
     keys and values quantised into the 8-bit cache as they are written (dfl_qkv_rope_append_q8);
     returns the rotated queries [M, Hq, hd] bf16. Rows with pos < 0 are skipped. The rows of one
     call must name distinct (sequence, position) pairs."""
-    dev, hd, M = kv.device, kv.head_dim, qkv.shape[0]
+    idx, hd, M, Hkv = kv.index, kv.head_dim, qkv.shape[0], kv.n_kv_heads
     qs = hd if q_stride is None else q_stride
-    if qkv.dtype != torch.bfloat16 or qkv.device != dev or qkv.dim() != 2 \
-            or qkv.shape[1] < Hq * qs + 2 * kv.n_kv_heads * hd:
-        raise ValueError(f"qkv must be bf16 rows of at least {Hq * qs + 2 * kv.n_kv_heads * hd} columns on {dev}")
-    _index_rows("pos", pos, M, dev)
-    _index_rows("row_seq", row_seq, M, dev)
+    if qkv.dtype is not torch.bfloat16 or qkv.dim() != 2 or qkv.get_device() != idx \
+            or qkv.shape[1] < Hq * qs + 2 * Hkv * hd:
+        raise ValueError(f"qkv must be bf16 rows of at least {Hq * qs + 2 * Hkv * hd} columns on cuda:{idx}")
+    p_pos = _index_rows("pos", pos, M, idx)
+    p_seq = None if row_seq is None else _index_rows("row_seq", row_seq, M, idx)
     for w in (q_norm, k_norm) if do_q else (k_norm,):
-        if w.dtype != torch.bfloat16 or w.shape != (hd,) or not w.is_contiguous() or w.device != dev:
-            raise ValueError(f"norm weights must be contiguous bf16 [{hd}] on {dev}")
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous() \
-            or inv_freq.device != dev:
-        raise ValueError(f"inv_freq must be contiguous fp32 with rot_dim / 2 entries on {dev}")
+        if w.dtype is not torch.bfloat16 or w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous() \
+                or w.get_device() != idx:
+            raise ValueError(f"norm weights must be contiguous bf16 [{hd}] on cuda:{idx}")
+    if inv_freq.dtype is not torch.float32 or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous() \
+            or inv_freq.get_device() != idx:
+        raise ValueError(f"inv_freq must be contiguous fp32 with rot_dim / 2 entries on cuda:{idx}")
     if not do_q:
         q_out = None
     elif q_out is None:
-        q_out = torch.empty((M, Hq, hd), dtype=torch.bfloat16, device=dev)
-    elif q_out.dtype != torch.bfloat16 or q_out.shape != (M, Hq, hd) or not q_out.is_contiguous() \
-            or q_out.device != dev:
-        raise ValueError(f"q_out must be contiguous bf16 [{M}, {Hq}, {hd}] on {dev}")
-    _call_on(dev, "dfl_qkv_rope_append_q8", qkv.data_ptr(), _row_stride(qkv), qs, pos.data_ptr(), _ptr(row_seq),
-             _ptr(q_norm), k_norm.data_ptr(), inv_freq.data_ptr(), _ptr(q_out), kv._ref, M, Hq, rot_dim, float(eps),
-             int(do_q))
+        q_out = qkv.new_empty((M, Hq, hd))
+    elif q_out.dtype is not torch.bfloat16 or q_out.shape != (M, Hq, hd) or not q_out.is_contiguous() \
+            or q_out.get_device() != idx:
+        raise ValueError(f"q_out must be contiguous bf16 [{M}, {Hq}, {hd}] on cuda:{idx}")
+    _call_on(idx, "dfl_qkv_rope_append_q8", qkv.data_ptr(), _row_stride(qkv), qs, p_pos, p_seq,
+             q_norm.data_ptr() if do_q else None, k_norm.data_ptr(), inv_freq.data_ptr(), _ptr(q_out), kv._ref, M, Hq,
+             rot_dim, eps, int(do_q))
     return q_out
 
 
@@ -561,19 +566,18 @@ def kv_read_q8(kv: QuantKV, pos: torch.Tensor, row_seq: torch.Tensor | None = No
                ) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of position pos[r] of sequence row_seq[r] (None: sequence 0) of an 8-bit
     cache as bf16 [M, Hkv, hd] (dfl_kv_read_q8). Rows with pos < 0 are left as they are."""
-    dev, M = kv.device, pos.shape[0]
-    _index_rows("pos", pos, M, dev)
-    _index_rows("row_seq", row_seq, M, dev)
+    idx, M = kv.index, pos.shape[0]
+    p_pos = _index_rows("pos", pos, M, idx)
+    p_seq = None if row_seq is None else _index_rows("row_seq", row_seq, M, idx)
     shape = (M, kv.n_kv_heads, kv.head_dim)
-    outs = []
     for t in (k_out, v_out):
-        if t is None:
-            t = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-        elif t.dtype != torch.bfloat16 or t.shape != shape or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"outputs must be contiguous bf16 {list(shape)} on {dev}")
-        outs.append(t)
-    _call_on(dev, "dfl_kv_read_q8", kv._ref, pos.data_ptr(), _ptr(row_seq), M, outs[0].data_ptr(), outs[1].data_ptr())
-    return outs[0], outs[1]
+        if t is not None and (t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous()
+                              or t.get_device() != idx):
+            raise ValueError(f"outputs must be contiguous bf16 {list(shape)} on cuda:{idx}")
+    k_out = pos.new_empty(shape, dtype=torch.bfloat16) if k_out is None else k_out
+    v_out = pos.new_empty(shape, dtype=torch.bfloat16) if v_out is None else v_out
+    _call_on(idx, "dfl_kv_read_q8", kv._ref, p_pos, p_seq, M, k_out.data_ptr(), v_out.data_ptr())
+    return k_out, v_out
 
 
 def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, max_kv: int,
@@ -588,38 +592,41 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
     result depends on these two and its own query and keys only. Rows with pos < 0 are left as they are; rows that see no key are zero.
     ``ws``: partial results live in its attention scratch (one workspace per stream and captured
     graph, as for attention()); without it each call allocates its own."""
-    dev, hd = kv.device, kv.head_dim
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != hd or not q.is_contiguous() or q.device != dev:
-        raise ValueError(f"q must be contiguous bf16 [M, Hq, {hd}] on {dev}")
+    idx, hd = kv.index, kv.head_dim
+    if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.shape[2] != hd or not q.is_contiguous() \
+            or q.get_device() != idx:
+        raise ValueError(f"q must be contiguous bf16 [M, Hq, {hd}] on cuda:{idx}")
     M, Hq = q.shape[0], q.shape[1]
-    _index_rows("pos", pos, M, dev)
-    _index_rows("row_seq", row_seq, M, dev)
-    _index_rows("kv_len", kv_len, kv.n_seqs, dev)
+    p_pos = _index_rows("pos", pos, M, idx)
+    p_seq = None if row_seq is None else _index_rows("row_seq", row_seq, M, idx)
+    p_len = None if kv_len is None else _index_rows("kv_len", kv_len, kv.n_seqs, idx)
     fcode = Q8_FORMS.get(form)
     if fcode is None:
         raise ValueError(f"form must be one of {tuple(Q8_FORMS)}, not {form!r}")
-    if scale is None:
-        scale = 1.0 / math.sqrt(hd)
     if out is None:
-        out = torch.empty((M, Hq * hd), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or out.shape != (M, Hq * hd) or out.device != dev:
-        raise ValueError(f"out must be bf16 [{M}, {Hq * hd}] on {dev}")
+        out = q.new_empty((M, Hq * hd))
+    elif out.dtype is not torch.bfloat16 or out.shape != (M, Hq * hd) or out.get_device() != idx:
+        raise ValueError(f"out must be bf16 [{M}, {Hq * hd}] on cuda:{idx}")
     if gate is not None:
         ghs = gate_head_stride if gate_head_stride > 0 else hd
-        if gate.dtype != torch.bfloat16 or gate.device != dev or gate.dim() != 2 or gate.shape[0] < M \
+        if gate.dtype is not torch.bfloat16 or gate.get_device() != idx or gate.dim() != 2 or gate.shape[0] < M \
                 or gate.shape[1] < (Hq - 1) * ghs + hd:
-            raise ValueError(f"gate must be bf16 rows covering {Hq} heads on {dev}")
-    need = int(_lib.query("dfl_attention_q8_workspace_bytes", kv._ref, M, Hq, int(seq_rows), int(row_seq is None),
-                          int(max_kv), fcode, int(key_chunk)))
+            raise ValueError(f"gate must be bf16 rows covering {Hq} heads on cuda:{idx}")
+    sizes = (M, Hq, seq_rows, row_seq is None, max_kv, fcode, key_chunk)
+    need = kv._scratch.get(sizes)
+    if need is None:
+        need = int(_lib.query("dfl_attention_q8_workspace_bytes", kv._ref, *sizes))
+        if len(kv._scratch) < 256:
+            kv._scratch[sizes] = need
     if ws is not None:
         ws.ensure_attn(need)
-        scratch = ws.attn
+        scratch, size = ws.attn.data_ptr(), ws.attn.numel()
     else:
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call_on(dev, "dfl_attention_q8", q.data_ptr(), kv._ref, pos.data_ptr(), _ptr(row_seq), _ptr(kv_len),
-             int(seq_rows), M, Hq, int(causal), float(scale), int(max_kv), fcode, int(key_chunk), out.data_ptr(),
-             _row_stride(out), _ptr(gate), _row_stride(gate) if gate is not None else 0, int(gate_head_stride),
-             _ptr(scratch), scratch.numel() if scratch is not None else 0)
+        own = q.new_empty((need,), dtype=torch.uint8) if need else None
+        scratch, size = _ptr(own), need
+    _call_on(idx, "dfl_attention_q8", q.data_ptr(), kv._ref, p_pos, p_seq, p_len, seq_rows, M, Hq, int(causal),
+             hd ** -0.5 if scale is None else scale, max_kv, fcode, key_chunk, out.data_ptr(), _row_stride(out),
+             _ptr(gate), _row_stride(gate) if gate is not None else 0, gate_head_stride, scratch, size)
     return out
 
 
