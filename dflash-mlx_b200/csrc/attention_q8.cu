@@ -21,10 +21,12 @@
 // odd dims go to two accumulator tiles.
 //  * q is scaled by a power of two per row to [2^14, 2^15) at its largest element: every bf16 value
 //    down to 2^-29 of it stays exact in fp16.
-//  * The V scale goes into the weight, w_j = e_j vs_j, which is rounded to fp16 (2^-12 relative).
-//    e_j is taken relative to M = max x - 14 + log2 of the largest V scale the row has seen, so
-//    w_j < 2^15 whatever the scales are, and weights down to 2^-29 of the largest keep all their
-//    bits; the sum of e_j uses the same M, which cancels in the quotient.
+//  * The V scale goes into the weight, w_j = e_j vs_j, which is rounded to fp16 (2^-11 relative).
+//    e_j is taken relative to a base M that follows max x - 4 + log2 of the largest V scale the row has
+//    seen; it is raised, and sums and accumulators rescaled, only when it has fallen behind by more than
+//    10. So w_j < 2^15 whatever the scales are, and weights down to 2^-18 of the largest keep all their
+//    bits (those below are rounded to multiples of 2^-28 of it); the sum of e_j uses the same M, which
+//    cancels in the quotient.
 // Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales,
 // codes or query products may be anything), so infinities and NaN there do not reach the row.
 #include "attention_q8.cuh"
@@ -66,7 +68,8 @@ struct AttnQ8Layout {
 };
 
 template <int HD, int MT, int RG, int ST, bool E4M3>
-__global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __grid_constant__ AttnQ8Args a) {
+// single tokens at head_dim <= 128: three CTAs an SM (12 warps; 10 % faster than two at a 3-stage ring)
+__global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3 : 1) attn_q8_kernel(const __grid_constant__ AttnQ8Args a) {
   using L = AttnQ8Layout<HD, MT, RG, ST>;
   constexpr int NC = HD / 16;
   constexpr int NWARPS = Q8_STRANDS * RG;
@@ -87,32 +90,38 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
   const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
   if (ntok <= 0) return;
 
-  // the run's sequence: that of the tile's first row with a position
-  int seq = -1;
-  for (int i = 0; i < ntok && seq < 0; ++i)
-    if (a.pos[m0 + i] >= 0) seq = a.row_seq ? a.row_seq[m0 + i] : 0;
-  if (seq < 0 || seq >= a.c.n_seqs) {  // nothing to do, or no such sequence
-    if (seq >= 0 && threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
+  // the tile's rows, two a lane, by every warp alike: their positions and sequences, the run's sequence
+  // (that of the first row with a position), limits
+  int pos2[2], sq2[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = lane + 32 * k;
+    pos2[k] = i < ntok ? a.pos[m0 + i] : -1;
+    sq2[k] = i < ntok && a.row_seq ? a.row_seq[m0 + i] : 0;
+  }
+  const unsigned v0 = __ballot_sync(0xffffffffu, pos2[0] >= 0), v1 = __ballot_sync(0xffffffffu, pos2[1] >= 0);
+  if (!(v0 | v1)) return;
+  const int seq = __shfl_sync(0xffffffffu, v0 ? sq2[0] : sq2[1], __ffs(v0 ? v0 : v1) - 1);
+  if (seq < 0 || seq >= a.c.n_seqs) {  // a row that names no sequence of the cache is left as it is
+    if (threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
     return;
   }
-  if (threadIdx.x < ntok) {
-    const int m = m0 + threadIdx.x, p = a.pos[m];
-    int lim = 0, ok = p >= 0;
-    if (ok && a.row_seq && a.row_seq[m] != seq) {
-      q8_error(a.err, Q8_ERR_SEQ);
-      ok = 0;
-    }
-    if (ok) lim = q8_row_limit(a, m, p, seq, chunk == 0 && kvh == 0 ? a.err : nullptr);
-    s_tok_lim[threadIdx.x] = lim;
-    s_tok_ok[threadIdx.x] = ok;
-  }
-  __syncthreads();
   int lim_max = 0, lim_min = 0x7fffffff;
-  for (int i = 0; i < ntok; ++i) {
-    const int lim = s_tok_lim[i];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = lane + 32 * k;
+    const bool ok = pos2[k] >= 0 && sq2[k] == seq;
+    if (warp == 0 && pos2[k] >= 0 && !ok) q8_error(a.err, Q8_ERR_SEQ);
+    const int lim = ok ? q8_row_limit(a, m0 + i, pos2[k], seq, warp == 0 && chunk == 0 && kvh == 0 ? a.err : nullptr) : 0;
+    if (warp == 0 && i < L::ROWS) {
+      s_tok_lim[i] = lim;
+      s_tok_ok[i] = ok;
+    }
     lim_max = max(lim_max, lim);
     if (lim > 0) lim_min = min(lim_min, lim);
   }
+  lim_max = __reduce_max_sync(0xffffffffu, lim_max);
+  lim_min = __reduce_min_sync(0xffffffffu, lim_min);
   const int k_begin = chunk * a.key_chunk;
   if (k_begin >= lim_max && a.n_chunks > 1) return;  // the merge kernel writes rows without keys
   const int k_end = min(k_begin + a.key_chunk, lim_max);
@@ -125,25 +134,43 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
   const float* VSh = a.c.vs + kvh * a.c.s_head_stride;
   const int n_blocks = (max(k_end - k_begin, 0) + Q8_KB - 1) / Q8_KB;
   const int my_n = n_blocks > strand ? (n_blocks - strand + Q8_STRANDS - 1) / Q8_STRANDS : 0;
+  // Thread `first` of the strand copies 16-byte chunks first, first + T, ... of a block, which is contiguous in
+  // the cache: chunk u * T + first lies in row r0 + u * SR, whose swizzle is r0's with SR * u's low bits flipped.
+  constexpr int T = 32 * RG, SR = T / NC;
+  const int first = rg * 32 + lane, r0c = first / NC;
+  const uint32_t dst0 = smem_u32(ring) + q8_swz<HD>(r0c, first % NC);
+  // the page of the next block to load, looked up one block ahead; -1 when it is refused
+  auto page_of = [&](int i) -> int {
+    long long page = -1;
+    int row;
+    if (i < my_n && !q8_place(a.c, seq, k_begin + (strand + i * Q8_STRANDS) * Q8_KB, lane == 0 ? a.err : nullptr, page, row))
+      page = -1;
+    return (int)page;
+  };
+  int next_page = page_of(0);
   auto load = [&](int i) {  // block i of the strand
     const int kb = k_begin + (strand + i * Q8_STRANDS) * Q8_KB;
     unsigned char* st = ring + (i % ST) * L::STAGE;
-    long long page;
-    int row;
-    const bool ok = q8_place(a.c, seq, kb, lane == 0 ? a.err : nullptr, page, row);
-    if (!ok) page = row = 0;
-    const long long off = page * a.c.seq_stride + (long long)row * HD;
+    const bool ok = next_page >= 0;
+    const long long page = max(next_page, 0);
+    const int row = !ok ? 0 : a.c.page_table ? kb & ((1 << a.c.page_shift) - 1) : kb;
+    next_page = page_of(i + 1);
+    const unsigned char* kp = Kh + (page * a.c.seq_stride + (long long)row * HD) + first * 16;
+    const unsigned char* vp = Vh + (page * a.c.seq_stride + (long long)row * HD) + first * 16;
     const long long soff = page * a.c.s_seq_stride + row;
     const int n = ok ? min(Q8_KB, k_end - kb) : 0;  // rows of the block that hold keys
-    const int first = rg * 32 + lane;
+    const uint32_t d = dst0 + (i % ST) * L::STAGE;
 #pragma unroll
-    for (int u = 0; u < Q8_KB * NC / (32 * RG); ++u) {
-      const int idx = first + u * 32 * RG;
-      const int r = idx / NC, c = idx % NC;
-      const int bytes = r < n ? 16 : 0;
-      const long long o = off + (r < n ? idx * 16 : 0);
-      cp_async16(smem_u32(st + q8_swz<HD>(r, c)), Kh + o, bytes);
-      cp_async16(smem_u32(st + Q8_KB * HD + q8_swz<HD>(r, c)), Vh + o, bytes);
+    for (int u = 0; u < Q8_KB * NC / T; ++u) {
+      const uint32_t du = (HD == 64 ? d : d ^ ((u * SR & 7) << 4)) + u * SR * HD;
+      if (n == Q8_KB) {
+        cp_async16(du, kp + u * T * 16, 16);
+        cp_async16(du + Q8_KB * HD, vp + u * T * 16, 16);
+      } else {  // rows behind the last key read as zeros
+        const bool in = r0c + u * SR < n;
+        cp_async16(du, in ? kp + u * T * 16 : Kh, in ? 16 : 0);
+        cp_async16(du + Q8_KB * HD, in ? vp + u * T * 16 : Vh, in ? 16 : 0);
+      }
     }
     if (rg == 0) {
       float* sc = reinterpret_cast<float*>(st + 2 * Q8_KB * HD);
@@ -162,6 +189,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
     cp_async_commit();
   }
 
+  __syncthreads();  // the rows' limits
   // ---- Q rows to scaled fp16, dims permuted within 16 to the order of a K register ----
   for (int r = warp; r < L::ROWS; r += NWARPS) {
     const int tok = r / a.G, hg = r % a.G;
@@ -317,16 +345,17 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG) attn_q8_kernel(const __g
           const int en = max(er[mt][h], (int)(vm >> 23) - 127);
           mrow[mt][h] = mn;
           er[mt][h] = en;
-          const float Mn = mn + (float)(en - 14);  // -inf while the row has seen no key
-          const float mu = Mn == -INFINITY ? 0.f : Mn;
-          fac[h] = exp2f(Mr[mt][h] - mu);
-          Mr[mt][h] = Mn;
+          const float Mn = mn + ((float)en - Q8_BASE);  // -inf while the row has seen no key
+          const bool grow = Mn > Mr[mt][h] + Q8_LAZY || (Mr[mt][h] == -INFINITY && Mn > -INFINITY);
+          fac[h] = grow ? q8_exp2(Mr[mt][h] - Mn) : 1.f;
+          if (grow) Mr[mt][h] = Mn;
+          const float mu = Mr[mt][h] == -INFINITY ? 0.f : Mr[mt][h];
           float ps = 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kb + j * 8 + 2 * t;
-            const float e0 = exp2f(__fmaf_rn(s[mt][j][2 * h], rowf[mt][h], -mu));
-            const float e1 = exp2f(__fmaf_rn(s[mt][j][2 * h + 1], rowf[mt][h], -mu));
+            const float e0 = q8_exp2(__fmaf_rn(s[mt][j][2 * h], rowf[mt][h], -mu));
+            const float e1 = q8_exp2(__fmaf_rn(s[mt][j][2 * h + 1], rowf[mt][h], -mu));
             ps += e0 + e1;
             float w0 = e0 * vs[j].x, w1 = e1 * vs[j].y;
             if (!FULL) {
@@ -574,7 +603,7 @@ static int launch_attn_q8(const AttnQ8Args& a, int tiles, cudaStream_t st) {
 
 template <int HD, bool E4M3>
 static int launch_attn_q8_rows(const AttnQ8Args& a, int rows, int tiles, cudaStream_t st) {
-  if (rows <= 16) return launch_attn_q8<HD, 1, 1, 3, E4M3>(a, tiles, st);
+  if (rows <= 16) return launch_attn_q8<HD, 1, 1, HD == 256 ? 3 : 2, E4M3>(a, tiles, st);
   if constexpr (HD == 256) {
     return launch_attn_q8<HD, 1, 2, 2, E4M3>(a, tiles, st);
   } else {

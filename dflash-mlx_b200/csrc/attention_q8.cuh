@@ -11,6 +11,15 @@ namespace dfl {
 // nor the weights leave fp32's normal range, over 2^20 keys and more.
 constexpr int Q8_ER_MIN = -104;
 constexpr float Q8_SUM_UNIT = 1.f / 65536.f;
+// The exponent base starts Q8_BASE above the row's maximum and is raised when it lags by Q8_LAZY (log2).
+constexpr float Q8_BASE = 4.f, Q8_LAZY = 10.f;
+
+// 2^x, results below the normal range flushed to zero (fp16 weights and their sum lose nothing)
+__device__ __forceinline__ float q8_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
 
 struct AttnQ8Args {
   const __nv_bfloat16* q;  // [M][Hq][hd]

@@ -28,7 +28,6 @@ constexpr int QT_KB = 64;       // keys per block
 constexpr int QT_ROWS = 64;     // (token, head) rows per tile
 constexpr int QT_THREADS = 288;
 constexpr int QT_SCALES = 4;    // scale ring: block i's are read until its weights are written
-constexpr float QT_BASE = 4.f, QT_LAZY = 10.f;
 
 template <int HD>
 struct QtLayout {
@@ -38,8 +37,8 @@ struct QtLayout {
   static constexpr int OFF_V = 2 * TILE;        // 2 stages; the epilogue reuses K and V for O
   static constexpr int OFF_Q = 4 * TILE;        // [units][128 rows][128 B]
   static constexpr int OFF_S = OFF_Q + 128 * HD * 2;  // scales [4][2][64], largest V scales [4][2]
-  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of both copies
-  static constexpr int OFF_BAR = OFF_R + QT_ROWS * 8 + 128 * 8;
+  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of both copies, output weights
+  static constexpr int OFF_BAR = OFF_R + QT_ROWS * 8 + 128 * 8 + QT_ROWS * 16;
   static constexpr int N_BAR = 2 * 4 + 2 * 3 + QT_SCALES;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
   static constexpr uint32_t COLS = HD == 256 ? 512 : 256;  // S / weights 2 x 64, O hd
@@ -94,13 +93,6 @@ __device__ __forceinline__ bool qt_wait(uint64_t* bar, uint32_t parity, int site
   return false;
 }
 
-// 2^x, results below the normal range flushed to zero (fp16 weights and their sum lose nothing)
-__device__ __forceinline__ float qt_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // two fp32 operations an instruction
 __device__ __forceinline__ uint64_t qt_pack(float a, float b) {
   uint64_t r;
@@ -142,6 +134,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_R);
   int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + QT_ROWS;
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + QT_ROWS * 8);  // [128]
+  float4* s_w = reinterpret_cast<float4*>(s_ml + 128);  // [64]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* k_full = bars;        // [2] 64 converter arrivals
   uint64_t* k_empty = bars + 2;   // [2] MMA commit
@@ -373,27 +366,31 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     if (ok && n_blocks > 0) pv(n_blocks - 1);
   } else if (warp < 4) {
     // ---------------- softmax: thread = (row, copy) ----------------
-    // Q rows to scaled fp16, twice; a row's factor undoes its power of two. hd / 16 lanes a row, 16
-    // dims each; a rolled loop, since code that runs once a CTA comes from a cold instruction cache.
+    // Q rows to scaled fp16, twice; a row's factor undoes its power of two. The raw rows all come at once
+    // into the second copy's place, where each thread then converts what it copied: hd / 16 lanes a row,
+    // 32 bytes each, in rolled loops (code that runs once a CTA comes from a cold instruction cache).
     {
       constexpr int LPR = HD / 16, RPW = 32 / LPR;
-      const int ql = lane % LPR;
-      uint4 nx[2];
-      auto qload = [&](int r) {
-        const int th = r < QT_ROWS ? s_row[r] : -1;
-        nx[0] = nx[1] = make_uint4(0, 0, 0, 0);
-        if (th >= 0 && s_tok_lim[th >> 4] > 0) {
-          const uint4* q = reinterpret_cast<const uint4*>(
-              a.q + ((long long)(m0 + (th >> 4)) * a.Hq + kvh * a.G + (th & 15)) * HD + ql * 16);
-          nx[0] = q[0];
-          nx[1] = q[1];
-        }
-      };
-      qload(warp * RPW + lane / LPR);
+      const int ql = lane % LPR, qr = warp * RPW + lane / LPR;
+      unsigned char* q1 = smem + L::OFF_Q + (ql >> 2) * 16384 + QT_ROWS * 128;
 #pragma unroll 1
-      for (int r = warp * RPW + lane / LPR; r < QT_ROWS; r += 4 * RPW) {
-        const uint32_t u[8] = {nx[0].x, nx[0].y, nx[0].z, nx[0].w, nx[1].x, nx[1].y, nx[1].z, nx[1].w};
-        qload(r + 4 * RPW);
+      for (int r = qr; r < QT_ROWS; r += 4 * RPW) {
+        const int th = s_row[r];
+        const bool ok = th >= 0 && s_tok_lim[th >> 4] > 0;
+        const __nv_bfloat16* q =
+            ok ? a.q + ((long long)(m0 + (th >> 4)) * a.Hq + kvh * a.G + (th & 15)) * HD + ql * 16 : a.q;
+        const uint32_t d = smem_u32(q1) + qt_sw(r, (ql & 3) * 2);
+        cp_async16(d, q, ok ? 16 : 0);
+        cp_async16(d ^ 16, q + (ok ? 8 : 0), ok ? 16 : 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+#pragma unroll 1
+      for (int r = qr; r < QT_ROWS; r += 4 * RPW) {
+        uint4* d0 = reinterpret_cast<uint4*>(q1 + qt_sw(r, (ql & 3) * 2));
+        uint4* d1 = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d0) ^ 16);
+        const uint4 n0 = *d0, n1 = *d1;
+        const uint32_t u[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
         // magnitudes compare as integers; one that is not finite leaves the row unscaled
         uint32_t mx2 = 0;
 #pragma unroll
@@ -409,12 +406,11 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
           const __half2 y = __floats2half2_rn(__uint_as_float(u[j] << 16) * f, __uint_as_float(u[j] & 0xffff0000u) * f);
           h[j] = *reinterpret_cast<const uint32_t*>(&y);
         }
-        unsigned char* d = smem + L::OFF_Q + (ql >> 2) * 16384 + qt_sw(r, (ql & 3) * 2);
-#pragma unroll
-        for (int copy = 0; copy < 2; ++copy, d += QT_ROWS * 128) {
-          *reinterpret_cast<uint4*>(d) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d) ^ 16) = make_uint4(h[4], h[5], h[6], h[7]);
-        }
+        const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+        *d0 = h0;
+        *d1 = h1;
+        *(d0 - QT_ROWS * 8) = h0;  // the first copy, 64 rows of 128 bytes before
+        *(d1 - QT_ROWS * 8) = h1;
         if (ql == 0) {
           s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
           s_lim[r] = s_row[r] < 0 ? 0 : s_tok_lim[s_row[r] >> 4];
@@ -480,10 +476,10 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       }
       m = fmaxf(m, fmaxf(mx0, mx1) * rowf);
       er = max(er, (int)(vm >> 23) - 127);
-      const float M = m + ((float)er - QT_BASE);
-      const bool grow = M > mu_used + QT_LAZY || (mu_used == -INFINITY && M > -INFINITY);
+      const float M = m + ((float)er - Q8_BASE);
+      const bool grow = M > mu_used + Q8_LAZY || (mu_used == -INFINITY && M > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
-        const float fac = grow ? qt_exp2(mu_used - M) : 1.f;
+        const float fac = grow ? q8_exp2(mu_used - M) : 1.f;
         if (grow) mu_used = M;
         l = qt_mul2(l, qt_pack(fac, fac));
         if (i > 0) {
@@ -512,7 +508,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           const float2 y = qt_unpack(qt_fma2(x[c + d], rf2, mu2));
-          const uint64_t e = qt_pack(qt_exp2(y.x), qt_exp2(y.y));
+          const uint64_t e = qt_pack(q8_exp2(y.x), q8_exp2(y.y));
           l = qt_fma2(e, unit2, l);
           const float2 ww = qt_unpack(qt_mul2(e, d ? vs.y : vs.x));
           const __half2 h = __floats2half2_rn(ww.x, ww.y);
@@ -554,31 +550,48 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     }
     s_ml[threadIdx.x] = make_float2(mu_used, qt_unpack(l).x + qt_unpack(l).y);
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
-    constexpr int RPW = CH >= 32 ? 1 : 32 / CH;  // rows a warp writes at a time
-#pragma unroll 2
-    for (int r0 = warp * RPW; r0 < ntok * a.G; r0 += 4 * RPW) {
-      const int r = r0 + lane / (32 / RPW), c0 = lane % (32 / RPW);
-      const int th = s_row[r], tok = th >> 4, head = kvh * a.G + (th & 15);
-      const int lm = s_lim[r];
+    // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and the row
+    // of the output (or of the partials) it goes to, -1 for none
+    if (threadIdx.x < QT_ROWS) {
+      const int r = threadIdx.x, th = s_row[r], tok = th >> 4;
       const float2 x0 = s_ml[r], x1 = s_ml[r + QT_ROWS];
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
-      const float w0 = qt_exp2(x0.x - mu), w1 = qt_exp2(x1.x - mu);
+      float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
       const float den = w0 * x0.y + w1 * x1.y;
-      if (!ok || th < 0 || !s_tok_ok[tok] || (a.n_chunks > 1 && lm <= k_begin)) continue;
-      const int mrow = m0 + tok;
-      const long long base = ((long long)chunk * a.M + mrow) * a.Hq + head;
+      int to = -1;
+      if (ok && th >= 0 && s_tok_ok[tok] && (a.n_chunks == 1 || lim > k_begin)) {
+        to = (m0 + tok) * a.Hq + kvh * a.G + (th & 15);
+        if (a.n_chunks > 1) {
+          a.part_ml[(long long)chunk * a.M * a.Hq + to] = make_float2(mm, den);
+        } else {
+          const float inv = lim > 0 ? Q8_SUM_UNIT / den : 0.f;
+          w0 *= inv;
+          w1 *= inv;
+        }
+      }
+      s_w[r] = make_float4(w0, w1, __int_as_float(to), lim > 0 ? 1.f : 0.f);
+    }
+    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    constexpr int RPW = CH >= 32 ? 1 : 32 / CH;  // rows a warp writes at a time
+#pragma unroll 4
+    for (int r0 = warp * RPW; r0 < ntok * a.G; r0 += 4 * RPW) {
+      const int r = r0 + lane / (32 / RPW);
+      const float4 w = s_w[r];
+      const int to = __float_as_int(w.z);
+      if (to < 0) continue;
 #pragma unroll
-      for (int c = c0; c < CH; c += 32) {
+      for (int c = lane % (32 / RPW); c < CH; c += 32) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (n_blocks > 0) {
+        if (w.w != 0.f) {
           const float4 o0 = s_o[r * CH + (c ^ (r & 7))], o1 = s_o[(r + QT_ROWS) * CH + (c ^ (r & 7))];
-          y = make_float4(w0 * o0.x + w1 * o1.x, w0 * o0.y + w1 * o1.y, w0 * o0.z + w1 * o1.z, w0 * o0.w + w1 * o1.w);
+          y = make_float4(w.x * o0.x + w.y * o1.x, w.x * o0.y + w.y * o1.y, w.x * o0.z + w.y * o1.z,
+                          w.x * o0.w + w.y * o1.w);
         }
         if (a.n_chunks > 1) {
-          *reinterpret_cast<float4*>(a.part_o + base * HD + c * 4) = y;
+          *reinterpret_cast<float4*>(a.part_o + ((long long)chunk * a.M * a.Hq + to) * HD + c * 4) = y;
         } else {
-          const float inv = lm > 0 ? Q8_SUM_UNIT / den : 0.f;
-          float f[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+          const int mrow = to / a.Hq, head = to - mrow * a.Hq;
+          float f[4] = {y.x, y.y, y.z, y.w};
           if (a.gate) {
             const __nv_bfloat16* gr = a.gate + (long long)mrow * a.ldg + (long long)head * a.gate_hs + c * 4;
 #pragma unroll
@@ -588,7 +601,6 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
               make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
         }
       }
-      if (a.n_chunks > 1 && c0 == 0) a.part_ml[base] = make_float2(mm, den);
     }
   }
   tc_fence_before();
