@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
   grid_dependency_launch_dependents();
   grid_dependency_wait();
 
-  const int run = blockIdx.x / a.run_tiles, tile = blockIdx.x % a.run_tiles, kvh = blockIdx.y, chunk = blockIdx.z;
+  const Q8Tile at = q8_tile(a);
+  const int run = at.run, tile = at.tile, kvh = at.kvh, chunk = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int strand = warp % Q8_STRANDS, rg = warp / Q8_STRANDS;
   const int g = lane >> 2, t = lane & 3;
@@ -587,7 +588,7 @@ static int launch_attn_q8(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles, a.c.Hkv, a.n_chunks);
+  cfg.gridDim = dim3(tiles * a.c.Hkv, a.n_chunks);
   cfg.blockDim = dim3(32 * Q8_STRANDS * RG);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = st;
@@ -620,24 +621,27 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
   return one_seq ? M : seq_rows > 0 ? (seq_rows < M ? seq_rows : M) : 1;
 }
 
-// The form and the keys per chunk of a call. Up to 16 (token, head) rows a run take the warp form, more the
-// tcgen05 form, whose tile of 64 rows they fill better (one token of 64 sequences 105 against
-// 123 us, 16 tokens 280 against 168).
+// The form and the keys per chunk of a call. The tcgen05 form for calls of more than 16 (token, head) rows a
+// run, whose tile of 64 rows they fill, and with work for it: 512 keys a CTA on every SM (its CTAs start
+// and end slowly). Measured: 64 sequences of 512 to 4096 keys, one token each 66 (warp) against 107 us, 16
+// tokens 338 against 134; one sequence of 1053 keys, 16 tokens 17 against 21.
+// Chunks: as many as keep every CTA in one wave (three CTAs an SM, two in the tcgen05 form, one at
+// head_dim 256), one more for several runs, whose lengths may differ. One chunk needs no merge.
 struct Q8Plan {
   int form, key_chunk, n_chunks;
 };
 static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int G, int Hkv, int hd, int max_kv) {
   Q8Plan p;
   const long long want = (long long)run_rows * G;
-  p.form = form != DFL_Q8_AUTO ? form : want <= 16 ? DFL_Q8_WARP : DFL_Q8_TC;
+  const long long units = runs * Hkv * ((want + 63) / 64);
+  p.form = form != DFL_Q8_AUTO ? form : want > 16 && units * max_kv >= 148 * 512 ? DFL_Q8_TC : DFL_Q8_WARP;
   if (key_chunk <= 0) {
-    // about as many CTAs as the SMs hold at a time (warp form: eight an SM, its CTAs are short-lived;
-    // tcgen05 form: one wave, since a CTA's start and end cost it some ten blocks)
-    const long long units = runs * Hkv * ((want + 63) / 64);
-    const long long slots = 148 * (p.form == DFL_Q8_TC ? (hd == 256 ? 1 : 2) : 8);
-    const long long lo = p.form == DFL_Q8_TC ? 512 : Q8_CHUNK_UNIT, hi = p.form == DFL_Q8_TC ? 8192 : 4096;
-    const long long r = (max_kv * units / slots + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT;
-    key_chunk = (int)(r < lo ? lo : r > hi ? hi : r);
+    const long long slots = 148 * (p.form == DFL_Q8_TC ? (hd == 256 ? 1 : 2) : 3);
+    const long long n = slots / units + (runs > 1 && slots % units ? 1 : 0);
+    const long long lo = p.form == DFL_Q8_TC ? 512 : Q8_CHUNK_UNIT;
+    long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
+    c = c < lo ? lo : c > 8192 ? 8192 : c;
+    key_chunk = (int)((c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT);
   }
   p.key_chunk = key_chunk;
   p.n_chunks = (int)(((long long)max_kv + key_chunk - 1) / key_chunk);
@@ -720,7 +724,9 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
   a.run_tiles = (run_rows + rows / G - 1) / (rows / G);
   a.tile_toks = (run_rows + a.run_tiles - 1) / a.run_tiles;
   const long long tiles = (long long)runs * a.run_tiles;
-  if (tiles > 0x7fffffffLL) {
+  a.runs = runs;
+  a.ranked = runs > 1 && runs <= Q8_RANK_RUNS && tiles * Hkv * a.n_chunks > 148;
+  if (tiles * Hkv > 0x7fffffffLL) {
     set_error("%s: too many rows (%d)", who, M);
     return DFL_ERR_UNSUPPORTED;
   }

@@ -36,6 +36,8 @@ struct AttnQ8Args {
   int gate_hs;
   int M, Hq, G, causal, max_kv, n_chunks, key_chunk;
   int run_rows;   // rows per run
+  int runs;       // runs of the call
+  int ranked;     // the launch takes the runs with the most keys first
   int tile_toks;  // tokens per tile
   int run_tiles;  // tiles per run
   float scale_log2;  // |softmax scale| * log2(e); 1 when the scale is 0
@@ -71,6 +73,53 @@ __device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, i
   const int most = min(a.max_kv, a.c.cap);
   if (lim > most) q8_error(err, Q8_ERR_POS);
   return lim > most ? most : lim < 0 ? 0 : (int)lim;
+}
+
+// Tile and kv head of a CTA: heads of a run side by side, runs in the launch's order. That order is by keys,
+// most first (ties by index), where a.ranked: a long run started last would leave the other SMs idle
+// (64 runs of 512 to 4096 keys, tcgen05 form: 169 us in index order, RANKED us so). Every CTA
+// ranks the runs alike from their last rows' limits, a permutation whatever those are.
+constexpr int Q8_RANK_RUNS = 256;
+struct Q8Tile {
+  int run, tile, kvh;
+};
+__device__ __forceinline__ Q8Tile q8_tile(const AttnQ8Args& a) {
+  __shared__ int4 s_keys[Q8_RANK_RUNS / 4];
+  __shared__ int s_run;
+  Q8Tile t;
+  const int id = blockIdx.x / a.c.Hkv;
+  t.kvh = blockIdx.x - id * a.c.Hkv;
+  t.run = id / a.run_tiles;
+  t.tile = id - t.run * a.run_tiles;
+  if (!a.ranked) return t;
+  const int n4 = (a.runs + 3) & ~3;
+  for (int r = threadIdx.x; r < n4; r += blockDim.x) {
+    int key = -1;
+    if (r < a.runs) {
+      const int m = min((r + 1) * a.run_rows, a.M) - 1;
+      key = a.pos[m];
+      if (!a.causal && key >= 0) {
+        const int seq = a.row_seq ? a.row_seq[m] : 0;
+        key = seq >= 0 && seq < a.c.n_seqs ? a.kv_len[seq] : 0;
+      }
+      key = max(key, 0);
+    }
+    reinterpret_cast<int*>(s_keys)[r] = key;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < a.runs; r += blockDim.x) {
+    const int key = reinterpret_cast<const int*>(s_keys)[r];
+    int rank = 0;
+    for (int j = 0; j < n4 / 4; ++j) {  // runs before r win ties; the padding (-1) never counts
+      const int4 k = s_keys[j];
+      rank += (k.x > key || (k.x == key && 4 * j < r)) + (k.y > key || (k.y == key && 4 * j + 1 < r)) +
+              (k.z > key || (k.z == key && 4 * j + 2 < r)) + (k.w > key || (k.w == key && 4 * j + 3 < r));
+    }
+    if (rank == t.run) s_run = r;
+  }
+  __syncthreads();
+  t.run = s_run;
+  return t;
 }
 
 // The tcgen05 form (attention_q8_tc.cu): the chunk kernel alone.

@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   __shared__ int s_row[QT_ROWS];  // token * 16 + head in group of each tile row, -1 behind the last
 
   grid_dependency_wait();
-  const int run = blockIdx.x / a.run_tiles, tile = blockIdx.x % a.run_tiles, kvh = blockIdx.y, chunk = blockIdx.z;
+  const Q8Tile at = q8_tile(a);
+  const int run = at.run, tile = at.tile, kvh = at.kvh, chunk = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = run * a.run_rows + tile * a.tile_toks;
   const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
@@ -630,7 +631,7 @@ static int launch_qt(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles, a.c.Hkv, a.n_chunks);
+  cfg.gridDim = dim3(tiles * a.c.Hkv, a.n_chunks);
   cfg.blockDim = dim3(QT_THREADS);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = st;
