@@ -93,28 +93,6 @@ __device__ __forceinline__ bool qt_wait(uint64_t* bar, uint32_t parity, int site
   return false;
 }
 
-// two fp32 operations an instruction
-__device__ __forceinline__ uint64_t qt_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 qt_unpack(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t qt_mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t qt_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // 16-byte chunk c of row r of a [rows][128 B] 128-byte-swizzled unit
 __device__ __forceinline__ uint32_t qt_sw(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -451,17 +429,17 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {
         const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + 2 * c);
-        x[c] = qt_mul2(qt_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
-        x[c + 1] = qt_mul2(qt_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
+        x[c] = q8_mul2(q8_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
+        x[c + 1] = q8_mul2(q8_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
       }
       uint32_t vm = s_vmax[(i & (QT_SCALES - 1)) * 2 + half];
       if (!full) {
         vm = 0;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          const float2 y = qt_unpack(x[c]);
+          const float2 y = q8_unpack(x[c]);
           const bool seen0 = kb + 2 * c < lim, seen1 = kb + 2 * c + 1 < lim;
-          x[c] = qt_pack(seen0 ? y.x : -INFINITY, seen1 ? y.y : -INFINITY);
+          x[c] = q8_pack(seen0 ? y.x : -INFINITY, seen1 ? y.y : -INFINITY);
           const uint2 v = *reinterpret_cast<const uint2*>(sc + QT_KB + 2 * c);
           const uint32_t v0 = v.x & 0x7fffffffu, v1 = v.y & 0x7fffffffu;
           if (seen0 && v0 < 0x7f800000u) vm = max(vm, v0);
@@ -471,7 +449,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {
-        const float2 y = qt_unpack(x[c]), z = qt_unpack(x[c + 1]);
+        const float2 y = q8_unpack(x[c]), z = q8_unpack(x[c + 1]);
         mx0 = fmaxf(fmaxf(mx0, y.x), y.y);
         mx1 = fmaxf(fmaxf(mx1, z.x), z.y);
       }
@@ -482,7 +460,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       if (__any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
         const float fac = grow ? q8_exp2(mu_used - M) : 1.f;
         if (grow) mu_used = M;
-        l = qt_mul2(l, qt_pack(fac, fac));
+        l = q8_mul2(l, q8_pack(fac, fac));
         if (i > 0) {
           ok = qt_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 357, a.err);
           if (!__all_sync(0xffffffffu, ok)) {
@@ -501,17 +479,17 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         }
       }
       const float mu = mu_used == -INFINITY ? 0.f : mu_used;
-      const uint64_t rf2 = qt_pack(rowf, rowf), mu2 = qt_pack(-mu, -mu), unit2 = qt_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
+      const uint64_t rf2 = q8_pack(rowf, rowf), mu2 = q8_pack(-mu, -mu), unit2 = q8_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
       uint32_t w[16];
 #pragma unroll
       for (int c = 0; c < 16; c += 2) {
         const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + QT_KB + 2 * c);
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
-          const float2 y = qt_unpack(qt_fma2(x[c + d], rf2, mu2));
-          const uint64_t e = qt_pack(q8_exp2(y.x), q8_exp2(y.y));
-          l = qt_fma2(e, unit2, l);
-          const float2 ww = qt_unpack(qt_mul2(e, d ? vs.y : vs.x));
+          const float2 y = q8_unpack(q8_fma2(x[c + d], rf2, mu2));
+          const uint64_t e = q8_pack(q8_exp2(y.x), q8_exp2(y.y));
+          l = q8_fma2(e, unit2, l);
+          const float2 ww = q8_unpack(q8_mul2(e, d ? vs.y : vs.x));
           const __half2 h = __floats2half2_rn(ww.x, ww.y);
           w[c + d] = *reinterpret_cast<const uint32_t*>(&h);
         }
@@ -549,7 +527,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       }
       tc_fence_before();
     }
-    s_ml[threadIdx.x] = make_float2(mu_used, qt_unpack(l).x + qt_unpack(l).y);
+    s_ml[threadIdx.x] = make_float2(mu_used, q8_unpack(l).x + q8_unpack(l).y);
     asm volatile("bar.sync 1, 128;\n" ::: "memory");
     // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and the row
     // of the output (or of the partials) it goes to, -1 for none

@@ -62,11 +62,15 @@ int q8_cache(const dfl_kv_q8* c, const char* who, Q8Cache* out) {
 }
 
 // ---------------------------------------------------------------------------
-// Append. hd / 8 lanes per head, eight consecutive values each (one 16-byte load), so a warp holds
-// 256 / hd heads (a slot) at a time and a head's sums take log2(hd / 8) shuffles. A CTA takes ROWS
-// rows: its threads make the rows' (cos, sin) tables together, then 8 / ROWS warps walk each row's slots, a
-// slot's load in flight while the one before it is worked on. Few rows: one row a CTA and its
-// slots spread over CTAs (a slot a warp, for latency); many: four rows a CTA.
+// Append. hd / 8 lanes per head, eight values each, so a warp holds 256 / hd heads (a slot) at a time and a
+// head's sums take log2(hd / 8) shuffles. A CTA takes ROWS rows: its threads make the rows' (cos, sin)
+// tables together, then 8 / ROWS warps walk each row's slots. One row: its slots spread over CTAs (a slot a
+// warp, for latency). Two and four: a warp has four slots in flight through shared memory.
+// With many rows the issue of instructions bounds it before memory does, so a lane of the rotated dims holds four
+// values of the first half and their partners of the second (the rotation needs no other lane), the arithmetic
+// runs two values an instruction, and slots of q heads alone have a loop of their own. 16384 rows of
+// 32 + 16 heads of 128, int8: 80 us, 4.6 TB/s (eight consecutive values a lane, partners by shuffle, one value an
+// instruction, one slot in flight: 135 us; the lane layout and pairs alone: 111; the ring: 97; the q loop: 80).
 // ---------------------------------------------------------------------------
 struct AppendQ8Args {
   const __nv_bfloat16* qkv;
@@ -87,6 +91,7 @@ struct AppendQ8Args {
 };
 
 constexpr int APPEND_WARPS = 8;
+constexpr int APPEND_RING = 4;  // slots a warp has in flight (forms of several rows)
 
 // cos and sin of p * f: the product and its reduction by turns in fp64 (an fp32 product is off by
 // 2^-24 p f, 0.008 rad at position 131072), the reduced angle in fp32.
@@ -101,27 +106,35 @@ __device__ __forceinline__ float2 rope_cos_sin(int p, float f) {
 // Codes of four values x * up, rounded to nearest even: int8 by an addition of 1.5 * 2^23, whose sum's low
 // byte is the integer (|x * up| <= 127 up to rounding, so none is out of range).
 template <bool E4M3>
-__device__ __forceinline__ uint32_t q8_codes4(const float* x, float up) {
+__device__ __forceinline__ uint32_t q8_codes4(uint64_t x01, uint64_t x23, uint64_t up) {
+  const uint64_t y01 = q8_mul2(x01, up), y23 = q8_mul2(x23, up);
   if constexpr (E4M3) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * up, x[1] * up), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * up, x[3] * up), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(q8_unpack(y01), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(q8_unpack(y23), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
   } else {
-    uint32_t b[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[j], up), 12582912.f));
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    const uint64_t magic = q8_pack(12582912.f, 12582912.f);
+    const float2 a = q8_unpack(q8_add2(y01, magic)), b = q8_unpack(q8_add2(y23, magic));
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
   }
 }
 
+// two bf16 of a word as two fp32
+__device__ __forceinline__ uint64_t q8_bf16x2(uint32_t u) {
+  return q8_pack(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
 template <int HD, bool E4M3, int ROWS>
-__global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __grid_constant__ AppendQ8Args a) {
+__global__ void __launch_bounds__(32 * APPEND_WARPS, ROWS == 1 ? 1 : 4) append_q8_kernel(const __grid_constant__ AppendQ8Args a) {
   grid_dependency_launch_dependents();
   grid_dependency_wait();
   constexpr int LPH = HD / 8;               // lanes per head
   constexpr int HPW = 32 / LPH;             // heads per slot
   constexpr int WPR = APPEND_WARPS / ROWS;  // warps per row
+  constexpr bool RINGED = ROWS > 1;
   __shared__ float2 cs[ROWS][HD / 2];
+  __shared__ uint4 ring[RINGED ? APPEND_WARPS : 1][APPEND_RING][32];
   const int m0 = blockIdx.x * ROWS;
   const int half = a.rot_dim >> 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -130,19 +143,39 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __gr
   const int sub = lane / LPH, l = lane % LPH;  // head within the slot, lane within the head
   const int Hkv = a.c.Hkv;
   const int n_heads = a.Hq + 2 * Hkv;
-  const __nv_bfloat16* row = a.qkv + (long long)m * a.ldqkv + l * 8;
+  // this lane's eight values: i .. i + 3 of both halves of the rotated dims, or eight behind those
+  const bool turned = l < half / 4;
+  const int d0 = turned ? 4 * l : a.rot_dim + 8 * (l - half / 4), d1 = d0 + (turned ? half : 4);
+  const __nv_bfloat16* row = a.qkv + (long long)m * a.ldqkv;
   const long long kv0 = (long long)a.Hq * a.q_stride;
-  auto load = [&](int slot) -> uint4 {
-    const int h = slot * HPW + sub;
-    if (p < 0 || h < a.first_head || h >= n_heads) return make_uint4(0, 0, 0, 0);
-    return *reinterpret_cast<const uint4*>(row + (h < a.Hq ? (long long)h * a.q_stride : kv0 + (long long)(h - a.Hq) * HD));
+  auto head_at = [&](int h) { return row + (h < a.Hq ? (long long)h * a.q_stride : kv0 + (long long)(h - a.Hq) * HD); };
+  auto load = [&](const __nv_bfloat16* x) -> uint4 {
+    const uint2 lo = *reinterpret_cast<const uint2*>(x + d0), hi = *reinterpret_cast<const uint2*>(x + d1);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
   };
   const int slots = (n_heads + HPW - 1) / HPW;
   const int slot0 = a.first_head / HPW + blockIdx.y * a.slots_per_cta;
   const int slot_end = min(slots, slot0 + a.slots_per_cta);
   int slot = slot0 + warp % WPR;
+  // one-row form: this warp's slot; four-row form: slot `s`, the i-th of this warp, into its place in the ring
   uint4 nx = make_uint4(0, 0, 0, 0);
-  if (slot < slot_end) nx = load(slot);
+  auto fetch = [&](int s, int i) {
+    if (p >= 0 && s < slot_end) {
+      const __nv_bfloat16* x = head_at(min(s * HPW + sub, n_heads - 1));
+      if constexpr (RINGED) {
+        cp_async16(smem_u32(&ring[warp][i % APPEND_RING][lane]), x + 8 * l, 16);
+      } else {
+        nx = load(x);
+      }
+    }
+    if constexpr (RINGED) cp_async_commit();
+  };
+  if constexpr (RINGED) {
+#pragma unroll
+    for (int i = 0; i < APPEND_RING - 1; ++i) fetch(slot + i * WPR, i);
+  } else {
+    fetch(slot, 0);
+  }
   // tables: thread t makes entries t, t + 256, ... of the CTA's rows
   for (int i = threadIdx.x; i < ROWS * half; i += 32 * APPEND_WARPS) {
     const int r = ROWS == 1 ? 0 : i / half, k = ROWS == 1 ? i : i - r * half;
@@ -155,82 +188,122 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) append_q8_kernel(const __gr
   long long page = 0;
   int prow = 0;
   const bool placed = q8_place(a.c, seq, p, lane == 0 ? a.err : nullptr, page, prow);
-  // this lane's rotation: its eight values are i .. i + 7 of the first half (partner half / 8
-  // lanes up), of the second (down), or behind the rotated dims (turned by 0)
-  const int hl = half / 8;
-  const bool first = l < hl, second = l >= hl && l < 2 * hl;
-  const int src = sub * LPH + (first ? l + hl : second ? l - hl : l);
-  float cr[8], sr[8];
+  // x' = x cos - partner sin of the first half, x cos + partner sin of the second; other dims: cos 1, sin 0
+  uint64_t cr[2], sp[2], sn[2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float2 t = first || second ? cs[warp / WPR][(first ? l : l - hl) * 8 + j] : make_float2(1.f, 0.f);
-    cr[j] = t.x;
-    sr[j] = first ? -t.y : t.y;  // x' = x cos -/+ partner sin
+  for (int j = 0; j < 2; ++j) {
+    const float2 t0 = turned ? cs[warp / WPR][4 * l + 2 * j] : make_float2(1.f, 0.f);
+    const float2 t1 = turned ? cs[warp / WPR][4 * l + 2 * j + 1] : make_float2(1.f, 0.f);
+    cr[j] = q8_pack(t0.x, t1.x);
+    sp[j] = q8_pack(t0.y, t1.y);
+    sn[j] = q8_pack(-t0.y, -t1.y);
   }
-  const uint4 qw = *reinterpret_cast<const uint4*>(a.q_norm + l * 8);
-  const uint4 kw = *reinterpret_cast<const uint4*>(a.k_norm + l * 8);
-  const long long code0 = page * a.c.seq_stride + (long long)prow * HD + l * 8;
+  uint64_t w[4];  // the norm's weights
+  auto weights = [&](const __nv_bfloat16* g) {
+    const uint2 lo = *reinterpret_cast<const uint2*>(g + d0), hi = *reinterpret_cast<const uint2*>(g + d1);
+    w[0] = q8_bf16x2(lo.x);
+    w[1] = q8_bf16x2(lo.y);
+    w[2] = q8_bf16x2(hi.x);
+    w[3] = q8_bf16x2(hi.y);
+  };
+  const long long code0 = page * a.c.seq_stride + (long long)prow * HD;
   const long long scale0 = page * a.c.s_seq_stride + prow;
+  int i = 0;  // the slot's number among this warp's
+  auto take = [&](uint64_t (&x)[4]) {
+    if constexpr (RINGED) {
+      __syncwarp();  // every lane has read the place that this fetch fills
+      fetch(slot + (APPEND_RING - 1) * WPR, i + APPEND_RING - 1);
+      cp_async_wait<APPEND_RING - 1>();
+      __syncwarp();
+      nx = load(reinterpret_cast<const __nv_bfloat16*>(&ring[warp][i % APPEND_RING][sub * LPH]));
+    }
+    x[0] = q8_bf16x2(nx.x);
+    x[1] = q8_bf16x2(nx.y);
+    x[2] = q8_bf16x2(nx.z);
+    x[3] = q8_bf16x2(nx.w);
+  };
+  auto inverse_norm = [&](const uint64_t (&x)[4]) -> float {
+    uint64_t sq = q8_mul2(x[0], x[0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) sq = q8_fma2(x[j], x[j], sq);
+    const float2 s2 = q8_unpack(sq);
+    float ss = s2.x + s2.y;
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return rsqrtf(ss * (1.f / (float)HD) + a.eps);
+  };
+  auto turn = [&](uint64_t (&x)[4], float inv) {
+    const uint64_t inv2 = q8_pack(inv, inv);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = q8_mul2(w[j], q8_mul2(x[j], inv2));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t y = x[j], z = x[2 + j];
+      x[j] = q8_fma2(y, cr[j], q8_mul2(z, sn[j]));
+      x[2 + j] = q8_fma2(z, cr[j], q8_mul2(y, sp[j]));
+    }
+  };
+  auto put_q = [&](const uint64_t (&x)[4], int h) {
+    __nv_bfloat16* o = a.q_out + ((long long)m * a.Hq + h) * HD;
+    const float2 f0 = q8_unpack(x[0]), f1 = q8_unpack(x[1]), f2 = q8_unpack(x[2]), f3 = q8_unpack(x[3]);
+    *reinterpret_cast<uint2*>(o + d0) = make_uint2(pack_bf16x2(f0.x, f0.y), pack_bf16x2(f1.x, f1.y));
+    *reinterpret_cast<uint2*>(o + d1) = make_uint2(pack_bf16x2(f2.x, f2.y), pack_bf16x2(f3.x, f3.y));
+  };
+  // slots of q heads alone
+  if (a.first_head == 0) {
+    weights(a.q_norm);
+    const int q_end = min(slot_end, a.Hq / HPW);
 #pragma unroll 1
-  for (; slot < slot_end; slot += WPR) {
-    const uint32_t u[4] = {nx.x, nx.y, nx.z, nx.w};
-    if (slot + WPR < slot_end) nx = load(slot + WPR);
+    for (; slot < q_end; slot += WPR, ++i) {
+      uint64_t x[4];
+      take(x);
+      turn(x, inverse_norm(x));
+      put_q(x, slot * HPW + sub);
+    }
+  }
+  // the others: k and v heads, and a slot that begins with q heads
+  if (slot < slot_end) weights(slot * HPW + sub < a.Hq ? a.q_norm : a.k_norm);
+#pragma unroll 1
+  for (; slot < slot_end; slot += WPR, ++i) {
+    uint64_t x[4];
+    take(x);
     const int h = slot * HPW + sub;
     const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + Hkv;
     const bool live = h >= a.first_head && h < n_heads && (is_q || placed);
-    float x[8];
+    if (slot * HPW < a.Hq + Hkv) {  // some head of the slot is a q or k head: norm and rotation
+      const float inv = inverse_norm(x);
+      if (is_q || is_k) turn(x, inv);
+      if (is_q) {
+        if (live) put_q(x, h);
+        weights(a.k_norm);
+      }
+    }
+    // the maximum magnitude as an unsigned comparison of the bits, in which a NaN or an
+    // infinity is larger than every finite value
+    unsigned am = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[2 * j] = __uint_as_float(u[j] << 16);
-      x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+      const float2 f = q8_unpack(x[j]);
+      am = max(am, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
     }
-    if (slot * HPW < a.Hq + Hkv) {  // some head of the slot is a q or k head: norm and rotation
-      float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = sq_acc(ss, x[j]);
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = rsqrtf(ss * (1.f / (float)HD) + a.eps);
-      const uint32_t wu[4] = {is_q ? qw.x : kw.x, is_q ? qw.y : kw.y, is_q ? qw.z : kw.z, is_q ? qw.w : kw.w};
-      const bool turn = is_q || is_k;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float wj = __uint_as_float(j & 1 ? wu[j >> 1] & 0xffff0000u : wu[j >> 1] << 16);
-        const float y = wj * (x[j] * inv);
-        const float z = __shfl_sync(0xffffffffu, y, src);
-        const float r = __fmaf_rn(y, cr[j], z * sr[j]);
-        x[j] = turn ? r : x[j];
-      }
-    }
-    if (is_q && live) {
-      uint4 o;
-      o.x = pack_bf16x2(x[0], x[1]);
-      o.y = pack_bf16x2(x[2], x[3]);
-      o.z = pack_bf16x2(x[4], x[5]);
-      o.w = pack_bf16x2(x[6], x[7]);
-      *reinterpret_cast<uint4*>(a.q_out + ((long long)m * a.Hq + h) * HD + l * 8) = o;
-    }
-    if (slot * HPW + HPW > a.Hq) {  // some head of the slot is a k or v head: quantise
-      // the maximum magnitude as an unsigned comparison of the bits, in which a NaN or an
-      // infinity is larger than every finite value
-      unsigned am = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) am = max(am, __float_as_uint(x[j]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-      if (!is_q && live) {
-        constexpr float TOP = E4M3 ? 448.f : 127.f;
-        const bool finite = am < 0x7f800000u;
-        const float amax = __uint_as_float(am);
-        // below 2^-119 the reciprocal would overflow: such a row is all but zero, and is held as zeros
-        const bool some = finite && amax >= 1.5046328e-36f;
-        const float up = some ? __fdiv_rn(TOP, amax) : 0.f;
-        const float scale = finite ? (some ? __fdiv_rn(amax, TOP) : 0.f) : __uint_as_float(0x7fc00000u);
-        const uint32_t c0 = some ? q8_codes4<E4M3>(x, up) : 0u, c1 = some ? q8_codes4<E4M3>(x + 4, up) : 0u;
-        const int kh = h - a.Hq - (is_k ? 0 : Hkv);
-        *reinterpret_cast<uint2*>((is_k ? a.c.k : a.c.v) + code0 + kh * a.c.head_stride) = make_uint2(c0, c1);
-        if (l == 0) (is_k ? a.c.ks : a.c.vs)[scale0 + kh * a.c.s_head_stride] = scale;
-      }
+    for (int o = LPH / 2; o > 0; o >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+    if (!is_q && live) {
+      constexpr float TOP = E4M3 ? 448.f : 127.f;
+      const bool finite = am < 0x7f800000u;
+      const float amax = __uint_as_float(am);
+      // below 2^-119 the reciprocal would overflow: such a row is all but zero, and is held as zeros
+      const bool some = finite && amax >= 1.5046328e-36f;
+      const float up = some ? __fdiv_rn(TOP, amax) : 0.f;
+      const float scale = finite ? (some ? __fdiv_rn(amax, TOP) : 0.f) : __uint_as_float(0x7fc00000u);
+      const uint64_t up2 = q8_pack(up, up);
+      const uint32_t c0 = some ? q8_codes4<E4M3>(x[0], x[1], up2) : 0u;
+      const uint32_t c1 = some ? q8_codes4<E4M3>(x[2], x[3], up2) : 0u;
+      const int kh = h - a.Hq - (is_k ? 0 : Hkv);
+      unsigned char* codes = (is_k ? a.c.k : a.c.v) + code0 + kh * a.c.head_stride;
+      *reinterpret_cast<uint32_t*>(codes + d0) = c0;
+      *reinterpret_cast<uint32_t*>(codes + d1) = c1;
+      if (l == 0) (is_k ? a.c.ks : a.c.vs)[scale0 + kh * a.c.s_head_stride] = scale;
     }
   }
 }
@@ -370,24 +443,31 @@ extern "C" int dfl_qkv_rope_append_q8(const void* qkv, int64_t ldqkv, int q_stri
   a.err = device_error_word();
   const int per_slot = 256 / hd;
   const int slots = (Hq + 2 * cache->n_kv_heads + per_slot - 1) / per_slot;
-  // Up to about four CTAs an SM: one row each, its slots over CTAs of eight. Beyond: four rows a CTA
-  // (16384 rows of 48 heads of 128: APPEND_TIMES).
+  // Up to about four CTAs an SM: one row each, its slots over CTAs of eight. Beyond: two rows a CTA, with more
+  // than 16 rows an SM four, whose tables cost less a row (24 + 8 heads of 256: 256 rows 6.4 us
+  // with two, 10.4 with four; 1024 10.5 and 12.4; 16384 105 and 98).
   const int groups = (slots - a.first_head / per_slot + APPEND_WARPS - 1) / APPEND_WARPS;
-  const bool few = (long long)M * groups <= 148 * 4;
-  a.slots_per_cta = few ? APPEND_WARPS : slots;
-  const dim3 grid(few ? M : (M + 3) / 4, few ? groups : 1);
+  const int rows = (long long)M * groups <= 148 * 4 ? 1 : M <= 148 * 16 ? 2 : 4;
+  a.slots_per_cta = rows == 1 ? APPEND_WARPS : slots;
+  const dim3 grid((M + rows - 1) / rows, rows == 1 ? groups : 1);
   cudaStream_t st = as_stream(stream);
   const int thr = 32 * APPEND_WARPS;
   const bool e4 = cache->type == DFL_KV_E4M3;
-#define APPEND_Q8(HD)                                                                                              \
-  return few ? launch_q8(e4 ? append_q8_kernel<HD, true, 1> : append_q8_kernel<HD, false, 1>, a, grid, thr, who, st) \
-             : launch_q8(e4 ? append_q8_kernel<HD, true, 4> : append_q8_kernel<HD, false, 4>, a, grid, thr, who, st)
+#define APPEND_Q8_T(HD, E4)                                                      \
+  return launch_q8(rows == 1   ? append_q8_kernel<HD, E4, 1>                    \
+                   : rows == 2 ? append_q8_kernel<HD, E4, 2>                    \
+                               : append_q8_kernel<HD, E4, 4>,                   \
+                   a, grid, thr, who, st)
+#define APPEND_Q8(HD)         \
+  if (e4) APPEND_Q8_T(HD, true); \
+  APPEND_Q8_T(HD, false)
   switch (hd) {
     case 64: APPEND_Q8(64);
     case 128: APPEND_Q8(128);
     default: APPEND_Q8(256);
   }
 #undef APPEND_Q8
+#undef APPEND_Q8_T
 }
 
 extern "C" int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq, int M, void* k_out,

@@ -404,3 +404,61 @@ def test_views_streams_and_graphs(form, chunk):
         graphs[0].replay()
         torch.cuda.synchronize()
         check()
+
+
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 512)])
+@pytest.mark.parametrize("B,rows,Hkv,G,hd,causal", [
+    (60, 3, 4, 4, 128, True), (60, 1, 4, 2, 64, False), (45, 16, 4, 3, 256, True), (255, 1, 1, 8, 128, True),
+    (256, 2, 1, 8, 128, False), (300, 2, 1, 4, 64, True)])
+def test_order_of_runs_changes_nothing(B, rows, Hkv, G, hd, causal, form, chunk):
+    """Calls of many runs start the longest first; the answer is that of one call a run, bit for bit."""
+    from dflash_b200 import ops
+    g = torch.Generator().manual_seed(B)
+    lens = [int(x) for x in torch.randint(rows, 600, (B,), generator=g)]
+    lens[3] = lens[4] = lens[5]  # ties
+    c = Cache("int8", lens, Hkv, hd, 64, seed=B)
+    q = torch.randn(B * rows, Hkv * G, hd, generator=g).bfloat16().to(DEV)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32)
+    pos[7 * rows:8 * rows] = -1
+    pos[9 * rows + rows - 1] = -1
+    pos, kv_len = pos.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    seq = torch.arange(B, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+
+    def call(a, b):
+        out = torch.full((b - a, Hkv * G * hd), 9.0, dtype=torch.bfloat16, device=DEV)
+        return ops.attention_q8(q[a:b], c.kv, pos[a:b], causal, 640, kv_len=kv_len, row_seq=seq[a:b], seq_rows=rows,
+                                form=form, key_chunk=chunk, out=out)
+
+    whole = call(0, B * rows)
+    parts = torch.cat([call(b * rows, (b + 1) * rows) for b in range(B)])
+    assert ops.device_error() == 0
+    assert torch.equal(whole, parts)
+    assert (whole[7 * rows:8 * rows] == 9).all() and whole.isfinite().all()
+
+
+@pytest.mark.parametrize("t", ["int8", "e4m3"])
+@pytest.mark.parametrize("M,Hq,Hkv,hd,rot,do_q", [
+    (700, 6, 3, 128, 128, True), (2501, 3, 2, 64, 32, True), (701, 3, 2, 64, 16, False), (2402, 5, 1, 256, 64, True)])
+def test_append_of_many_rows_is_that_of_few(t, M, Hq, Hkv, hd, rot, do_q):
+    from dflash_b200 import ops
+    g = torch.Generator().manual_seed(M)
+    qkv = torch.randn(M, (Hq + 2 * Hkv) * hd, generator=g).bfloat16().to(DEV)
+    qn, kn = [(1 + 0.2 * torch.randn(hd, generator=g)).bfloat16().to(DEV) for _ in range(2)]
+    inv = torch.rand(rot // 2, generator=g).to(DEV)
+    pos = torch.randperm(M + 40, generator=g)[:M].to(torch.int32)
+    pos[5] = pos[M - 1] = -1
+    pos = pos.to(DEV)
+    got = []
+    for step in (M, 11):
+        codes = torch.full((2, 1, Hkv, M + 40, hd), 0x55, dtype=torch.uint8, device=DEV).view(TYPES[t])
+        scale = torch.full((2, 1, Hkv, M + 40), 77.0, device=DEV)
+        kv = ops.QuantKV(codes[0], codes[1], scale[0], scale[1])
+        q = torch.full((M, Hq, hd), 9.0, dtype=torch.bfloat16, device=DEV)
+        for i in range(0, M, step):
+            j = min(i + step, M)
+            ops.qkv_rope_append_q8(qkv[i:j], pos[i:j], qn, kn, inv, kv, Hq, rot, 1e-6,
+                                   q_out=q[i:j] if do_q else None, do_q=do_q)
+        got.append((codes.view(torch.uint8), scale, q))
+    assert ops.device_error() == 0
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
