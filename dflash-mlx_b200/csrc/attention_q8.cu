@@ -5,8 +5,8 @@
 //
 // Work split: one CTA per (run tile, kv head, key chunk). A run is the rows of one sequence; its
 // tile's rows are (token, query head of the group) pairs packed without gaps, so a single token
-// with G heads fills G rows of one 16-row MMA tile and a 16-token verify block with G = 4 the 64
-// rows of a full CTA: K and V are read once for all of them. The four warps of a row group are
+// with G heads fills G rows of one 16-row MMA tile. Small calls take tiles of 16 rows (more CTAs, lower latency),
+// large ones 32 or 64 (a 16-token verify block with G = 4), which read K and V once for all of them. The four warps of a row group are
 // four strands: strand s takes the 32-key blocks s, s + 4, ... of the chunk with its own running
 // maximum and sum, and the strands are merged in order at the end. Chunks are merged in order by
 // a second kernel (one chunk: written directly). A row's arithmetic depends on the chunk size and
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
   int* s_lim = reinterpret_cast<int*>(smem + L::OFF_F) + L::ROWS;
   __shared__ int s_tok_lim[L::ROWS], s_tok_ok[L::ROWS];
 
-  grid_dependency_launch_dependents();
   grid_dependency_wait();
+  grid_dependency_launch_dependents();  // the merge kernel relies on this order
 
   const Q8Tile at = q8_tile(a);
   const int run = at.run, tile = at.tile, kvh = at.kvh, chunk = blockIdx.y;
@@ -481,51 +481,70 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
     }
 }
 
-// Merges the chunk partials of one (row, head) in chunk order: one warp each, hd / 32 dims a lane.
+// Merges the chunk partials of one (row, head) in chunk order: one warp each, hd / 32 dims a lane. What it needs
+// to know of the row is read before it waits for the chunk kernel, which lets it start only after what came before
+// both; behind the wait the first partials are loaded together with their maxima and sums.
 template <int HD>
 __global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constant__ AttnQ8Args a) {
   grid_dependency_launch_dependents();
-  grid_dependency_wait();
   constexpr int VEC = HD / 32;
   constexpr int FL = 8;  // chunks' loads in flight
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
-  if (item >= (long long)a.M * a.Hq) return;
-  const int m = (int)(item / a.Hq), h = (int)(item % a.Hq);
-  const int p = a.pos[m];
-  if (p < 0) return;
-  const int seq = a.row_seq ? a.row_seq[m] : 0;
-  if (seq < 0 || seq >= a.c.n_seqs) return;
-  if (a.row_seq && a.run_rows > 1) {  // a row that is not of its tile's sequence was refused
+  bool live = item < (long long)a.M * a.Hq;
+  const int m = live ? (int)(item / a.Hq) : 0, h = (int)(item - (long long)m * a.Hq);
+  const int p = __ldcg(a.pos + m), seq = a.row_seq ? __ldcg(a.row_seq + m) : 0;
+  live = live && p >= 0 && seq >= 0 && seq < a.c.n_seqs;
+  if (live && a.row_seq && a.run_rows > 1) {  // a row that is not of its tile's sequence was refused
     const int run0 = m / a.run_rows * a.run_rows;
-    const int t0 = run0 + (m - run0) / a.tile_toks * a.tile_toks;
-    int first = t0;
-    while (a.pos[first] < 0) ++first;  // ends at m at the latest
-    if (a.row_seq[first] != seq) return;
+    int first = run0 + (m - run0) / a.tile_toks * a.tile_toks;
+    while (__ldcg(a.pos + first) < 0) ++first;  // ends at m at the latest
+    live = __ldcg(a.row_seq + first) == seq;
   }
-  const int lim = q8_row_limit(a, m, p, seq, nullptr);
+  const int lim = live ? q8_row_limit(a, m, p, seq, nullptr) : 0;
   const int nch = lim > 0 ? min((lim - 1) / a.key_chunk + 1, a.n_chunks) : 0;
+  grid_dependency_wait();
+  if (!live) return;
   const long long cstride = (long long)a.M * a.Hq;
   const float2* ml = a.part_ml + item;
   const float* po = a.part_o + item * HD + lane * VEC;
-  float mmax = -INFINITY;
-  for (int c = lane; c < nch; c += 32) mmax = fmaxf(mmax, ml[c * cstride].x);
+  float v[FL][VEC];
+  auto fetch = [&](int c) {  // the partials of chunks c .. c + FL - 1
+#pragma unroll
+    for (int u = 0; u < FL; ++u) {
+      const float* src = po + (long long)(c + u) * cstride * HD;
+      if constexpr (VEC == 2) {
+        const float2 y = c + u < nch ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
+        v[u][0] = y.x;
+        v[u][1] = y.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+          const float4 y = c + u < nch ? *reinterpret_cast<const float4*>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[u][i] = y.x;
+          v[u][i + 1] = y.y;
+          v[u][i + 2] = y.z;
+          v[u][i + 3] = y.w;
+        }
+      }
+    }
+  };
+  float2 x = lane < nch ? ml[lane * cstride] : make_float2(-INFINITY, 0.f);
+  fetch(0);
+  float mmax = x.x;
+  for (int c = lane + 32; c < nch; c += 32) mmax = fmaxf(mmax, ml[c * cstride].x);
   mmax = warp_max(mmax);
   const float mu = mmax == -INFINITY ? 0.f : mmax;
   float acc[VEC], den = 0.f;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   for (int c0 = 0; c0 < nch; c0 += 32) {
-    const float2 x = c0 + lane < nch ? ml[(c0 + lane) * cstride] : make_float2(-INFINITY, 0.f);
+    if (c0 > 0) x = c0 + lane < nch ? ml[(c0 + lane) * cstride] : make_float2(-INFINITY, 0.f);
     const float w = exp2f(x.x - mu);
     den += warp_sum(w * x.y);
     const int n = min(32, nch - c0);
     for (int j0 = 0; j0 < n; j0 += FL) {
-      float v[FL][VEC];
-#pragma unroll
-      for (int u = 0; u < FL; ++u)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[u][i] = j0 + u < n ? po[(long long)(c0 + j0 + u) * cstride * HD + i] : 0.f;
+      if (c0 + j0 > 0) fetch(c0 + j0);
 #pragma unroll
       for (int u = 0; u < FL; ++u) {
         const float wj = __shfl_sync(0xffffffffu, w, (j0 + u) & 31);
@@ -621,24 +640,35 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
   return one_seq ? M : seq_rows > 0 ? (seq_rows < M ? seq_rows : M) : 1;
 }
 
-// The form and the keys per chunk of a call. The tcgen05 form for calls of more than 16 (token, head) rows a
-// run, whose tile of 64 rows they fill, and with work for it: 512 keys a CTA on every SM (its CTAs start
-// and end slowly). Measured: 64 sequences of 512 to 4096 keys, one token each 66 (warp) against 107 us, 16
-// tokens 338 against 134; one sequence of 1053 keys, 16 tokens 17 against 21.
-// Chunks: as many as keep every CTA in one wave (three CTAs an SM, two in the tcgen05 form, one at
-// head_dim 256), one more for several runs, whose lengths may differ. One chunk needs no merge.
+// The form, tile rows and keys per chunk of a call.
+// Few: runs of at most 16 (token, head) rows, and calls small enough that tiles of 16 rows with 384 keys each
+// fit one wave (three CTAs an SM, one at head_dim 256). They take the warp form in 16-row tiles, for
+// their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128: 10.3 us (64-row tiles 15.2, tcgen05
+// 16.2), 4096 keys 16.0 (20.5, 16.5). Others take the tcgen05 form, which reads K and V once per 64 rows: four such
+// sequences of 2048 keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 130 (338 in 64-row
+// tiles); 64 single tokens 107, in the warp form 66.
+// Chunks: as many as keep every CTA in one wave (tcgen05: two an SM, at head_dim 256 one), one more for several
+// runs (warp form: that have four and more), as their lengths may differ: 8 sequences of 512 to 6000 keys, 16
+// tokens of 24 heads of 256, 66 us with the one more, 81 without. One chunk needs no merge, and each costs the merge and its CTA's
+// start: at least 128 keys, 256 where those make more than 16 chunks (one token, 4096 keys: 9.2 us, with
+// 128 11.1), and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in
+// two 13.6).
 struct Q8Plan {
-  int form, key_chunk, n_chunks;
+  int form, rows, key_chunk, n_chunks;  // rows: (token, head) pairs a CTA takes
 };
 static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int G, int Hkv, int hd, int max_kv) {
   Q8Plan p;
-  const long long want = (long long)run_rows * G;
-  const long long units = runs * Hkv * ((want + 63) / 64);
-  p.form = form != DFL_Q8_AUTO ? form : want > 16 && units * max_kv >= 148 * 512 ? DFL_Q8_TC : DFL_Q8_WARP;
+  const long long want = (long long)run_rows * G, wave = 148 * (hd == 256 ? 1 : 3);
+  auto units = [&](int rows) { return runs * Hkv * ((run_rows + rows / G - 1) / (rows / G)); };
+  const bool few = want <= 16 || units(16) * max_kv <= wave * 384;
+  p.form = form != DFL_Q8_AUTO ? form : few ? DFL_Q8_WARP : DFL_Q8_TC;
+  const bool tc = p.form == DFL_Q8_TC;
+  p.rows = tc ? 64 : few ? 16 : want <= 32 || hd == 256 ? 32 : 64;
   if (key_chunk <= 0) {
-    const long long slots = 148 * (p.form == DFL_Q8_TC ? (hd == 256 ? 1 : 2) : 3);
-    const long long n = slots / units + (runs > 1 && slots % units ? 1 : 0);
-    const long long lo = p.form == DFL_Q8_TC ? 512 : Q8_CHUNK_UNIT;
+    const long long slots = tc ? 148 * (hd == 256 ? 1 : 2) : p.rows == 64 ? 148 : wave, u = units(p.rows);
+    long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 : slots >= 4 * u) ? 1 : 0);
+    if (!tc && u > 74 && max_kv <= 512) n = 1;
+    const long long lo = tc ? 512 : max_kv <= 16 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
     long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
     c = c < lo ? lo : c > 8192 ? 8192 : c;
     key_chunk = (int)((c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT);
@@ -657,7 +687,8 @@ static size_t q8_workspace(int M, int Hq, int hd, int n_chunks) {
 extern "C" size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq,
                                                    int max_kv, int form, int key_chunk) {
   if (!cache || M <= 0 || Hq <= 0 || max_kv <= 0 || key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT ||
-      cache->n_kv_heads <= 0 || form < DFL_Q8_AUTO || form > DFL_Q8_TC)
+      cache->n_kv_heads <= 0 || Hq % cache->n_kv_heads || Hq / cache->n_kv_heads > 16 || form < DFL_Q8_AUTO ||
+      form > DFL_Q8_TC)
     return 0;
   const int rr = q8_run_rows(M, seq_rows, one_seq != 0);
   return q8_workspace(M, Hq, cache->head_dim,
@@ -716,10 +747,7 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
     return DFL_ERR_WORKSPACE;
   }
   const bool tc = plan.form == DFL_Q8_TC;
-  // rows a CTA takes: 16, 32 or (tcgen05 form, or head_dim <= 128) 64 (token, head) pairs
-  const int most = hd == 256 && !tc ? 32 : 64;
-  const long long want = (long long)run_rows * G;
-  const int rows = tc ? 64 : want <= 16 ? 16 : want <= 32 ? 32 : most;
+  const int rows = plan.rows;
   a.run_rows = run_rows;
   a.run_tiles = (run_rows + rows / G - 1) / (rows / G);
   a.tile_toks = (run_rows + a.run_tiles - 1) / a.run_tiles;

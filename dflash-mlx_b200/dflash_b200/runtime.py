@@ -124,7 +124,7 @@ class SpecSession:
         # an 8-bit cache's attention: form and keys per split of the steps and of the prefill chunks
         self.step_split, self.prefill_split = {"key_chunk": self.key_chunk}, {"key_chunk": self.key_chunk}
         if kv_dtype != "bf16":
-            form, chunk = q8_split(batch, tc.num_key_value_heads, max_total)
+            form, chunk = q8_split(batch, tc.num_key_value_heads, max_total, tc.head_dim)
             self.step_split = {"form": form, "key_chunk": chunk}
             self.prefill_split = {"form": "tc", "key_chunk": 1024}
         self.max_steps = max_steps or (max_total + 1)

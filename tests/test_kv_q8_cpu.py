@@ -92,3 +92,15 @@ def test_wrappers_take_cuda_tensors_only():
     s = torch.zeros((1, 2, 64))
     with pytest.raises(ValueError, match="CUDA"):
         ops.QuantKV(z, z, s, s)
+
+
+def test_scratch_query_answers_0_where_the_call_would_refuse(lib):
+    """Head counts that the attention refuses (no whole group, more than 16 heads a group, none at
+    all) give 0 bytes, not an arithmetic fault."""
+    from dflash_b200 import _lib, ops
+    c = ops.KvQ8(n_kv_heads=8, n_seqs=1, cap=4096, head_dim=128)
+    ref = ctypes.byref(c)
+    for Hq in (4, 12, 136, 264):
+        assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, Hq, 16, 1, 4096, 0, 0) == 0
+    assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, 32, 16, 1, 4096, 0, 0) > 0
+    assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, 128, 16, 1, 4096, 1, 128) > 0

@@ -462,3 +462,28 @@ def test_append_of_many_rows_is_that_of_few(t, M, Hq, Hkv, hd, rot, do_q):
     assert ops.device_error() == 0
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", ["int8", "e4m3"])
+@pytest.mark.parametrize("lens,rows,Hkv,G,hd,causal,gated", [
+    ([700, 33, 400], 8, 4, 4, 128, True, False), ([130, 517], 20, 4, 4, 128, True, True),
+    ([300, 257], 9, 8, 3, 64, False, False), ([391, 64], 7, 4, 6, 256, True, True)])
+def test_larger_tiles_of_the_warp_form(t, lens, rows, Hkv, G, hd, causal, gated):
+    """The warp form's tiles hold 16 rows when the call is small and 32 or 64 when max_kv (here far
+    above the lengths) makes it large: the same bits, and within the tolerance of 64 bits."""
+    from dflash_b200 import ops
+    c = Cache(t, lens, Hkv, hd, 64, seed=hd)
+    g = torch.Generator().manual_seed(9)
+    B, Hq = len(lens), Hkv * G
+    q = (1.5 * torch.randn(B * rows, Hq, hd, generator=g)).bfloat16()
+    seq = torch.arange(B, dtype=torch.int32).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32)
+    kv_len = torch.tensor(lens, dtype=torch.int32)
+    gate = torch.randn(B * rows, Hq * hd, generator=g).bfloat16() if gated else None
+    d = [x if x is None else x.to(DEV) for x in (q, pos, kv_len, seq, gate)]
+    got = [ops.attention_q8(d[0], c.kv, d[1], causal, max_kv, kv_len=d[2], row_seq=d[3], seq_rows=rows, form="warp",
+                            key_chunk=256, gate=d[4]) for max_kv in (max(lens), 60000)]
+    assert ops.device_error() == 0
+    assert torch.equal(*got)
+    ref, tol = _attention64(c.val, q, pos + 1 if causal else kv_len[seq.long()], seq, hd ** -0.5, gate)
+    assert ((got[0].double().cpu() - ref).abs() <= tol).all()
