@@ -644,15 +644,17 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // Few: runs of at most 16 (token, head) rows, and calls small enough that tiles of 16 rows with 384 keys each
 // fit one wave (three CTAs an SM, one at head_dim 256). They take the warp form in 16-row tiles, for
 // their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128: 10.3 us (64-row tiles 15.2, tcgen05
-// 16.2), 4096 keys 16.0 (20.5, 16.5). Others take the tcgen05 form, which reads K and V once per 64 rows: four such
-// sequences of 2048 keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 130 (338 in 64-row
-// tiles); 64 single tokens 107, in the warp form 66.
-// Chunks: as many as keep every CTA in one wave (tcgen05: two an SM, at head_dim 256 one), one more for several
-// runs (warp form: that have four and more), as their lengths may differ: 8 sequences of 512 to 6000 keys, 16
-// tokens of 24 heads of 256, 66 us with the one more, 81 without. One chunk needs no merge, and each costs the merge and its CTA's
-// start: at least 128 keys, 256 where those make more than 16 chunks (one token, 4096 keys: 9.2 us, with
-// 128 11.1), and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in
-// two 13.6).
+// 16.2), 4096 keys 16.0 (20.5, 16.5). Others take a tcgen05 form, tc of 64 rows a CTA: four such sequences of 2048
+// keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 124 (338 in 64-row tiles); 64 single
+// tokens 107, in the warp form 66. Wide, of 256 rows (head_dim 256: 128), for runs that fill more than half of them
+// and calls with 384 keys for every SM: 128 rows of 32 heads at 4096 keys 30 us (tc 36), at 1024 28 (17);
+// 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256, 50 us (tc 57).
+// Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for several
+// runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 57 us
+// with it, 72 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
+// keys, 256 where those make more than 16 chunks (one token, 4096 keys: 9.2 us, with 128 11.1), in the tcgen05
+// forms 512, and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us,
+// split in two 13.6).
 struct Q8Plan {
   int form, rows, key_chunk, n_chunks;  // rows: (token, head) pairs a CTA takes
 };
@@ -661,11 +663,15 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
   const long long want = (long long)run_rows * G, wave = 148 * (hd == 256 ? 1 : 3);
   auto units = [&](int rows) { return runs * Hkv * ((run_rows + rows / G - 1) / (rows / G)); };
   const bool few = want <= 16 || units(16) * max_kv <= wave * 384;
-  p.form = form != DFL_Q8_AUTO ? form : few ? DFL_Q8_WARP : DFL_Q8_TC;
-  const bool tc = p.form == DFL_Q8_TC;
-  p.rows = tc ? 64 : few ? 16 : want <= 32 || hd == 256 ? 32 : 64;
+  const int wide = hd == 256 ? 128 : 256;
+  p.form = form != DFL_Q8_AUTO                                              ? form
+           : few                                                          ? DFL_Q8_WARP
+           : want > wide / 2 && units(wide) * max_kv >= (long long)148 * 384 ? DFL_Q8_WIDE
+                                                                          : DFL_Q8_TC;
+  const bool tc = p.form >= DFL_Q8_TC;
+  p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? 16 : want <= 32 || hd == 256 ? 32 : 64;
   if (key_chunk <= 0) {
-    const long long slots = tc ? 148 * (hd == 256 ? 1 : 2) : p.rows == 64 ? 148 : wave, u = units(p.rows);
+    const long long slots = tc ? 148 * (p.rows == 64 && hd < 256 ? 2 : 1) : p.rows == 64 ? 148 : wave, u = units(p.rows);
     long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 : slots >= 4 * u) ? 1 : 0);
     if (!tc && u > 74 && max_kv <= 512) n = 1;
     const long long lo = tc ? 512 : max_kv <= 16 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
@@ -688,7 +694,7 @@ extern "C" size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M
                                                    int max_kv, int form, int key_chunk) {
   if (!cache || M <= 0 || Hq <= 0 || max_kv <= 0 || key_chunk < 0 || key_chunk % Q8_CHUNK_UNIT ||
       cache->n_kv_heads <= 0 || Hq % cache->n_kv_heads || Hq / cache->n_kv_heads > 16 || form < DFL_Q8_AUTO ||
-      form > DFL_Q8_TC)
+      form > DFL_Q8_WIDE)
     return 0;
   const int rr = q8_run_rows(M, seq_rows, one_seq != 0);
   return q8_workspace(M, Hq, cache->head_dim,
@@ -714,7 +720,7 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
     set_error("%s: query heads per kv head must be 1..16 (got %d)", who, G);
     return DFL_ERR_UNSUPPORTED;
   }
-  if (form < DFL_Q8_AUTO || form > DFL_Q8_TC) {
+  if (form < DFL_Q8_AUTO || form > DFL_Q8_WIDE) {
     set_error("%s: unknown form %d", who, form);
     return DFL_ERR_INVALID;
   }
@@ -746,7 +752,7 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
     set_error("%s: workspace missing, misaligned or too small (%zu < %zu)", who, workspace_bytes, need);
     return DFL_ERR_WORKSPACE;
   }
-  const bool tc = plan.form == DFL_Q8_TC;
+  const bool tc = plan.form >= DFL_Q8_TC;
   const int rows = plan.rows;
   a.run_rows = run_rows;
   a.run_tiles = (run_rows + rows / G - 1) / (rows / G);
@@ -782,7 +788,7 @@ extern "C" int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int
   const bool e4 = cache->type == DFL_KV_E4M3;
   int status;
   if (tc) {
-    status = launch_attention_q8_tc(a, hd, e4, (int)tiles, st);
+    status = launch_attention_q8_tc(a, hd, e4, rows, (int)tiles, st);
   } else if (hd == 64) {
     status = e4 ? launch_attn_q8_rows<64, true>(a, rows, (int)tiles, st) : launch_attn_q8_rows<64, false>(a, rows, (int)tiles, st);
   } else if (hd == 128) {

@@ -122,7 +122,7 @@ __device__ __forceinline__ Q8Tile q8_tile(const AttnQ8Args& a) {
   return t;
 }
 
-// The tcgen05 form (attention_q8_tc.cu): the chunk kernel alone.
-int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int tiles, cudaStream_t st);
+// The tcgen05 forms (attention_q8_tc.cu), tiles of 64 or 128 rows: the chunk kernel alone.
+int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int rows, int tiles, cudaStream_t st);
 
 }  // namespace dfl

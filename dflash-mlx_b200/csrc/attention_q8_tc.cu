@@ -2,19 +2,25 @@
 // softmax weights in TMEM), for long key chunks. Same work split, masks, scales and partial-result
 // format as attn_q8_kernel (attention_q8.cu); same independence of a row from its tile.
 //
-// One CTA per (run tile of up to 64 (token, head) rows, kv head, key chunk). The 128-row MMA tile
-// holds the rows twice: copy 0 (TMEM lanes 0-63) takes keys 0-31 of every 64-key block, copy 1
-// (lanes 64-127) keys 32-63, so that all four softmax warps have work; the copies are merged at the
-// end. Per block:
+// One CTA per (run tile, kv head, key chunk), in two shapes:
+//  * tc: tiles of up to 64 (token, head) rows. The 128-row MMA tile holds them twice: copy 0 (TMEM lanes
+//    0-63) takes keys 0-31 of every 64-key block, copy 1 (lanes 64-127) keys 32-63, so that all four softmax
+//    warps have work; the copies are merged at the end. Two CTAs an SM (one at head_dim 256).
+//  * wide, for prefill: a row once, and two groups of 128 rows and four softmax warps each that share the
+//    converted tiles (256 rows; at head_dim 256, where TMEM holds one group, 128). One CTA an SM. 1024 rows of
+//    32 heads of 128 at 4096 keys: 111 us, 0.54 PFLOP/s (tc: 173 us).
+// Per block and group:
 //   S = Q K^T      M = 128, N = 64, K = hd, both operands fp16 in shared memory
-//   w = e vs       one thread per (row, copy), 32 keys each; fp16, over S's own TMEM columns, the
+//   w = e vs       one thread per (row, copy), 32 (wide: 64) keys each; fp16, over S's own TMEM columns, the
 //                  other copy's keys zero
 //   O += w V       A = w from TMEM, B = V as [key][dim] in shared memory (MN-major), N = hd
-// Warps 0-3 softmax and epilogue, 4-7 convert codes to fp16 tiles, 8 issues the MMAs.
-// The converters load codes straight into registers, one block ahead of the one they convert, with
-// the blocks after it prefetched into L2 by bulk prefetches: raw codes never pass shared memory, whose
-// bandwidth (fp16 tiles written once and read once by the MMA: 8 bytes per code) is what this form
-// is closest to.
+// Four softmax and epilogue warps a group, then four that convert codes to fp16 tiles (two K, two V), the last
+// issues the MMAs. The converters load codes straight into registers, one block ahead of the one they convert.
+// What bounds it is the chain of these roles, not one unit (64 blocks of 16, 512 to 4096 keys: 124 us, 42 % of
+// the copy rate; without the softmax arithmetic 108, without MMAs 113, without the loads 122, issue slots 41 %
+// busy). A block's softmax takes about 1200 clocks, and the issuing thread, at 58 clocks an MMA, 80 a commit and
+// 130 a wait even for a barrier that is complete, nearly as many: it has one wait and two commits a
+// block (with a barrier for each tile: 130 us, wide 129 instead of 111).
 // A row's exponent base M follows its maximum lazily: sums, weights and O are rescaled only when
 // M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to 2^-18 of
 // the largest keep all their bits (those below are rounded to multiples of 2^-28 of it).
@@ -25,24 +31,27 @@
 namespace dfl {
 
 constexpr int QT_KB = 64;       // keys per block
-constexpr int QT_ROWS = 64;     // (token, head) rows per tile
-constexpr int QT_THREADS = 288;
 constexpr int QT_SCALES = 4;    // scale ring: block i's are read until its weights are written
 
-template <int HD>
+template <int HD, int CP, int SG>  // CP copies of the rows in each of SG softmax groups' 128-row MMA tiles
 struct QtLayout {
+  static constexpr int ROWS = 128 / CP * SG;  // (token, head) rows per tile
+  static constexpr int CONV = 4 * SG, ISSUER = CONV + 4;  // first converter warp, the issuing warp
+  static constexpr int THREADS = 32 * (ISSUER + 1);
   static constexpr int UNITS = HD / 64;  // 64-dim (128-byte) units of an fp16 row
   static constexpr int TILE = QT_KB * HD * 2;
   static constexpr int OFF_K = 0;               // 2 stages
-  static constexpr int OFF_V = 2 * TILE;        // 2 stages; the epilogue reuses K and V for O
-  static constexpr int OFF_Q = 4 * TILE;        // [units][128 rows][128 B]
-  static constexpr int OFF_S = OFF_Q + 128 * HD * 2;  // scales [4][2][64], largest V scales [4][2]
-  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of both copies, output weights
-  static constexpr int OFF_BAR = OFF_R + QT_ROWS * 8 + 128 * 8 + QT_ROWS * 16;
-  static constexpr int N_BAR = 2 * 4 + 2 * 3 + QT_SCALES;
+  static constexpr int OFF_V = 2 * TILE;        // 2 stages
+  static constexpr int OFF_Q = 4 * TILE;        // [group][units][128 rows][128 B]; the epilogue reuses K, V and Q for O
+  static constexpr int OFF_S = OFF_Q + SG * 128 * HD * 2;  // scales [4][2][64], largest V scales [4][2]
+  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of all copies, output weights
+  static constexpr int OFF_BAR = OFF_R + ROWS * 8 + SG * 128 * 8 + ROWS * 16;
+  static constexpr int N_BAR = 2 + SG * 2 * 3;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
-  static constexpr uint32_t COLS = HD == 256 ? 512 : 256;  // S / weights 2 x 64, O hd
-  static_assert(4 * TILE >= 128 * HD * 4, "O of both copies fits the K and V stages");
+  static constexpr int GCOLS = 128 + HD;  // a group's columns: S / weights 2 x 64, O hd
+  static constexpr uint32_t COLS = SG * GCOLS > 256 ? 512 : 256;
+  static_assert(SG * GCOLS <= 512, "TMEM columns");
+  static_assert(OFF_S >= SG * 128 * HD * 4, "O of all copies fits the K, V and Q tiles");
 };
 
 __device__ __forceinline__ void tc_mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
@@ -101,30 +110,32 @@ __host__ __device__ constexpr uint32_t qt_idesc(int n, bool mn) {
   return (1u << 4) | (mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-template <int HD, bool E4M3>
-__global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kernel(const __grid_constant__ AttnQ8Args a) {
-  using L = QtLayout<HD>;
+template <int HD, bool E4M3, int CP, int SG>
+__global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || SG > 1 ? 1 : 2)
+    attn_q8_tc_kernel(const __grid_constant__ AttnQ8Args a) {
+  using L = QtLayout<HD, CP, SG>;
+  constexpr int ROWS = L::ROWS, LANE_ROWS = ROWS / 32;
+  constexpr int KT = QT_KB / CP;  // keys of a block that a softmax thread takes
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* s_sc = reinterpret_cast<float*>(smem + L::OFF_S);  // [ring][K, V][64]
   uint32_t* s_vmax = reinterpret_cast<uint32_t*>(s_sc + QT_SCALES * 2 * QT_KB);  // [ring][half], finite scales' bits
   float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_R);
-  int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + QT_ROWS;
-  float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + QT_ROWS * 8);  // [128]
-  float4* s_w = reinterpret_cast<float4*>(s_ml + 128);  // [64]
+  int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + ROWS;
+  float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + ROWS * 8);  // [128 SG]
+  float4* s_w = reinterpret_cast<float4*>(s_ml + SG * 128);  // [rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* k_full = bars;        // [2] 64 converter arrivals
-  uint64_t* k_empty = bars + 2;   // [2] MMA commit
-  uint64_t* v_full = bars + 4;    // [2] 64 converter arrivals
-  uint64_t* v_empty = bars + 6;   // [2] MMA commit
-  uint64_t* s_full = bars + 8;    // [2] MMA commit
-  uint64_t* p_full = bars + 10;   // [2] 128 softmax arrivals: weights written (and S consumed)
-  uint64_t* pv_done = bars + 12;  // [2] MMA commit: O holds the block
-  uint64_t* sc_full = bars + 14;  // [QT_SCALES] 128 converter arrivals
+  // k_full: K of the first two blocks. s_full and pv_done (MMA commits) also give their block's K and V tiles
+  // back to the converters. p_full: a block's weights written (and its scores consumed), and, for group 0, its V
+  // and the K of two blocks on converted: the one barrier that the issuer waits for per block and group.
+  uint64_t* k_full = bars;             // [2]
+  uint64_t* s_full = bars + 2;         // [SG][2]
+  uint64_t* p_full = s_full + SG * 2;  // [SG][2]
+  uint64_t* pv_done = p_full + SG * 2; // [SG][2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::N_BAR);
-  __shared__ int s_tok_lim[QT_ROWS], s_tok_ok[QT_ROWS];
-  __shared__ int s_row[QT_ROWS];  // token * 16 + head in group of each tile row, -1 behind the last
+  __shared__ int s_tok_lim[ROWS], s_tok_ok[ROWS];
+  __shared__ int s_row[ROWS];  // token * 16 + head in group of each tile row, -1 behind the last
 
   grid_dependency_wait();
   const Q8Tile at = q8_tile(a);
@@ -133,25 +144,31 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   const int m0 = run * a.run_rows + tile * a.tile_toks;
   const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
   if (ntok <= 0) return;
-  // the tile's rows, two a lane, by every warp alike: their positions and sequences, the run's sequence
-  // (that of the first row with a position), limits
-  int pos2[2], sq2[2];
+  // the tile's rows, two or four a lane, by every warp alike: their positions and sequences, the run's
+  // sequence (that of the first row with a position), limits
+  int pos2[LANE_ROWS], sq2[LANE_ROWS], seq = 0;
+  bool any = false;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < LANE_ROWS; ++k) {
     const int i = lane + 32 * k;
     pos2[k] = i < ntok ? a.pos[m0 + i] : -1;
     sq2[k] = i < ntok && a.row_seq ? a.row_seq[m0 + i] : 0;
   }
-  const unsigned v0 = __ballot_sync(0xffffffffu, pos2[0] >= 0), v1 = __ballot_sync(0xffffffffu, pos2[1] >= 0);
-  if (!(v0 | v1)) return;
-  const int seq = __shfl_sync(0xffffffffu, v0 ? sq2[0] : sq2[1], __ffs(v0 ? v0 : v1) - 1);
+#pragma unroll
+  for (int k = LANE_ROWS - 1; k >= 0; --k) {
+    const unsigned v = __ballot_sync(0xffffffffu, pos2[k] >= 0);
+    const int s = __shfl_sync(0xffffffffu, sq2[k], v ? __ffs(v) - 1 : 0);
+    if (v) seq = s;
+    any = any || v;
+  }
+  if (!any) return;
   if (seq < 0 || seq >= a.c.n_seqs) {  // a row that names no sequence of the cache is left as it is
     if (threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
     return;
   }
   int lim_max = 0, lim_min = 0x7fffffff;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < LANE_ROWS; ++k) {
     const int i = lane + 32 * k;
     const bool ok = pos2[k] >= 0 && sq2[k] == seq;
     if (warp == 0 && pos2[k] >= 0 && !ok) q8_error(a.err, Q8_ERR_SEQ);
@@ -169,37 +186,36 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   if (k_begin >= lim_max && a.n_chunks > 1) return;
   const int k_end = min(k_begin + a.key_chunk, lim_max);
   const int n_blocks = (max(k_end - k_begin, 0) + QT_KB - 1) / QT_KB;
-  if (threadIdx.x == 256) {
+  const int n_rows = ntok * a.G, groups = SG == 1 || n_rows <= 128 ? 1 : SG;
+  if (threadIdx.x == 32 * L::ISSUER) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 64);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 64);
-      mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], ntok * a.G > 32 ? 128 : 64);
-      mbar_init(&pv_done[s], 1);
+      for (int g = 0; g < groups; ++g) {
+        mbar_init(&s_full[2 * g + s], 1);
+        mbar_init(&p_full[2 * g + s], CP * ((min(n_rows - g * 128, 128) + 31) / 32) * 32 + (g == 0 ? 128 : 0));
+        mbar_init(&pv_done[2 * g + s], 1);
+      }
     }
-    for (int s = 0; s < QT_SCALES; ++s) mbar_init(&sc_full[s], 128);
     fence_barrier_init();
   }
-  if (threadIdx.x >= 128 && threadIdx.x < 128 + QT_ROWS) {
-    const int r = threadIdx.x - 128, tok = r / a.G;
+  for (int r = threadIdx.x; r < ROWS; r += L::THREADS) {
+    const int tok = r / a.G;
     s_row[r] = tok < ntok ? tok * 16 + r - tok * a.G : -1;
   }
   __syncthreads();
   const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-  if (warp >= 4 && warp < 8) {
-    // ---------------- converters: warps 4-5 K, 6-7 V ----------------
+  if (warp >= L::CONV && warp < L::ISSUER) {
+    // ---------------- converters: two warps K, two V ----------------
     constexpr int NC = HD / 16;            // 16-code chunks per key
     constexpr int PER = QT_KB * NC / 64;   // chunks per thread and block
     const int ct = threadIdx.x & 63;
-    const bool is_v = warp >= 6;
+    const bool is_v = warp >= L::CONV + 2;
     const unsigned char* src = (is_v ? a.c.v : a.c.k) + kvh * a.c.head_stride;
-    const float* ssrc = (is_v ? a.c.vs : a.c.ks) + kvh * a.c.s_head_stride + ct;
+    const float* ks_src = a.c.ks + kvh * a.c.s_head_stride + ct;
+    const float* vs_src = a.c.vs + kvh * a.c.s_head_stride + ct;
     unsigned char* dst = smem + (is_v ? L::OFF_V : L::OFF_K);
-    float* sdst = s_sc + (is_v ? QT_KB : 0) + ct;
-    uint64_t* full = is_v ? v_full : k_full;
-    uint64_t* empty = is_v ? v_empty : k_empty;
+    float* sdst = s_sc + ct;
+    uint64_t* empty = (is_v ? pv_done : s_full) + 2 * (groups - 1);
     // A thread's chunk column c and rows r, r + STEP, ... Lane bits: two of the chunk, one of the row,
     // the rest of the chunk, the rest of the row: the eight lanes of a 16-byte store phase write two
     // rows' chunks of one unit, eight different bank groups. STEP is a multiple of 4; for head_dim 256
@@ -218,7 +234,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       int row = 0;
       win = i;
       win_off = -1;
-      if (i + lane < n_blocks && q8_place(a.c, seq, k_begin + (i + lane) * QT_KB, warp == 4 ? a.err : nullptr, page, row)) {
+      if (i + lane < n_blocks && q8_place(a.c, seq, k_begin + (i + lane) * QT_KB, warp == L::CONV ? a.err : nullptr, page, row)) {
         win_off = page * a.c.seq_stride + (long long)row * HD;
         win_soff = page * a.c.s_seq_stride + row;
       }
@@ -255,19 +271,26 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     window(0);
     int n = where(0, off, soff);
     fetch(src + off, n);
-    float scale = ct < n ? __ldg(ssrc + soff) : 0.f;
-    for (int i = 0; i < n_blocks; ++i) {
+    // both scales of a key come through the K warps: they are there when the block's scores are
+    float ks = !is_v && ct < n ? __ldg(ks_src + soff) : 0.f, vs = !is_v && ct < n ? __ldg(vs_src + soff) : 0.f;
+    const int n_turns = n_blocks + (is_v || n_blocks == 0 ? 0 : 2);  // K is two blocks ahead of the barrier it arrives on
+    for (int i = 0; i < n_turns; ++i) {
       const int s = i & 1;
       if (i + 1 - win >= 32) window(i + 1);
       n = where(i + 1, off, soff);
       if (!qt_wait(&empty[s], ((i >> 1) & 1) ^ 1, 350, a.err)) break;
-      sdst[(i & (QT_SCALES - 1)) * 2 * QT_KB] = scale;
-      if (is_v) {  // a warp holds the 32 keys of one copy
-        const uint32_t v = __float_as_uint(scale) & 0x7fffffffu;
+      if (i >= n_blocks) {
+        mbar_arrive(i < 2 ? &k_full[s] : &p_full[s]);
+        continue;
+      }
+      if (!is_v) {
+        float* sd = sdst + (i & (QT_SCALES - 1)) * 2 * QT_KB;
+        sd[0] = ks;
+        sd[QT_KB] = vs;
+        const uint32_t v = __float_as_uint(vs) & 0x7fffffffu;  // a warp holds 32 keys
         const uint32_t vm = __reduce_max_sync(0xffffffffu, v < 0x7f800000u ? v : 0u);
         if (lane == 0) s_vmax[(i & (QT_SCALES - 1)) * 2 + (ct >> 5)] = vm;
       }
-      mbar_arrive(&sc_full[i & (QT_SCALES - 1)]);
       unsigned char* d = dst + s * L::TILE + dst0;
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
@@ -283,78 +306,85 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(du) ^ 16) = h1;
       }
       fetch(src + off, n);
-      scale = ct < n ? __ldg(ssrc + soff) : 0.f;
+      if (!is_v) {
+        ks = ct < n ? __ldg(ks_src + soff) : 0.f;
+        vs = ct < n ? __ldg(vs_src + soff) : 0.f;
+      }
       fence_proxy_async_smem();
-      mbar_arrive(&full[s]);
+      mbar_arrive(!is_v && i < 2 ? &k_full[s] : &p_full[s]);
     }
-  } else if (warp == 8) {
+  } else if (warp == L::ISSUER) {
     // ---------------- MMA issuer ----------------
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_slot)),
                  "n"(L::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     tc_fence_before();
-    asm volatile("bar.sync 2, 160;\n" ::: "memory");  // Q written, TMEM allocated
+    asm volatile("bar.sync 2, %0;\n" ::"n"(SG * 128 + 32) : "memory");  // Q written, TMEM allocated
     tc_fence_after();
     grid_dependency_launch_dependents();  // not before the allocation: a dependent's must not come first
-    const uint32_t tmem = *tmem_slot, t_o = tmem + 128;  // S / weights: columns 0-63, 64-127
+    const uint32_t tmem = *tmem_slot;  // a group's S / weights: columns 0-63, 64-127, O from 128 on
     // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
     const bool leader = lane == 0;
     const uint64_t qd = sw128_desc(smem_u32(smem + L::OFF_Q));
     const uint64_t kd0 = sw128_desc(smem_u32(smem + L::OFF_K));
     const uint64_t vd0 = sw128_mn_desc(smem_u32(smem + L::OFF_V), QT_KB * 128, 1024);
-    auto pv = [&](int j) -> bool {
-      const int s = j & 1;
-      if (!qt_wait(&p_full[s], (j >> 1) & 1, 352, a.err)) return false;
-      if (!qt_wait(&v_full[s], (j >> 1) & 1, 353, a.err)) return false;
-      tc_fence_after();
-      if (leader) {
-        const uint64_t vd = vd0 + s * (L::TILE >> 4);
-        const uint32_t tw = tmem + s * 64;
+    auto qk = [&](int i, int g) {
+      const int s = i & 1;
+      const uint32_t ts = tmem + g * L::GCOLS + s * 64;
+      const uint64_t qg = qd + g * (128 * HD * 2 >> 4), kd = kd0 + s * (L::TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < QT_KB / 16; ++kk)
-          tc_mma_ts(t_o, tw + kk * 8, vd + kk * (2048 >> 4), qt_idesc(HD, true), j > 0 || kk > 0 ? 1u : 0u);
-        tc_commit(&v_empty[s]);
-        tc_commit(&pv_done[s]);
-      }
-      __syncwarp();
-      return true;
+      for (int kk = 0; kk < HD / 16; ++kk)
+        tc_mma(ts, qg + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (QT_KB * 128 >> 4) + 2 * (kk & 3),
+               qt_idesc(QT_KB, false), kk > 0 ? 1u : 0u);
+      tc_commit(&s_full[2 * g + s]);
+    };
+    auto pv = [&](int j, int g) {
+      const int s = j & 1;
+      const uint64_t vd = vd0 + s * (L::TILE >> 4);
+      const uint32_t tw = tmem + g * L::GCOLS + s * 64, t_o = tmem + g * L::GCOLS + 128;
+#pragma unroll
+      for (int kk = 0; kk < QT_KB / 16; ++kk)
+        tc_mma_ts(t_o, tw + kk * 8, vd + kk * (2048 >> 4), qt_idesc(HD, true), j > 0 || kk > 0 ? 1u : 0u);
+      tc_commit(&pv_done[2 * g + s]);
     };
     bool ok = true;
-    for (int i = 0; i < n_blocks && ok; ++i) {
-      const int s = i & 1;
-      if (!qt_wait(&k_full[s], (i >> 1) & 1, 354, a.err)) {
-        ok = false;
-        break;
-      }
+    for (int i = 0; i < min(n_blocks, 2) && ok; ++i) {
+      ok = qt_wait(&k_full[i], 0, 354, a.err);
+      if (!ok) break;
       tc_fence_after();
-      if (leader) {
-        // S of block i overwrites the weights of block i - 2, whose product was issued before it
-        const uint64_t kd = kd0 + s * (L::TILE >> 4);
-        const uint32_t ts = tmem + s * 64;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          tc_mma(ts, qd + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3), kd + (kk >> 2) * (QT_KB * 128 >> 4) + 2 * (kk & 3),
-                 qt_idesc(QT_KB, false), kk > 0 ? 1u : 0u);
-        tc_commit(&k_empty[s]);
-        tc_commit(&s_full[s]);
-      }
+      if (leader)
+        for (int g = 0; g < groups; ++g) qk(i, g);
       __syncwarp();
-      if (i > 0) ok = pv(i - 1);
     }
-    if (ok && n_blocks > 0) pv(n_blocks - 1);
-  } else if (warp < 4) {
-    // ---------------- softmax: thread = (row, copy) ----------------
-    // Q rows to scaled fp16, twice; a row's factor undoes its power of two. The raw rows all come at once
-    // into the second copy's place, where each thread then converts what it copied: hd / 16 lanes a row,
+    // Behind a block's barrier nothing stands between its product and the scores of two blocks on, which overwrite
+    // its weights (the tensor core takes them in order).
+    for (int j = 0; j < n_blocks && ok; ++j) {
+      const int s = j & 1, ph = (j >> 1) & 1;
+      for (int g = 0; g < groups && ok; ++g) {
+        ok = qt_wait(&p_full[2 * g + s], ph, 352, a.err);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          pv(j, g);
+          if (j + 2 < n_blocks) qk(j + 2, g);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ---------------- softmax: thread = (row, copy), four warps a group ----------------
+    // Q rows to scaled fp16, CP times; a row's factor undoes its power of two. The raw rows all come at once
+    // into the last copy's place, where each thread then converts what it copied: hd / 16 lanes a row,
     // 32 bytes each, in rolled loops (code that runs once a CTA comes from a cold instruction cache).
     {
       constexpr int LPR = HD / 16, RPW = 32 / LPR;
-      const int ql = lane % LPR, qr = warp * RPW + lane / LPR;
-      unsigned char* q1 = smem + L::OFF_Q + (ql >> 2) * 16384 + QT_ROWS * 128;
+      constexpr int GR = 128 / CP;  // a group's rows
+      const int ql = lane % LPR, qr = (warp & 3) * RPW + lane / LPR, g0 = (warp >> 2) * GR;
+      unsigned char* q1 = smem + L::OFF_Q + (warp >> 2) * 128 * HD * 2 + (ql >> 2) * 16384 + (CP - 1) * GR * 128;
 #pragma unroll 1
-      for (int r = qr; r < QT_ROWS; r += 4 * RPW) {
-        const int th = s_row[r];
+      for (int r = qr; r < GR; r += 4 * RPW) {
+        const int th = s_row[g0 + r];
         const bool ok = th >= 0 && s_tok_lim[th >> 4] > 0;
         const __nv_bfloat16* q =
             ok ? a.q + ((long long)(m0 + (th >> 4)) * a.Hq + kvh * a.G + (th & 15)) * HD + ql * 16 : a.q;
@@ -365,7 +395,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       cp_async_commit();
       cp_async_wait<0>();
 #pragma unroll 1
-      for (int r = qr; r < QT_ROWS; r += 4 * RPW) {
+      for (int r = qr; r < GR; r += 4 * RPW) {
         uint4* d0 = reinterpret_cast<uint4*>(q1 + qt_sw(r, (ql & 3) * 2));
         uint4* d1 = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d0) ^ 16);
         const uint4 n0 = *d0, n1 = *d1;
@@ -388,20 +418,25 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
         *d0 = h0;
         *d1 = h1;
-        *(d0 - QT_ROWS * 8) = h0;  // the first copy, 64 rows of 128 bytes before
-        *(d1 - QT_ROWS * 8) = h1;
+        if (CP == 2) {
+          *(d0 - GR * 8) = h0;  // the first copy, 64 rows of 128 bytes before
+          *(d1 - GR * 8) = h1;
+        }
         if (ql == 0) {
-          s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
-          s_lim[r] = s_row[r] < 0 ? 0 : s_tok_lim[s_row[r] >> 4];
+          s_rowf[g0 + r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
+          s_lim[g0 + r] = s_row[g0 + r] < 0 ? 0 : s_tok_lim[s_row[g0 + r] >> 4];
         }
       }
     }
     fence_proxy_async_smem();
     tc_fence_before();
-    asm volatile("bar.sync 2, 160;\n" ::: "memory");
+    asm volatile("bar.sync 2, %0;\n" ::"n"(SG * 128 + 32) : "memory");
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot, t_o = tmem + 128;
-    const int row = threadIdx.x & 63, half = threadIdx.x >> 6;
+    const int grp = SG == 1 ? 0 : warp >> 2;
+    s_full += 2 * grp;
+    p_full += 2 * grp;
+    const uint32_t tmem = *tmem_slot + grp * L::GCOLS, t_o = tmem + 128;
+    const int row = threadIdx.x & (ROWS - 1), half = CP == 2 ? threadIdx.x >> 6 : 0;
     const int lim = s_lim[row];
     const float rowf = s_rowf[row];
     float m = -INFINITY, mu_used = -INFINITY;
@@ -410,33 +445,36 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
     bool ok = true;
     // a warp whose 32 rows all lie behind the tile's does nothing: what its lanes hold goes to its own
     // rows of O, which nobody reads
-    const int my_blocks = (row & 32) < ntok * a.G ? n_blocks : 0;
+    const int my_blocks = (row & ~31) < n_rows ? n_blocks : 0;
     for (int i = 0; i < my_blocks && ok; ++i) {
       const int s = i & 1;
       const float* sc = s_sc + (i & (QT_SCALES - 1)) * 2 * QT_KB + half * 32;
       const int kb = k_begin + i * QT_KB + half * 32;
-      ok = qt_wait(&sc_full[i & (QT_SCALES - 1)], (i / QT_SCALES) & 1, 355, a.err) &&
-           qt_wait(&s_full[s], (i >> 1) & 1, 356, a.err);
+      ok = qt_wait(&s_full[s], (i >> 1) & 1, 356, a.err);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float sv[32];
-      tc_ld32(tmem + lane_base + (uint32_t)(s * 64 + half * 32), sv);
-      const bool full = kb + 32 <= lim_min;
-      uint64_t x[16];
+      const bool full = kb + KT <= lim_min;
+      uint64_t x[KT / 2];
 #pragma unroll
-      for (int c = 0; c < 16; c += 2) {
-        const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + 2 * c);
-        x[c] = q8_mul2(q8_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
-        x[c + 1] = q8_mul2(q8_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
+      for (int k = 0; k < KT; k += 32) {
+        float sv[32];
+        tc_ld32(tmem + lane_base + (uint32_t)(s * 64 + half * 32 + k), sv);
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + k + 2 * c);
+          x[k / 2 + c] = q8_mul2(q8_pack(sv[2 * c], sv[2 * c + 1]), ks.x);
+          x[k / 2 + c + 1] = q8_mul2(q8_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
+        }
       }
       uint32_t vm = s_vmax[(i & (QT_SCALES - 1)) * 2 + half];
+      if (CP == 1) vm = max(vm, s_vmax[(i & (QT_SCALES - 1)) * 2 + 1]);
       if (!full) {
         vm = 0;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
+        for (int c = 0; c < KT / 2; ++c) {
           const float2 y = q8_unpack(x[c]);
           const bool seen0 = kb + 2 * c < lim, seen1 = kb + 2 * c + 1 < lim;
           x[c] = q8_pack(seen0 ? y.x : -INFINITY, seen1 ? y.y : -INFINITY);
@@ -448,7 +486,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       }
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 16; c += 2) {
+      for (int c = 0; c < KT / 2; c += 2) {
         const float2 y = q8_unpack(x[c]), z = q8_unpack(x[c + 1]);
         mx0 = fmaxf(fmaxf(mx0, y.x), y.y);
         mx1 = fmaxf(fmaxf(mx1, z.x), z.y);
@@ -462,7 +500,7 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
         if (grow) mu_used = M;
         l = q8_mul2(l, q8_pack(fac, fac));
         if (i > 0) {
-          ok = qt_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 357, a.err);
+          ok = qt_wait(&pv_done[2 * grp + ((i - 1) & 1)], ((i - 1) >> 1) & 1, 357, a.err);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -480,37 +518,44 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       }
       const float mu = mu_used == -INFINITY ? 0.f : mu_used;
       const uint64_t rf2 = q8_pack(rowf, rowf), mu2 = q8_pack(-mu, -mu), unit2 = q8_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
-      uint32_t w[16];
-#pragma unroll
-      for (int c = 0; c < 16; c += 2) {
-        const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + QT_KB + 2 * c);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          const float2 y = q8_unpack(q8_fma2(x[c + d], rf2, mu2));
-          const uint64_t e = q8_pack(q8_exp2(y.x), q8_exp2(y.y));
-          l = q8_fma2(e, unit2, l);
-          const float2 ww = q8_unpack(q8_mul2(e, d ? vs.y : vs.x));
-          const __half2 h = __floats2half2_rn(ww.x, ww.y);
-          w[c + d] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      }
-      if (!full) {  // 0 * scale of a key that is not seen may be NaN
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          w[c] &= (kb + 2 * c < lim ? 0xffffu : 0u) | (kb + 2 * c + 1 < lim ? 0xffff0000u : 0u);
-      }
       const uint32_t t_w = tmem + lane_base + (uint32_t)(s * 64);
-      tc_st16_nowait(t_w + half * 16, w);
 #pragma unroll
-      for (int c = 0; c < 16; ++c) w[c] = 0;
-      tc_st16_nowait(t_w + (half ^ 1) * 16, w);
+      for (int k = 0; k < KT; k += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+          const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + QT_KB + k + 2 * c);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const float2 y = q8_unpack(q8_fma2(x[k / 2 + c + d], rf2, mu2));
+            const uint64_t e = q8_pack(q8_exp2(y.x), q8_exp2(y.y));
+            l = q8_fma2(e, unit2, l);
+            const float2 ww = q8_unpack(q8_mul2(e, d ? vs.y : vs.x));
+            const __half2 h = __floats2half2_rn(ww.x, ww.y);
+            w[c + d] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        if (!full) {  // 0 * scale of a key that is not seen may be NaN
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            w[c] &= (kb + k + 2 * c < lim ? 0xffffu : 0u) | (kb + k + 2 * c + 1 < lim ? 0xffff0000u : 0u);
+        }
+        tc_st16_nowait(t_w + half * 16 + k / 2, w);
+      }
+      if (CP == 2) {
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) w[c] = 0;
+        tc_st16_nowait(t_w + (half ^ 1) * 16, w);
+      }
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[s]);
     }
     // ---- O of both copies through shared memory, then merged, row by row ----
     const int nb1 = n_blocks - 1;
-    if (ok && n_blocks > 0) ok = qt_wait(&pv_done[nb1 & 1], (nb1 >> 1) & 1, 358, a.err);
+    for (int g = 0; g < groups && n_blocks > 0; ++g)  // every group's: O goes where all read K, V and Q
+      if (ok) ok = qt_wait(&pv_done[2 * g + (nb1 & 1)], (nb1 >> 1) & 1, 358, a.err);
     ok = __all_sync(0xffffffffu, ok);
     constexpr int CH = HD / 4;  // float4 chunks per row
     float4* s_o = reinterpret_cast<float4*>(smem);
@@ -528,12 +573,12 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       tc_fence_before();
     }
     s_ml[threadIdx.x] = make_float2(mu_used, q8_unpack(l).x + q8_unpack(l).y);
-    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    asm volatile("bar.sync 1, %0;\n" ::"n"(SG * 128) : "memory");
     // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and the row
     // of the output (or of the partials) it goes to, -1 for none
-    if (threadIdx.x < QT_ROWS) {
+    if (threadIdx.x < ROWS) {
       const int r = threadIdx.x, th = s_row[r], tok = th >> 4;
-      const float2 x0 = s_ml[r], x1 = s_ml[r + QT_ROWS];
+      const float2 x0 = s_ml[r], x1 = CP == 2 ? s_ml[r + ROWS] : make_float2(-INFINITY, 0.f);
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
       float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
       const float den = w0 * x0.y + w1 * x1.y;
@@ -550,10 +595,10 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       }
       s_w[r] = make_float4(w0, w1, __int_as_float(to), lim > 0 ? 1.f : 0.f);
     }
-    asm volatile("bar.sync 1, 128;\n" ::: "memory");
+    asm volatile("bar.sync 1, %0;\n" ::"n"(SG * 128) : "memory");
     constexpr int RPW = CH >= 32 ? 1 : 32 / CH;  // rows a warp writes at a time
 #pragma unroll 4
-    for (int r0 = warp * RPW; r0 < ntok * a.G; r0 += 4 * RPW) {
+    for (int r0 = warp * RPW; r0 < n_rows; r0 += 4 * SG * RPW) {
       const int r = r0 + lane / (32 / RPW);
       const float4 w = s_w[r];
       const int to = __float_as_int(w.z);
@@ -562,9 +607,13 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
       for (int c = lane % (32 / RPW); c < CH; c += 32) {
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (w.w != 0.f) {
-          const float4 o0 = s_o[r * CH + (c ^ (r & 7))], o1 = s_o[(r + QT_ROWS) * CH + (c ^ (r & 7))];
-          y = make_float4(w.x * o0.x + w.y * o1.x, w.x * o0.y + w.y * o1.y, w.x * o0.z + w.y * o1.z,
-                          w.x * o0.w + w.y * o1.w);
+          const float4 o0 = s_o[r * CH + (c ^ (r & 7))];
+          y = make_float4(w.x * o0.x, w.x * o0.y, w.x * o0.z, w.x * o0.w);
+          if (CP == 2) {
+            const float4 o1 = s_o[(r + ROWS) * CH + (c ^ (r & 7))];
+            y = make_float4(w.x * o0.x + w.y * o1.x, w.x * o0.y + w.y * o1.y, w.x * o0.z + w.y * o1.z,
+                            w.x * o0.w + w.y * o1.w);
+          }
         }
         if (a.n_chunks > 1) {
           *reinterpret_cast<float4*>(a.part_o + ((long long)chunk * a.M * a.Hq + to) * HD + c * 4) = y;
@@ -584,20 +633,20 @@ __global__ void __launch_bounds__(QT_THREADS, HD == 256 ? 1 : 2) attn_q8_tc_kern
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == L::ISSUER) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(*tmem_slot), "n"(L::COLS));
   }
 }
 
-template <int HD, bool E4M3>
+template <int HD, bool E4M3, int CP, int SG>
 static int launch_qt(const AttnQ8Args& a, int tiles, cudaStream_t st) {
-  using L = QtLayout<HD>;
+  using L = QtLayout<HD, CP, SG>;
   static bool opted[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !opted[dev]) {
-    if (cudaFuncSetAttribute(attn_q8_tc_kernel<HD, E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) !=
+    if (cudaFuncSetAttribute(attn_q8_tc_kernel<HD, E4M3, CP, SG>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) !=
         cudaSuccess) {
       cudaGetLastError();
       set_error("dfl_attention_q8: cannot opt in to %d bytes of shared memory", L::SMEM);
@@ -610,12 +659,12 @@ static int launch_qt(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * a.c.Hkv, a.n_chunks);
-  cfg.blockDim = dim3(QT_THREADS);
+  cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_tc_kernel<HD, E4M3>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_q8_tc_kernel<HD, E4M3, CP, SG>, a);
   if (e != cudaSuccess) {
     set_error("dfl_attention_q8: launch failed: %s", cudaGetErrorString(e));
     return DFL_ERR_CUDA;
@@ -623,11 +672,16 @@ static int launch_qt(const AttnQ8Args& a, int tiles, cudaStream_t st) {
   return DFL_OK;
 }
 
-int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int tiles, cudaStream_t st) {
+template <int HD, bool E4M3>
+static int launch_qt_rows(const AttnQ8Args& a, int rows, int tiles, cudaStream_t st) {
+  return rows == 64 ? launch_qt<HD, E4M3, 2, 1>(a, tiles, st) : launch_qt<HD, E4M3, 1, HD == 256 ? 1 : 2>(a, tiles, st);
+}
+
+int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int rows, int tiles, cudaStream_t st) {
   switch (hd) {
-    case 64: return e4m3 ? launch_qt<64, true>(a, tiles, st) : launch_qt<64, false>(a, tiles, st);
-    case 128: return e4m3 ? launch_qt<128, true>(a, tiles, st) : launch_qt<128, false>(a, tiles, st);
-    default: return e4m3 ? launch_qt<256, true>(a, tiles, st) : launch_qt<256, false>(a, tiles, st);
+    case 64: return e4m3 ? launch_qt_rows<64, true>(a, rows, tiles, st) : launch_qt_rows<64, false>(a, rows, tiles, st);
+    case 128: return e4m3 ? launch_qt_rows<128, true>(a, rows, tiles, st) : launch_qt_rows<128, false>(a, rows, tiles, st);
+    default: return e4m3 ? launch_qt_rows<256, true>(a, rows, tiles, st) : launch_qt_rows<256, false>(a, rows, tiles, st);
   }
 }
 

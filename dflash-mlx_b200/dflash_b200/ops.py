@@ -459,7 +459,7 @@ class KvQ8(ctypes.Structure):
 
 
 Q8_CHUNK = 128  # the unit of attention_q8's key_chunk
-Q8_FORMS = {"auto": 0, "warp": 1, "tc": 2}  # DFL_Q8_AUTO, DFL_Q8_WARP, DFL_Q8_TC
+Q8_FORMS = {"auto": 0, "warp": 1, "tc": 2, "wide": 3}  # DFL_Q8_AUTO, DFL_Q8_WARP, DFL_Q8_TC, DFL_Q8_WIDE
 KV_Q8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # DFL_KV_INT8, DFL_KV_E4M3
 
 
@@ -587,8 +587,8 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
                  key_chunk: int = 0, form: str = "auto") -> torch.Tensor:
     """attention() over an 8-bit cache (dfl_attention_q8): q [M, Hq, hd] bf16 against ``kv``;
     returns [M, Hq*hd] bf16. seq_rows: rows per sequence when row_seq groups contiguous runs (0 =
-    any layout). ``form``: "warp" (mma.sync, few rows), "tc" (tcgen05, verify blocks and prefill) or
-    "auto"; key_chunk: keys per split, a multiple of 128, 0 = chosen by the call's sizes. A row's
+    any layout). ``form``: "warp" (mma.sync, few rows), "tc" (tcgen05, verify blocks of many sequences), "wide"
+    (tcgen05, prefill) or "auto"; key_chunk: keys per split, a multiple of 128, 0 = chosen by the call's sizes. A row's
     result depends on these two and its own query and keys only. Rows with pos < 0 are left as they are; rows that see no key are zero.
     ``ws``: partial results live in its attention scratch (one workspace per stream and captured
     graph, as for attention()); without it each call allocates its own."""

@@ -126,7 +126,7 @@ class SpecSession:
         if kv_dtype != "bf16":
             form, chunk = q8_split(batch, tc.num_key_value_heads, max_total, tc.head_dim)
             self.step_split = {"form": form, "key_chunk": chunk}
-            self.prefill_split = {"form": "tc", "key_chunk": 1024}
+            self.prefill_split = {"form": "wide", "key_chunk": 2048}
         self.max_steps = max_steps or (max_total + 1)
         # under 16 sequences, weights with few 128-row tiles also split K (fixed ranges)
         self.ws = ops.Workspace(self.dev, wide=self.batched, wide_split=4 if batch < 16 else 1)

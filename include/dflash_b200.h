@@ -341,6 +341,7 @@ int dfl_attention_qkv(const void* qkv, int64_t ldqkv, const void* q_norm, const 
 #define DFL_Q8_AUTO 0
 #define DFL_Q8_WARP 1
 #define DFL_Q8_TC 2
+#define DFL_Q8_WIDE 3
 typedef struct dfl_kv_q8 {
   void* k;               /* codes */
   void* v;
@@ -375,7 +376,8 @@ int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* ro
  * kv head. Rows of one sequence share a tile: with row_seq, every run of seq_rows rows starting
  * at a multiple of seq_rows belongs to one sequence (0 = any layout: each row is its own run);
  * without it all rows are sequence 0's. form: DFL_Q8_WARP (mma.sync, keys split over a CTA's
- * warps: few rows) or DFL_Q8_TC (tcgen05, 64 rows a CTA: verify blocks and prefill); key_chunk:
+ * warps: few rows), DFL_Q8_TC (tcgen05, 64 rows a CTA: verify blocks of many sequences) or
+ * DFL_Q8_WIDE (tcgen05, 256 rows a CTA, 128 at head_dim 256: prefill); key_chunk:
  * keys per split, a multiple of 128. A row's result depends on these two and on nothing else
  * of the call but the row's own query and keys, so calls to be compared bit for bit name
  * both; DFL_Q8_AUTO and key_chunk 0 choose by the call's sizes. A row with pos >= 0 that sees no key

@@ -64,7 +64,7 @@ def test_bad_caches_are_refused_by_every_entry_point(lib, bad, status):
     (_attn(_desc(), scale=float("nan")), 1), (_attn(_desc(), scale=float("inf")), 1), (_attn(_desc(), ldo=510), 2),
     (_attn(_desc(), ldo=256), 2), (_attn(_desc(), out=68), 2), (_attn(_desc(), q=72), 2),
     (_attn(_desc(), chunk=128), 4), (_attn(_desc(), chunk=128, ws=64, ws_bytes=100), 4),
-    (_attn(_desc(), seq_rows=-1), 1), (_attn(_desc(), form=3), 1), (_attn(_desc(), form=-1), 1), (_attn(_desc(cap=1 << 30), max_kv=1 << 30, chunk=128, ws=64, ws_bytes=1 << 62), 2),
+    (_attn(_desc(), seq_rows=-1), 1), (_attn(_desc(), form=4), 1), (_attn(_desc(), form=-1), 1), (_attn(_desc(cap=1 << 30), max_kv=1 << 30, chunk=128, ws=64, ws_bytes=1 << 62), 2),
 ])
 def test_bad_arguments_are_refused_before_any_launch(lib, call, status):
     from dflash_b200 import _lib
@@ -78,12 +78,12 @@ def test_empty_calls_succeed_and_scratch_follows_the_chunks(lib):
     for make in (_append, _attn, _read):
         _lib.call(*make(_desc(), M=0))
     size = lambda *a: _lib.query("dfl_attention_q8_workspace_bytes", _desc(), *a)  # noqa: E731
-    for form in (1, 2):
+    for form in (1, 2, 3):
         assert size(2, 4, 1, 0, 512, form, 512) == 0  # one chunk
         assert size(2, 4, 1, 0, 512, form, 128) == 4 * 2 * 4 * 128 * 4 + 4 * 2 * 4 * 8
         assert size(2, 4, 1, 0, 513, form, 128) > size(2, 4, 1, 0, 512, form, 128)
         assert size(0, 4, 1, 0, 512, form, 128) == 0 and size(2, 4, 1, 0, 512, form, 100) == 0
-    assert size(2, 4, 1, 0, 512, 3, 128) == 0
+    assert size(2, 4, 1, 0, 512, 4, 128) == 0
 
 
 def test_wrappers_take_cuda_tensors_only():

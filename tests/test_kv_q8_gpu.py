@@ -121,6 +121,14 @@ CASES = [
     ("e4m3", [900, 64], 16, 2, 2, 64, 64, False, True, "tc", 512),
     ("int8", [2500], 100, 1, 8, 64, 64, True, False, "tc", 1024),
     ("int8", [1300, 514], 5, 2, 4, 128, 64, True, False, "tc", 1024),
+    # its 128-row tiles
+    ("int8", [1], 1, 1, 1, 128, 64, True, False, "wide", 512),
+    ("e4m3", [700, 33, 511], 32, 2, 4, 128, 64, True, True, "wide", 512),
+    ("int8", [300], 300, 1, 1, 64, 0, True, False, "wide", 512),
+    ("e4m3", [640, 130], 16, 1, 6, 256, 128, True, True, "wide", 512),
+    ("int8", [700, 45], 40, 2, 3, 256, 0, False, False, "wide", 1024),
+    ("e4m3", [900, 64, 65], 21, 2, 2, 64, 64, False, True, "wide", 384),
+    ("int8", [1300, 514], 5, 2, 4, 128, 64, True, False, "wide", 1024),
 ]
 
 
@@ -150,7 +158,7 @@ def test_attention_matches_64_bits(t, lens, rows, Hkv, G, hd, page, causal, gate
 
 
 @pytest.mark.parametrize("t", ["int8", "e4m3"])
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512), ("wide", 128), ("wide", 512)])
 @pytest.mark.parametrize("G,hd", [(1, 128), (4, 128), (2, 64), (3, 256), (6, 128)])
 def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, form, chunk):
     """A verify block's rows equal single-token calls bit for bit, with later rows' keys (masked for
@@ -182,7 +190,7 @@ def test_rows_do_not_depend_on_the_rows_beside_them(t, G, hd, form, chunk):
     assert ops.device_error() == 0
 
 
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512), ("wide", 128), ("wide", 512)])
 def test_rows_without_keys_are_zero_and_empty_calls_do_nothing(form, chunk):
     from dflash_b200 import ops
     c = Cache("int8", [40, 40, 40], 2, 128)
@@ -200,7 +208,7 @@ def test_rows_without_keys_are_zero_and_empty_calls_do_nothing(form, chunk):
     assert ops.device_error() == 0
 
 
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512), ("wide", 128), ("wide", 512)])
 def test_scales_and_queries_of_extreme_size(form, chunk):
     """Values far from 1 keep their relative precision; a softmax scale of 0 averages the values."""
     from dflash_b200 import ops
@@ -316,7 +324,7 @@ def test_rows_that_hold_infinities_or_nans_are_held_as_nan():
         assert v[0, 0].isnan().all() and v[0, 1].isfinite().all() and k.isfinite().all()
 
 
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512), ("wide", 128), ("wide", 512)])
 @pytest.mark.parametrize("page", [0, 64])
 def test_out_of_range_rows_are_refused_on_the_device(page, form, chunk):
     """Positions, sequences and pages out of range are not accessed and set the error word; the other
@@ -352,7 +360,7 @@ def test_out_of_range_rows_are_refused_on_the_device(page, form, chunk):
     assert torch.equal(before, c.codes.view(torch.uint8))
 
 
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 128), ("tc", 512), ("wide", 128), ("wide", 512)])
 def test_views_streams_and_graphs(form, chunk):
     """Strided caches (one layer of a [seq, layer, ...] pool), strided outputs and gates, another
     stream, and two captured graphs replayed out of order."""
@@ -406,7 +414,7 @@ def test_views_streams_and_graphs(form, chunk):
         check()
 
 
-@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 512)])
+@pytest.mark.parametrize("form,chunk", [("warp", 128), ("warp", 512), ("tc", 512), ("wide", 512)])
 @pytest.mark.parametrize("B,rows,Hkv,G,hd,causal", [
     (60, 3, 4, 4, 128, True), (60, 1, 4, 2, 64, False), (45, 16, 4, 3, 256, True), (255, 1, 1, 8, 128, True),
     (256, 2, 1, 8, 128, False), (300, 2, 1, 4, 64, True)])
