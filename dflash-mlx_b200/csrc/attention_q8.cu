@@ -642,8 +642,8 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 
 // The form, tile rows and keys per chunk of a call.
 // Few: runs of at most 16 (token, head) rows, and calls small enough that tiles of 16 rows with 384 keys each
-// fit one wave (three CTAs an SM, one at head_dim 256). They take the warp form in 16-row tiles, for
-// their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128: 10.3 us (64-row tiles 15.2, tcgen05
+// fit one wave (three CTAs an SM; at head_dim 256 one, of 32 rows where there are more than 16). They take the
+// warp form in such tiles, for their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128: 10.3 us (64-row tiles 15.2, tcgen05
 // 16.2), 4096 keys 16.0 (20.5, 16.5). Others take a tcgen05 form, tc of 64 rows a CTA: four such sequences of 2048
 // keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 124 (338 in 64-row tiles); 64 single
 // tokens 107, in the warp form 66. Wide, of 256 rows (head_dim 256: 128), for runs that fill more than half of them
@@ -652,7 +652,8 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for several
 // runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 57 us
 // with it, 72 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
-// keys, 256 where those make more than 16 chunks (one token, 4096 keys: 9.2 us, with 128 11.1), in the tcgen05
+// keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and 8.0,
+// with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05
 // forms 512, and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us,
 // split in two 13.6).
 struct Q8Plan {
@@ -662,19 +663,20 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
   Q8Plan p;
   const long long want = (long long)run_rows * G, wave = 148 * (hd == 256 ? 1 : 3);
   auto units = [&](int rows) { return runs * Hkv * ((run_rows + rows / G - 1) / (rows / G)); };
-  const bool few = want <= 16 || units(16) * max_kv <= wave * 384;
+  const int small = hd == 256 && want > 16 ? 32 : 16;
+  const bool few = want <= 16 || (units(small) <= wave && units(small) * max_kv <= wave * 384);
   const int wide = hd == 256 ? 128 : 256;
   p.form = form != DFL_Q8_AUTO                                              ? form
            : few                                                          ? DFL_Q8_WARP
            : want > wide / 2 && units(wide) * max_kv >= (long long)148 * 384 ? DFL_Q8_WIDE
                                                                           : DFL_Q8_TC;
   const bool tc = p.form >= DFL_Q8_TC;
-  p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? 16 : want <= 32 || hd == 256 ? 32 : 64;
+  p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? small : want <= 32 || hd == 256 ? 32 : 64;
   if (key_chunk <= 0) {
     const long long slots = tc ? 148 * (p.rows == 64 && hd < 256 ? 2 : 1) : p.rows == 64 ? 148 : wave, u = units(p.rows);
     long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 : slots >= 4 * u) ? 1 : 0);
     if (!tc && u > 74 && max_kv <= 512) n = 1;
-    const long long lo = tc ? 512 : max_kv <= 16 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
+    const long long lo = tc ? 512 : max_kv <= 8 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
     long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
     c = c < lo ? lo : c > 8192 ? 8192 : c;
     key_chunk = (int)((c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT);

@@ -1,6 +1,6 @@
 """Per-kernel roofline measurements of the hot-path kernels at the benchmark configurations' shapes.
 
-    python -m dflash_b200.kernel_bench [--only gdr,attn,gemm] [--iters N]
+    python -m dflash_b200.kernel_bench [--only gdr,attn,gemm,kv_q8] [--iters N]
 
 Prints one JSON line per case: the kernel, the workload, the algorithmic bytes
 (or FLOPs) one launch must move, the CUDA-event time per launch (mean over
@@ -21,6 +21,9 @@ Cases (synthetic inputs, shapes and distributions of the benchmark configuration
   attn_c4     batched verify attention, 64 sequences x 16 rows, contexts U[512, 4096]
   gemm_c4     verify GEMMs at 1024 rows (64 sequences x 16): QKV, O, gate/up, down, lm_head
               (wide form; "gemm_streaming" runs the M <= 16 form on the same shapes)
+  kv_q8       the 8-bit K/V cache, int8 and e4m3: attention at attn_c3's and attn_c4's shapes, one token of
+              each of those 64 sequences, and 1024 prompt rows behind 4096 keys; the append of 16 and 16384 rows;
+              the read-back of 64 sequences' last 1024 rows
 """
 from __future__ import annotations
 
@@ -149,6 +152,56 @@ def bench_attention(timer: Timer, B: int, rows: int, ctxs: list[int], case: str,
                         "key_chunk": key_chunk or 128})
 
 
+def bench_attention_q8(timer: Timer, dtype: torch.dtype, rows: int, ctxs: list[int], case: str):
+    """ops.attention_q8 with its own choice of form and split; bytes: codes and scales of every sequence once, q, out."""
+    B, Hq, Hkv, hd = len(ctxs), 32, 8, 128
+    cap = max(ctxs) + rows
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    kv = _quant_cache(dtype, B, Hkv, cap, hd, gen)
+    M = B * rows
+    q = torch.randn((M, Hq, hd), device="cuda", generator=gen).bfloat16()
+    pos = torch.tensor([c + i for c in ctxs for i in range(rows)], dtype=torch.int32, device="cuda")
+    row_seq = (torch.arange(M, dtype=torch.int32, device="cuda") // rows) if B > 1 else None
+    out = torch.empty((M, Hq * hd), dtype=torch.bfloat16, device="cuda")
+    ws = ops.Workspace(torch.device("cuda"))
+    sec = timer(lambda: ops.attention_q8(q, kv, pos, True, cap, row_seq=row_seq, out=out, ws=ws, seq_rows=rows))
+    by = sum(c + rows for c in ctxs) * Hkv * 2 * (hd + 4) + q.numel() * 2 + out.numel() * 2
+    fl = 4 * Hq * hd * sum(c + i + 1 for c in ctxs for i in range(rows))
+    return _line(case, "attn_q8_kernel / attn_q8_tc_kernel + attn_q8_merge_kernel", sec, bytes_=by, flops=fl,
+                 extra={"workload": f"{dtype} B={B} rows={rows} Hq={Hq} Hkv={Hkv} hd={hd} ctx mean "
+                                    f"{sum(ctxs) / len(ctxs):.0f}"})
+
+
+def _quant_cache(dtype, B, Hkv, cap, hd, gen):
+    codes = torch.randint(-127, 128, (2, B, Hkv, cap, hd), device="cuda", generator=gen, dtype=torch.int8)
+    if dtype != torch.int8:
+        codes = (codes.half() / 127).to(dtype)
+    scale = torch.rand((2, B, Hkv, cap), device="cuda", generator=gen) / 127
+    return ops.QuantKV(codes[0], codes[1], scale[0], scale[1])
+
+
+def bench_append_read_q8(timer: Timer, dtype: torch.dtype):
+    Hq, Hkv, hd = 32, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.ones(hd, device="cuda", dtype=torch.bfloat16)
+    inv = 1e6 ** (-torch.arange(0, hd, 2, device="cuda", dtype=torch.float32) / hd)
+    for M in (16, 16384):
+        kv = _quant_cache(dtype, 1, Hkv, M + 64, hd, gen)
+        qkv = torch.randn((M, (Hq + 2 * Hkv) * hd), device="cuda", generator=gen).bfloat16()
+        pos = torch.arange(M, dtype=torch.int32, device="cuda")
+        q = torch.empty((M, Hq, hd), dtype=torch.bfloat16, device="cuda")
+        sec = timer(lambda: ops.qkv_rope_append_q8(qkv, pos, w, w, inv, kv, Hq, hd, 1e-6, q_out=q))
+        _line("append_q8", "append_q8_kernel", sec, bytes_=qkv.numel() * 2 + q.numel() * 2 + M * Hkv * 2 * (hd + 4),
+              extra={"workload": f"{dtype} rows={M} Hq={Hq} Hkv={Hkv} hd={hd}"})
+    kv = _quant_cache(dtype, 64, Hkv, 1024, hd, gen)
+    pos = torch.arange(1024, dtype=torch.int32, device="cuda").repeat(64)
+    seq = torch.arange(64, dtype=torch.int32, device="cuda").repeat_interleave(1024)
+    k, v = ops.kv_read_q8(kv, pos, row_seq=seq)
+    sec = timer(lambda: ops.kv_read_q8(kv, pos, seq, k, v))
+    _line("read_q8", "read_q8_kernel", sec, bytes_=k.numel() * 2 * (1 + 2) + 2 * 64 * 1024 * Hkv * 4,
+          extra={"workload": f"{dtype} rows={64 * 1024} Hkv={Hkv} hd={hd}"})
+
+
 def bench_gemm_c4(timer: Timer, M: int = 1024, wide: bool = True, wide_split: int = 1):
     """The verify GEMMs at C4's 1024 rows; wide=True is the whole-K tile form batched
     sessions use, wide=False the M <= 16 weight-streaming form for comparison."""
@@ -218,6 +271,15 @@ def main(argv=None):
         ctxs = torch.randint(512, 4097, (64,), generator=g).tolist()
         for kc in ([args.key_chunk] if args.key_chunk else (128, 512, 1024, 4224)):
             bench_attention(timer, 64, 16, ctxs, "attn_c4", key_chunk=kc)
+    if "kv_q8" in sel:
+        g = torch.Generator().manual_seed(3)
+        ctxs = torch.randint(512, 4097, (64,), generator=g).tolist()
+        for dtype in (torch.int8, torch.float8_e4m3fn):
+            bench_attention_q8(timer, dtype, 16, [1536], "attn_q8_c3")
+            bench_attention_q8(timer, dtype, 16, ctxs, "attn_q8_c4")
+            bench_attention_q8(timer, dtype, 1, ctxs, "attn_q8_decode64")
+            bench_attention_q8(timer, dtype, 1024, [4096], "attn_q8_prefill")
+            bench_append_read_q8(timer, dtype)
     if "gemm" in sel:
         bench_gemm_c4(timer, wide_split=args.wide_split)
     if "verify" in sel:

@@ -140,12 +140,12 @@ def alloc_kv(n_layers: int, batch: int, n_kv: int, cap: int, hd: int, device,
 def q8_split(batch: int, n_kv: int, max_total: int, head_dim: int = 128) -> tuple[str, int]:
     """(form, keys per split) of a session's attention over an 8-bit cache. It depends on what a
     session's plain and speculative decode share (sequences, kv heads, total length), so that
-    their rows agree bit for bit. Up to about 4096 keys of one stream (8 kv heads; a sixth of that at
-    head_dim 256) the warp form in short splits; else the tcgen05 form, in splits that give each SM
-    about two CTAs, a power of two."""
+    their rows agree bit for bit. Up to about 4500 positions of one stream with 8 kv heads (head_dim
+    256: 3500 with 4) the warp form in short splits; else the tcgen05 form, in splits that give each
+    SM about two CTAs, a power of two."""
     work = max_total * batch * n_kv
-    if work <= (8192 if head_dim == 256 else 36864):
-        return "warp", 256 if work <= 16384 and head_dim < 256 else 3 * ops.Q8_CHUNK
+    if work <= (14336 if head_dim == 256 else 36864):
+        return "warp", (2 if work <= 16384 else 3) * ops.Q8_CHUNK
     chunk = 512
     while chunk < 8192 and chunk * 296 < work:
         chunk *= 2
