@@ -27,8 +27,9 @@
 //    10. So w_j < 2^15 whatever the scales are, and weights down to 2^-18 of the largest keep all their
 //    bits (those below are rounded to multiples of 2^-28 of it); the sum of e_j uses the same M, which
 //    cancels in the quotient.
-// Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales,
-// codes or query products may be anything), so infinities and NaN there do not reach the row.
+// Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales
+// and query products may be anything), so infinities and NaN there do not reach the row; codes are
+// numbers (a weight of 0 times e4m3's NaN code would not be 0; the append writes none).
 #include "attention_q8.cuh"
 
 #include <type_traits>

@@ -468,7 +468,8 @@ class QuantKV:
     [seq, Hkv, cap, hd] int8 or float8_e4m3fn and fp32 scales [seq, Hkv, cap], the value held
     being code * scale; or, with ``page_table`` [seq, pages] int32, page pools
     [n_pages, Hkv, page_size, hd] and [n_pages, Hkv, page_size]. The tensors may be views
-    (sequence and head strides are free), K and V alike."""
+    (sequence and head strides are free), K and V alike. Positions that a call reads hold no e4m3 NaN
+    codes (qkv_rope_append_q8 writes none)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  page_table: torch.Tensor | None = None, page_size: int = 0):
@@ -542,7 +543,7 @@ def qkv_rope_append_q8(qkv: torch.Tensor, pos: torch.Tensor, q_norm: torch.Tenso
     p_pos = _index_rows("pos", pos, M, idx)
     p_seq = None if row_seq is None else _index_rows("row_seq", row_seq, M, idx)
     for w in (q_norm, k_norm) if do_q else (k_norm,):
-        if w.dtype is not torch.bfloat16 or w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous() \
+        if w is None or w.dtype is not torch.bfloat16 or w.dim() != 1 or w.shape[0] != hd or not w.is_contiguous() \
                 or w.get_device() != idx:
             raise ValueError(f"norm weights must be contiguous bf16 [{hd}] on cuda:{idx}")
     if inv_freq.dtype is not torch.float32 or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous() \

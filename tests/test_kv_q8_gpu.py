@@ -495,3 +495,87 @@ def test_larger_tiles_of_the_warp_form(t, lens, rows, Hkv, G, hd, causal, gated)
     assert torch.equal(*got)
     ref, tol = _attention64(c.val, q, pos + 1 if causal else kv_len[seq.long()], seq, hd ** -0.5, gate)
     assert ((got[0].double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide", "auto"])
+def test_last_run_may_be_short_and_outputs_may_be_views(form):
+    """M no multiple of seq_rows, seq_rows above M, an output and a gate that are column slices."""
+    from dflash_b200 import ops
+    Hkv, G, hd = 2, 4, 128
+    c = Cache("e4m3", [300, 41, 500], Hkv, hd, 64, seed=6)
+    g = torch.Generator().manual_seed(6)
+    M = 37  # runs of 16, 16 and 5 rows
+    q = torch.randn(M, Hkv * G, hd, generator=g).bfloat16().to(DEV)
+    seq = (torch.arange(M, dtype=torch.int32) // 16).to(DEV)
+    pos = torch.tensor([n - 16 + i for n in (300, 41, 500) for i in range(16)][:M], dtype=torch.int32, device=DEV)
+    gate = torch.randn(M, 3, Hkv * G * hd, generator=g).bfloat16().to(DEV)
+    buf = torch.full((M, 2, Hkv * G * hd), 9.0, dtype=torch.bfloat16, device=DEV)
+    kw = dict(causal=True, max_kv=500, form=form, key_chunk=256)
+    ops.attention_q8(q, c.kv, pos, row_seq=seq, seq_rows=16, out=buf[:, 1], gate=gate[:, 2], **kw)
+    assert (buf[:, 0] == 9).all()
+    for a in (0, 16, 32):
+        b = min(a + 16, M)
+        one = ops.attention_q8(q[a:b], c.kv, pos[a:b], row_seq=seq[a:b], seq_rows=64, gate=gate[a:b, 2].contiguous(), **kw)
+        if form != "auto":  # whose form may differ with the call's size
+            assert torch.equal(one, buf[a:b, 1])
+    ref, tol = _attention64(c.val, q.cpu(), pos.cpu() + 1, seq.cpu(), hd ** -0.5, gate[:, 2].cpu())
+    assert ((buf[:, 1].double().cpu() - ref).abs() <= tol).all()
+    assert ops.device_error() == 0
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    from dflash_b200 import ops
+    c = Cache("int8", [64], 2, 128)
+    q, pos = torch.randn(3, 4, 128).bfloat16().to(DEV), torch.arange(3, dtype=torch.int32, device=DEV)
+    w, inv, qkv = torch.ones(128).bfloat16().to(DEV), torch.ones(64, device=DEV), torch.randn(3, 8 * 128).bfloat16().to(DEV)
+    att = lambda **kw: ops.attention_q8(**{**dict(q=q, kv=c.kv, pos=pos, causal=True, max_kv=64), **kw})  # noqa: E731
+    app = lambda **kw: ops.qkv_rope_append_q8(**{**dict(qkv=qkv, pos=pos, q_norm=w, k_norm=w, inv_freq=inv, kv=c.kv, Hq=4,  # noqa: E731
+                                                        rot_dim=128, eps=1e-6), **kw})
+    for call, kw in ((att, dict(q=q.float())), (att, dict(q=q[:, :, :64])), (att, dict(q=q.transpose(0, 1))),
+                     (att, dict(pos=pos[:2])), (att, dict(pos=pos.long())), (att, dict(pos=pos.cpu())),
+                     (att, dict(row_seq=pos[::2])), (att, dict(kv_len=pos[:0])), (att, dict(form="mma")),
+                     (att, dict(out=torch.empty(3, 512, device=DEV))), (att, dict(gate=qkv[:2])),
+                     (app, dict(qkv=qkv[:, :900])), (app, dict(qkv=qkv.float())), (app, dict(q_norm=None)),
+                     (app, dict(k_norm=w[:64])), (app, dict(inv_freq=inv[:10])), (app, dict(pos=pos[:1])),
+                     (app, dict(q_out=q[:2]))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    for call, kw in ((att, dict(key_chunk=100)), (att, dict(max_kv=0)), (att, dict(causal=False)),
+                     (att, dict(scale=math.inf)), (app, dict(rot_dim=24)), (app, dict(q_stride=64))):
+        with pytest.raises(Exception, match="dfl_"):
+            call(**kw)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_offsets_beyond_32_bits(paged):
+    """Sequences (or pages) more than 2^31 bytes apart: append, read-back and every form of the attention
+    give the bits of a small cache."""
+    from dflash_b200 import ops
+    Hkv, G, hd, n = 2, 4, 128, 128
+    far = 2 ** 31 + 4096
+    buf = torch.zeros(far + 2 ** 20, dtype=torch.int8, device=DEV)
+    sbuf = torch.zeros(2 ** 14, device=DEV)
+    cut = lambda b, o, st, shape: torch.as_strided(b, shape, st, o)  # noqa: E731
+    rows = 64 if paged else n
+    shape = (2, Hkv, rows, hd)
+    k, v = [cut(buf, o, (far, rows * hd, hd, 1), shape) for o in (0, 2 ** 19)]
+    ks, vs = [cut(sbuf, o, (2 ** 12, rows, 1), shape[:3]) for o in (0, 2 ** 13)]
+    small = [torch.zeros(shape, dtype=torch.int8, device=DEV) for _ in range(2)] + [torch.zeros(shape[:3], device=DEV) for _ in range(2)]
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV) if paged else None
+    got = []
+    for kv in (ops.QuantKV(k, v, ks, vs, table, 64 if paged else 0), ops.QuantKV(*small, table, 64 if paged else 0)):
+        g = torch.Generator().manual_seed(8)
+        seq = torch.full((n,), 0 if paged else 1, dtype=torch.int32, device=DEV)
+        pos = torch.arange(n, dtype=torch.int32, device=DEV)
+        qkv = torch.randn(n, (Hkv * G + 2 * Hkv) * hd, generator=g).bfloat16().to(DEV)
+        w, inv = torch.ones(hd).bfloat16().to(DEV), torch.ones(hd // 2, device=DEV)
+        q = ops.qkv_rope_append_q8(qkv, pos, w, w, inv, kv, Hkv * G, hd, 1e-6, row_seq=seq)
+        out = [q, *ops.kv_read_q8(kv, pos, row_seq=seq)]
+        for form in ("warp", "tc", "wide"):
+            out.append(ops.attention_q8(q, kv, pos, True, n, row_seq=seq, seq_rows=n, form=form, key_chunk=128))
+        got.append(out)
+    assert ops.device_error() == 0
+    assert got[0][1].abs().sum() > 0
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
