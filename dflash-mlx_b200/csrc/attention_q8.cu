@@ -648,11 +648,11 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // 16.2), 4096 keys 16.0 (20.5, 16.5). Others take a tcgen05 form, tc of 64 rows a CTA: four such sequences of 2048
 // keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 124 (338 in 64-row tiles); 64 single
 // tokens 107, in the warp form 66. Wide, of 256 rows (head_dim 256: 128), for runs that fill more than half of them
-// and calls with 384 keys for every SM: 128 rows of 32 heads at 4096 keys 30 us (tc 36), at 1024 28 (17);
-// 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256, 50 us (tc 57).
+// and calls with a CTA, or 384 keys, for every SM: 128 rows of 32 heads at 4096 keys 28 us (tc 36), at 1024 27 (16);
+// 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256, 46 us (tc 55).
 // Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for several
-// runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 57 us
-// with it, 72 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
+// runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 55 us
+// with it, 71 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
 // keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and 8.0,
 // with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05
 // forms 512, and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us,
@@ -669,7 +669,7 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
   const int wide = hd == 256 ? 128 : 256;
   p.form = form != DFL_Q8_AUTO                                              ? form
            : few                                                          ? DFL_Q8_WARP
-           : want > wide / 2 && units(wide) * max_kv >= (long long)148 * 384 ? DFL_Q8_WIDE
+           : want > wide / 2 && units(wide) * (max_kv < 384 ? 384 : max_kv) >= 148 * 384LL ? DFL_Q8_WIDE
                                                                           : DFL_Q8_TC;
   const bool tc = p.form >= DFL_Q8_TC;
   p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? small : want <= 32 || hd == 256 ? 32 : 64;

@@ -77,7 +77,7 @@ __device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, i
 
 // Tile and kv head of a CTA: heads of a run side by side, runs in the launch's order. That order is by keys,
 // most first (ties by index), where a.ranked: a long run started last would leave the other SMs idle
-// (64 runs of 512 to 4096 keys, tcgen05 form: 169 us in index order, 130 so). Every CTA
+// (64 runs of 512 to 4096 keys, tcgen05 form: 169 us in index order, 130 so, before later steps). Every CTA
 // ranks the runs alike from their last rows' limits, a permutation whatever those are.
 constexpr int Q8_RANK_RUNS = 256;
 struct Q8Tile {

@@ -8,7 +8,7 @@
 //    warps have work; the copies are merged at the end. Two CTAs an SM (one at head_dim 256).
 //  * wide, for prefill: a row once, and two groups of 128 rows and four softmax warps each that share the
 //    converted tiles (256 rows; at head_dim 256, where TMEM holds one group, 128). One CTA an SM. 1024 rows of
-//    32 heads of 128 at 4096 keys: 111 us, 0.54 PFLOP/s (tc: 173 us).
+//    32 heads of 128 at 4096 keys: 106 us, 0.56 PFLOP/s (tc: 171 us).
 // Per block and group:
 //   S = Q K^T      M = 128, N = 64, K = hd, both operands fp16 in shared memory
 //   w = e vs       one thread per (row, copy), 32 (wide: 64) keys each; fp16, over S's own TMEM columns, the
@@ -16,11 +16,13 @@
 //   O += w V       A = w from TMEM, B = V as [key][dim] in shared memory (MN-major), N = hd
 // Four softmax and epilogue warps a group, then four that convert codes to fp16 tiles (two K, two V), the last
 // issues the MMAs. The converters load codes straight into registers, one block ahead of the one they convert.
-// What bounds it is the chain of these roles, not one unit (64 blocks of 16, 512 to 4096 keys: 124 us, 42 % of
-// the copy rate; without the softmax arithmetic 108, without MMAs 113, without the loads 122, issue slots 41 %
-// busy). A block's softmax takes about 1200 clocks, and the issuing thread, at 58 clocks an MMA, 80 a commit and
+// What bounds it is the chain of these roles, not one unit (64 blocks of 16, 512 to 4096 keys: 119 us, 44 % of
+// the copy rate; at 130 us leaving out the softmax arithmetic gave 108, the MMAs 113, the loads 122; issue slots
+// are 46 % busy). A block's softmax takes about 1200 clocks, and the issuing thread, at 58 clocks an MMA, 80 a commit and
 // 130 a wait even for a barrier that is complete, nearly as many: it has one wait and two commits a
-// block (with a barrier for each tile: 130 us, wide 129 instead of 111).
+// block (with a barrier for each tile: 130 instead of 124 us, wide 129 instead of 111). A CTA's start and end, 12000 clocks
+// (18000 with one row after the other in the Q conversion and the epilogue, and Q loaded behind the positions;
+// 124 us, wide 111), are each a chain of latencies: several rows side by side.
 // A row's exponent base M follows its maximum lazily: sums, weights and O are rescaled only when
 // M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to 2^-18 of
 // the largest keep all their bits (those below are rounded to multiples of 2^-28 of it).
@@ -122,7 +124,6 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
   float* s_sc = reinterpret_cast<float*>(smem + L::OFF_S);  // [ring][K, V][64]
   uint32_t* s_vmax = reinterpret_cast<uint32_t*>(s_sc + QT_SCALES * 2 * QT_KB);  // [ring][half], finite scales' bits
   float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_R);
-  int* s_lim = reinterpret_cast<int*>(smem + L::OFF_R) + ROWS;
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + ROWS * 8);  // [128 SG]
   float4* s_w = reinterpret_cast<float4*>(s_ml + SG * 128);  // [rows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -154,6 +155,27 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     pos2[k] = i < ntok ? a.pos[m0 + i] : -1;
     sq2[k] = i < ntok && a.row_seq ? a.row_seq[m0 + i] : 0;
   }
+  const int n_rows = ntok * a.G, groups = SG == 1 || n_rows <= 128 ? 1 : SG;
+  // The softmax warps' Q rows, on their way while positions and limits are looked up: raw, into the last copy's place
+  // (hd / 16 lanes a row, 32 bytes each), where each thread later converts what it copied. Rolled loops here and
+  // there: code that runs once a CTA comes from a cold instruction cache.
+  constexpr int GR = 128 / CP, LPR = HD / 16, QPW = 32 / LPR;  // a group's rows, lanes a row, rows a warp
+  const int ql = lane % LPR, qr = (warp & 3) * QPW + lane / LPR, g0 = (warp >> 2) * GR;
+  unsigned char* q1 = smem + L::OFF_Q + (warp >> 2) * 128 * HD * 2 + (ql >> 2) * 16384 + (CP - 1) * GR * 128;
+  if (warp < L::CONV) {
+    const float inv_g = 1.f / (float)a.G;
+#pragma unroll 1
+    for (int r = qr; r < GR; r += 4 * QPW) {
+      const bool ok = g0 + r < n_rows;
+      const int tok = (int)(((float)(g0 + r) + 0.5f) * inv_g);  // (g0 + r) / G: at least 1 / 32 from an integer
+      const __nv_bfloat16* q =
+          ok ? a.q + ((long long)(m0 + tok) * a.Hq + kvh * a.G + (g0 + r - tok * a.G)) * HD + ql * 16 : a.q;
+      const uint32_t d = smem_u32(q1) + qt_sw(r, (ql & 3) * 2);
+      cp_async16(d, q, ok ? 16 : 0);
+      cp_async16(d ^ 16, q + (ok ? 8 : 0), ok ? 16 : 0);
+    }
+    cp_async_commit();
+  }
 #pragma unroll
   for (int k = LANE_ROWS - 1; k >= 0; --k) {
     const unsigned v = __ballot_sync(0xffffffffu, pos2[k] >= 0);
@@ -161,9 +183,13 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     if (v) seq = s;
     any = any || v;
   }
-  if (!any) return;
+  if (!any) {
+    cp_async_wait<0>();
+    return;
+  }
   if (seq < 0 || seq >= a.c.n_seqs) {  // a row that names no sequence of the cache is left as it is
     if (threadIdx.x == 0) q8_error(a.err, Q8_ERR_SEQ);
+    cp_async_wait<0>();
     return;
   }
   int lim_max = 0, lim_min = 0x7fffffff;
@@ -183,10 +209,12 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
   lim_max = __reduce_max_sync(0xffffffffu, lim_max);
   lim_min = __reduce_min_sync(0xffffffffu, lim_min);
   const int k_begin = chunk * a.key_chunk;
-  if (k_begin >= lim_max && a.n_chunks > 1) return;
+  if (k_begin >= lim_max && a.n_chunks > 1) {
+    cp_async_wait<0>();
+    return;
+  }
   const int k_end = min(k_begin + a.key_chunk, lim_max);
   const int n_blocks = (max(k_end - k_begin, 0) + QT_KB - 1) / QT_KB;
-  const int n_rows = ntok * a.G, groups = SG == 1 || n_rows <= 128 ? 1 : SG;
   if (threadIdx.x == 32 * L::ISSUER) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 64);
@@ -374,57 +402,55 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     }
   } else {
     // ---------------- softmax: thread = (row, copy), four warps a group ----------------
-    // Q rows to scaled fp16, CP times; a row's factor undoes its power of two. The raw rows all come at once
-    // into the last copy's place, where each thread then converts what it copied: hd / 16 lanes a row,
-    // 32 bytes each, in rolled loops (code that runs once a CTA comes from a cold instruction cache).
+    // Q rows to scaled fp16, CP times; a row's factor undoes its power of two. U rows of a warp side by side, as
+    // each is a chain of shared-memory and shuffle latencies.
     {
-      constexpr int LPR = HD / 16, RPW = 32 / LPR;
-      constexpr int GR = 128 / CP;  // a group's rows
-      const int ql = lane % LPR, qr = (warp & 3) * RPW + lane / LPR, g0 = (warp >> 2) * GR;
-      unsigned char* q1 = smem + L::OFF_Q + (warp >> 2) * 128 * HD * 2 + (ql >> 2) * 16384 + (CP - 1) * GR * 128;
-#pragma unroll 1
-      for (int r = qr; r < GR; r += 4 * RPW) {
-        const int th = s_row[g0 + r];
-        const bool ok = th >= 0 && s_tok_lim[th >> 4] > 0;
-        const __nv_bfloat16* q =
-            ok ? a.q + ((long long)(m0 + (th >> 4)) * a.Hq + kvh * a.G + (th & 15)) * HD + ql * 16 : a.q;
-        const uint32_t d = smem_u32(q1) + qt_sw(r, (ql & 3) * 2);
-        cp_async16(d, q, ok ? 16 : 0);
-        cp_async16(d ^ 16, q + (ok ? 8 : 0), ok ? 16 : 0);
-      }
-      cp_async_commit();
+      constexpr int TURNS = GR / (4 * QPW), U = TURNS < 4 ? TURNS : 4;
       cp_async_wait<0>();
 #pragma unroll 1
-      for (int r = qr; r < GR; r += 4 * RPW) {
-        uint4* d0 = reinterpret_cast<uint4*>(q1 + qt_sw(r, (ql & 3) * 2));
-        uint4* d1 = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d0) ^ 16);
-        const uint4 n0 = *d0, n1 = *d1;
-        const uint32_t u[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+      for (int r = qr; r < GR; r += 4 * QPW * U) {
+        uint4* d0[U];
+        uint32_t u[U][8], mx[U];
+#pragma unroll
+        for (int t = 0; t < U; ++t) {
+          d0[t] = reinterpret_cast<uint4*>(q1 + qt_sw(r + t * 4 * QPW, (ql & 3) * 2));
+          const uint4 n0 = *d0[t], n1 = *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d0[t]) ^ 16);
+          u[t][0] = n0.x, u[t][1] = n0.y, u[t][2] = n0.z, u[t][3] = n0.w;
+          u[t][4] = n1.x, u[t][5] = n1.y, u[t][6] = n1.z, u[t][7] = n1.w;
+        }
         // magnitudes compare as integers; one that is not finite leaves the row unscaled
-        uint32_t mx2 = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mx2 = __vmaxu2(mx2, u[j] & 0x7fff7fffu);
-        uint32_t mx = max(mx2 << 16, mx2 & 0xffff0000u);
+        for (int t = 0; t < U; ++t) {
+          uint32_t m2[4];
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const int sh = mx > 0 && mx < 0x7f800000u ? min(14 - ((int)(mx >> 23) - 127), 120) : 0;
-        const float f = __uint_as_float((uint32_t)(sh + 127) << 23) * a.q_sign;
-        uint32_t h[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __half2 y = __floats2half2_rn(__uint_as_float(u[j] << 16) * f, __uint_as_float(u[j] & 0xffff0000u) * f);
-          h[j] = *reinterpret_cast<const uint32_t*>(&y);
+          for (int j = 0; j < 4; ++j) m2[j] = __vmaxu2(u[t][j] & 0x7fff7fffu, u[t][j + 4] & 0x7fff7fffu);
+          m2[0] = __vmaxu2(__vmaxu2(m2[0], m2[1]), __vmaxu2(m2[2], m2[3]));
+          mx[t] = max(m2[0] << 16, m2[0] & 0xffff0000u);
         }
-        const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
-        *d0 = h0;
-        *d1 = h1;
-        if (CP == 2) {
-          *(d0 - GR * 8) = h0;  // the first copy, 64 rows of 128 bytes before
-          *(d1 - GR * 8) = h1;
-        }
-        if (ql == 0) {
-          s_rowf[g0 + r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
-          s_lim[g0 + r] = s_row[g0 + r] < 0 ? 0 : s_tok_lim[s_row[g0 + r] >> 4];
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int t = 0; t < U; ++t) mx[t] = max(mx[t], __shfl_xor_sync(0xffffffffu, mx[t], o));
+#pragma unroll
+        for (int t = 0; t < U; ++t) {
+          const int sh = mx[t] > 0 && mx[t] < 0x7f800000u ? min(14 - ((int)(mx[t] >> 23) - 127), 120) : 0;
+          const float f = __uint_as_float((uint32_t)(sh + 127) << 23) * a.q_sign;
+          uint32_t h[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const __half2 y =
+                __floats2half2_rn(__uint_as_float(u[t][j] << 16) * f, __uint_as_float(u[t][j] & 0xffff0000u) * f);
+            h[j] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+          uint4* d1 = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(d0[t]) ^ 16);
+          *d0[t] = h0;
+          *d1 = h1;
+          if (CP == 2) {
+            *(d0[t] - GR * 8) = h0;  // the first copy, 64 rows of 128 bytes before
+            *(d1 - GR * 8) = h1;
+          }
+          if (ql == 0) s_rowf[g0 + r + t * 4 * QPW] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
         }
       }
     }
@@ -437,7 +463,7 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     p_full += 2 * grp;
     const uint32_t tmem = *tmem_slot + grp * L::GCOLS, t_o = tmem + 128;
     const int row = threadIdx.x & (ROWS - 1), half = CP == 2 ? threadIdx.x >> 6 : 0;
-    const int lim = s_lim[row];
+    const int lim = s_row[row] < 0 ? 0 : s_tok_lim[s_row[row] >> 4];
     const float rowf = s_rowf[row];
     float m = -INFINITY, mu_used = -INFINITY;
     uint64_t l = 0;  // two partial sums
@@ -574,61 +600,103 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     }
     s_ml[threadIdx.x] = make_float2(mu_used, q8_unpack(l).x + q8_unpack(l).y);
     asm volatile("bar.sync 1, %0;\n" ::"n"(SG * 128) : "memory");
-    // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and the row
-    // of the output (or of the partials) it goes to, -1 for none
+    // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and where it goes
+    // (over the row factors, and the thread's own (M, l), read no more)
+    long long* s_dst = reinterpret_cast<long long*>(s_rowf);
+    long long* s_gate = reinterpret_cast<long long*>(s_ml);
     if (threadIdx.x < ROWS) {
       const int r = threadIdx.x, th = s_row[r], tok = th >> 4;
       const float2 x0 = s_ml[r], x1 = CP == 2 ? s_ml[r + ROWS] : make_float2(-INFINITY, 0.f);
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
       float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
       const float den = w0 * x0.y + w1 * x1.y;
-      int to = -1;
+      long long dst = -1, gate = 0;  // where the row of the output (or of the partials) begins, and its gate's
       if (ok && th >= 0 && s_tok_ok[tok] && (a.n_chunks == 1 || lim > k_begin)) {
-        to = (m0 + tok) * a.Hq + kvh * a.G + (th & 15);
+        const long long m = m0 + tok, head = kvh * a.G + (th & 15);
         if (a.n_chunks > 1) {
-          a.part_ml[(long long)chunk * a.M * a.Hq + to] = make_float2(mm, den);
+          const long long to = ((long long)chunk * a.M + m) * a.Hq + head;
+          a.part_ml[to] = make_float2(mm, den);
+          dst = to * HD;
         } else {
           const float inv = lim > 0 ? Q8_SUM_UNIT / den : 0.f;
           w0 *= inv;
           w1 *= inv;
+          dst = m * a.ldo + head * HD;
+          gate = m * a.ldg + head * a.gate_hs;
         }
       }
-      s_w[r] = make_float4(w0, w1, __int_as_float(to), lim > 0 ? 1.f : 0.f);
+      s_w[r] = make_float4(w0, w1, lim > 0 ? 1.f : 0.f, 0.f);
+      s_dst[r] = dst;
+      s_gate[r] = gate;
     }
     asm volatile("bar.sync 1, %0;\n" ::"n"(SG * 128) : "memory");
     constexpr int RPW = CH >= 32 ? 1 : 32 / CH;  // rows a warp writes at a time
-#pragma unroll 4
-    for (int r0 = warp * RPW; r0 < n_rows; r0 += 4 * SG * RPW) {
-      const int r = r0 + lane / (32 / RPW);
-      const float4 w = s_w[r];
-      const int to = __float_as_int(w.z);
-      if (to < 0) continue;
+    constexpr int NR = 4, STEP = 4 * SG * RPW;   // times in flight, rows between them
+    constexpr int NC = CH >= 32 ? CH / 32 : 1;   // float4s a lane has of a row
+    const int c0 = lane % (32 / RPW);
+    const bool wide_gate = (reinterpret_cast<uintptr_t>(a.gate) % 8 | a.ldg % 4 | a.gate_hs % 4) == 0;
+#pragma unroll 1
+    for (int r0 = warp * RPW + lane / (32 / RPW); r0 < n_rows; r0 += NR * STEP) {
+      float4 y[NR][NC];
+      long long dst[NR];
 #pragma unroll
-      for (int c = lane % (32 / RPW); c < CH; c += 32) {
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (w.w != 0.f) {
-          const float4 o0 = s_o[r * CH + (c ^ (r & 7))];
-          y = make_float4(w.x * o0.x, w.x * o0.y, w.x * o0.z, w.x * o0.w);
+      for (int u = 0; u < NR; ++u) {
+        const int r = min(r0 + u * STEP, ROWS - 1);
+        const float4 w = s_w[r];
+        dst[u] = r0 + u * STEP < n_rows ? s_dst[r] : -1;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          const int c = (c0 + 32 * k) ^ (r & 7);
+          const float4 o0 = s_o[r * CH + c];
+          float4 v = make_float4(w.x * o0.x, w.x * o0.y, w.x * o0.z, w.x * o0.w);
           if (CP == 2) {
-            const float4 o1 = s_o[(r + ROWS) * CH + (c ^ (r & 7))];
-            y = make_float4(w.x * o0.x + w.y * o1.x, w.x * o0.y + w.y * o1.y, w.x * o0.z + w.y * o1.z,
-                            w.x * o0.w + w.y * o1.w);
+            const float4 o1 = s_o[(r + ROWS) * CH + c];
+            v = make_float4(v.x + w.y * o1.x, v.y + w.y * o1.y, v.z + w.y * o1.z, v.w + w.y * o1.w);
           }
-        }
-        if (a.n_chunks > 1) {
-          *reinterpret_cast<float4*>(a.part_o + ((long long)chunk * a.M * a.Hq + to) * HD + c * 4) = y;
-        } else {
-          const int mrow = to / a.Hq, head = to - mrow * a.Hq;
-          float f[4] = {y.x, y.y, y.z, y.w};
-          if (a.gate) {
-            const __nv_bfloat16* gr = a.gate + (long long)mrow * a.ldg + (long long)head * a.gate_hs + c * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = f[e] / (1.f + __expf(-bf2f(gr[e])));
-          }
-          *reinterpret_cast<uint2*>(a.out + (long long)mrow * a.ldo + (long long)head * HD + c * 4) =
-              make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+          y[u][k] = w.z != 0.f ? v : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
+      if (a.n_chunks > 1) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+#pragma unroll
+          for (int k = 0; k < NC; ++k)
+            if (dst[u] >= 0) *reinterpret_cast<float4*>(a.part_o + dst[u] + (c0 + 32 * k) * 4) = y[u][k];
+        continue;
+      }
+      if (a.gate) {
+        uint2 g[NR][NC];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+          if (dst[u] < 0) continue;
+          const __nv_bfloat16* gr = a.gate + s_gate[r0 + u * STEP] + c0 * 4;
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            if (wide_gate) {
+              g[u][k] = *reinterpret_cast<const uint2*>(gr + 128 * k);
+            } else {
+              const unsigned short* gs = reinterpret_cast<const unsigned short*>(gr + 128 * k);
+              g[u][k] = make_uint2(gs[0] | (uint32_t)gs[1] << 16, gs[2] | (uint32_t)gs[3] << 16);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < NR; ++u)
+#pragma unroll
+          for (int k = 0; k < NC; ++k) {
+            y[u][k].x /= 1.f + __expf(-__uint_as_float(g[u][k].x << 16));
+            y[u][k].y /= 1.f + __expf(-__uint_as_float(g[u][k].x & 0xffff0000u));
+            y[u][k].z /= 1.f + __expf(-__uint_as_float(g[u][k].y << 16));
+            y[u][k].w /= 1.f + __expf(-__uint_as_float(g[u][k].y & 0xffff0000u));
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < NR; ++u)
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+          if (dst[u] >= 0)
+            *reinterpret_cast<uint2*>(a.out + dst[u] + (c0 + 32 * k) * 4) =
+                make_uint2(pack_bf16x2(y[u][k].x, y[u][k].y), pack_bf16x2(y[u][k].z, y[u][k].w));
     }
   }
   tc_fence_before();
