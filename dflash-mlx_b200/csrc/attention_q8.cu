@@ -101,6 +101,28 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
     pos2[k] = i < ntok ? a.pos[m0 + i] : -1;
     sq2[k] = i < ntok && a.row_seq ? a.row_seq[m0 + i] : 0;
   }
+  // this warp's Q rows, on their way while positions and limits are looked up
+  constexpr int VEC = HD / 32, NI = L::ROWS / NWARPS;
+  uint32_t qu[NI][VEC / 2];
+  {
+    const float inv_g = 1.f / (float)a.G;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = warp + i * NWARPS;
+      const int tok = (int)(((float)r + 0.5f) * inv_g);  // r / G: at least 1 / 32 from an integer
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          a.q + ((long long)(m0 + min(tok, ntok - 1)) * a.Hq + kvh * a.G + (r - tok * a.G)) * HD) + lane * (VEC / 2);
+      if constexpr (VEC == 2) {
+        qu[i][0] = src[0];
+      } else if constexpr (VEC == 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        qu[i][0] = w.x, qu[i][1] = w.y;
+      } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        qu[i][0] = w.x, qu[i][1] = w.y, qu[i][2] = w.z, qu[i][3] = w.w;
+      }
+    }
+  }
   const unsigned v0 = __ballot_sync(0xffffffffu, pos2[0] >= 0), v1 = __ballot_sync(0xffffffffu, pos2[1] >= 0);
   if (!(v0 | v1)) return;
   const int seq = __shfl_sync(0xffffffffu, v0 ? sq2[0] : sq2[1], __ffs(v0 ? v0 : v1) - 1);
@@ -193,29 +215,27 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
 
   __syncthreads();  // the rows' limits
   // ---- Q rows to scaled fp16, dims permuted within 16 to the order of a K register ----
-  for (int r = warp; r < L::ROWS; r += NWARPS) {
-    const int tok = r / a.G, hg = r % a.G;
-    const bool ok = tok < ntok && s_tok_lim[min(tok, ntok - 1)] > 0;
-    constexpr int VEC = HD / 32;
-    float x[VEC];
-    float mx = 0.f;
-    const __nv_bfloat16* src = a.q + ((long long)(ok ? m0 + tok : m0) * a.Hq + kvh * a.G + (ok ? hg : 0)) * HD;
-    uint32_t u[VEC / 2];
-    if constexpr (VEC == 2) {
-      u[0] = reinterpret_cast<const uint32_t*>(src)[lane];
-    } else if constexpr (VEC == 4) {
-      const uint2 w = reinterpret_cast<const uint2*>(src)[lane];
-      u[0] = w.x, u[1] = w.y;
-    } else {
-      const uint4 w = reinterpret_cast<const uint4*>(src)[lane];
-      u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
-    }
+  bool q_ok[NI];
+  float q_max[NI];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] = !ok ? 0.f : __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
-      mx = fmaxf(mx, fabsf(x[j]));
+  for (int i = 0; i < NI; ++i) {
+    const int tok = (warp + i * NWARPS) / a.G;
+    q_ok[i] = tok < ntok && s_tok_lim[min(tok, ntok - 1)] > 0;
+    q_max[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      if (!q_ok[i]) qu[i][j] = 0;
+      q_max[i] = fmaxf(q_max[i], fmaxf(fabsf(__uint_as_float(qu[i][j] << 16)), fabsf(__uint_as_float(qu[i][j] & 0xffff0000u))));
     }
-    mx = warp_max(mx);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) q_max[i] = fmaxf(q_max[i], __shfl_xor_sync(0xffffffffu, q_max[i], o));
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = warp + i * NWARPS;
+    const float mx = q_max[i];
     // 2^(14 - floor(log2 mx)), within fp32's normal powers of two; 1 for zero or non-finite rows
     int sh = 0;
     if (mx > 0.f && mx < INFINITY) sh = min(14 - ((int)(__float_as_uint(mx) >> 23) - 127), 120);
@@ -226,12 +246,13 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
       const int c = d >> 4, dd = d & 15;
       const int kp = 2 * (dd >> 2) + (dd & 2) * 4;  // place of dims (dd, dd + 1) among the 16
       const int cc = 2 * c + (kp >> 3);
-      const __half2 h = __floats2half2_rn(x[j] * f * a.q_sign, x[j + 1] * f * a.q_sign);
+      const __half2 h = __floats2half2_rn(__uint_as_float(qu[i][j / 2] << 16) * f * a.q_sign,
+                                          __uint_as_float(qu[i][j / 2] & 0xffff0000u) * f * a.q_sign);
       *reinterpret_cast<__half2*>(sQ + r * HD + ((cc ^ (r & 7)) << 3) + (kp & 7)) = h;
     }
     if (lane == 0) {
       s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
-      s_lim[r] = ok ? s_tok_lim[tok] : 0;
+      s_lim[r] = q_ok[i] ? s_tok_lim[r / a.G] : 0;
     }
   }
   __syncthreads();
@@ -644,19 +665,20 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // The form, tile rows and keys per chunk of a call.
 // Few: runs of at most 16 (token, head) rows, and calls small enough that tiles of 16 rows with 384 keys each
 // fit one wave (three CTAs an SM; at head_dim 256 one, of 32 rows where there are more than 16). They take the
-// warp form in such tiles, for their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128: 10.3 us (64-row tiles 15.2, tcgen05
-// 16.2), 4096 keys 16.0 (20.5, 16.5). Others take a tcgen05 form, tc of 64 rows a CTA: four such sequences of 2048
-// keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 124 (338 in 64-row tiles); 64 single
-// tokens 107, in the warp form 66. Wide, of 256 rows (head_dim 256: 128), for runs that fill more than half of them
-// and calls with a CTA, or 384 keys, for every SM: 128 rows of 32 heads at 4096 keys 28 us (tc 36), at 1024 27 (16);
-// 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256, 46 us (tc 55).
-// Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for several
-// runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 55 us
+// warp form in such tiles, for their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128, 10.3 us when
+// chosen (64-row tiles 15.2, tcgen05 16.2), 9.4 since Q is loaded beside the positions; 4096 keys 16.0 (20.5, 16.5),
+// now 14.9. Others take a tcgen05 form, tc of 64 rows a
+// CTA: four such sequences of 2048 keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 119
+// (338 in 64-row tiles); 64 single tokens 107, in the warp form 66 (now 63). Wide, of 256 rows (head_dim 256: 128), for
+// runs that fill more than half of them and calls with a CTA, or 384 keys, for every SM: 128 rows of 32 heads at
+// 4096 keys 28 us (tc 36), at 1024 27 (16); 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256,
+// 46 us (tc 55).
+// Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for
+// several runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 55 us
 // with it, 71 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
-// keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and 8.0,
-// with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05
-// forms 512, and no split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us,
-// split in two 13.6).
+// keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and
+// 8.0, with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05 forms 512, and no split of 512 keys where half
+// the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6).
 struct Q8Plan {
   int form, rows, key_chunk, n_chunks;  // rows: (token, head) pairs a CTA takes
 };
