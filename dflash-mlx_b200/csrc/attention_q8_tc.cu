@@ -8,7 +8,7 @@
 //    warps have work; the copies are merged at the end. Two CTAs an SM (one at head_dim 256).
 //  * wide, for prefill: a row once, and two groups of 128 rows and four softmax warps each that share the
 //    converted tiles (256 rows; at head_dim 256, where TMEM holds one group, 128). One CTA an SM. 1024 rows of
-//    32 heads of 128 at 4096 keys: 106 us, 0.56 PFLOP/s (tc: 171 us).
+//    32 heads of 128 at 4096 keys: 103 us, 0.58 PFLOP/s (tc: 171 us).
 // Per block and group:
 //   S = Q K^T      M = 128, N = 64, K = hd, both operands fp16 in shared memory
 //   w = e vs       one thread per (row, copy), 32 (wide: 64) keys each; fp16, over S's own TMEM columns, the
@@ -353,7 +353,9 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     grid_dependency_launch_dependents();  // not before the allocation: a dependent's must not come first
     const uint32_t tmem = *tmem_slot;  // a group's S / weights: columns 0-63, 64-127, O from 128 on
     // The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
-    const bool leader = lane == 0;
+    uint32_t elected;  // by elect.sync rather than by lane number: wide 106 -> 103 us
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(elected));
+    const bool leader = elected != 0;
     const uint64_t qd = sw128_desc(smem_u32(smem + L::OFF_Q));
     const uint64_t kd0 = sw128_desc(smem_u32(smem + L::OFF_K));
     const uint64_t vd0 = sw128_mn_desc(smem_u32(smem + L::OFF_V), QT_KB * 128, 1024);
