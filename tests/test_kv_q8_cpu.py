@@ -104,3 +104,18 @@ def test_scratch_query_answers_0_where_the_call_would_refuse(lib):
         assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, Hq, 16, 1, 4096, 0, 0) == 0
     assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, 32, 16, 1, 4096, 0, 0) > 0
     assert _lib.query("dfl_attention_q8_workspace_bytes", ref, 16, 128, 16, 1, 4096, 1, 128) > 0
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_session_split_follows_the_shared_sizes(hd):
+    """Forms the entry point knows, chunks it takes; short streams in the warp form, long or many in tcgen05."""
+    from dflash_b200.model import q8_split
+    from dflash_b200.ops import Q8_CHUNK, Q8_FORMS
+    seen = set()
+    for batch in (1, 2, 4, 64):
+        for total in (64, 1000, 5000, 40000, 131072):
+            form, chunk = q8_split(batch, 8, total, hd)
+            assert form in Q8_FORMS and chunk % Q8_CHUNK == 0 and Q8_CHUNK <= chunk <= 8192
+            assert (form == "warp") == (total * batch * 8 <= (14336 if hd == 256 else 36864))
+            seen.add(form)
+    assert seen == {"warp", "tc"}

@@ -579,3 +579,56 @@ def test_offsets_beyond_32_bits(paged):
     assert got[0][1].abs().sum() > 0
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide"])
+@pytest.mark.parametrize("page,causal", [(0, True), (64, False)])
+def test_nan_codes_behind_the_last_key_are_not_read(form, page, causal):
+    """Memory that no position of the call has reached may hold anything, e4m3's NaN codes included."""
+    from dflash_b200 import ops
+    lens, rows = [133, 64, 290], 7
+    c = Cache("e4m3", lens, 2, 128, page, seed=12)
+    g = torch.Generator().manual_seed(12)
+    q = torch.randn(3 * rows, 8, 128, generator=g).bfloat16().to(DEV)
+    seq = torch.arange(3, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    call = lambda: ops.attention_q8(q, c.kv, pos, causal, 290, kv_len=kv_len, row_seq=seq, seq_rows=rows, form=form,  # noqa: E731
+                                    key_chunk=128)
+    before = call()
+    raw = c.codes.view(torch.uint8)
+    for b, n in enumerate(lens):
+        if page:
+            table = c.kv.tensors[4]
+            raw[:, int(table[b, (n - 1) // page]), :, (n - 1) % page + 1:] = 0xff
+        else:
+            raw[:, b, :, n:] = 0x7f
+    assert torch.equal(call(), before) and before.isfinite().all()
+    assert ops.device_error() == 0
+
+
+def test_large_calls_side_by_side_on_two_streams():
+    """A prefill (all of an SM's TMEM) beside a batch of verify blocks (half of it) and single tokens."""
+    from dflash_b200 import ops
+    g = torch.Generator().manual_seed(13)
+    calls = []
+    for B, rows, n, form in ((1, 512, 1500, "wide"), (40, 16, 900, "tc"), (40, 1, 900, "warp")):
+        kv = ops.QuantKV(*[torch.randint(-127, 128, (B, 4, n, 128), dtype=torch.int8, generator=g).to(DEV) for _ in range(2)],
+                         *[torch.rand(B, 4, n, generator=g).div(60).to(DEV) for _ in range(2)])
+        q = torch.randn(B * rows, 16, 128, generator=g).bfloat16().to(DEV)
+        seq = torch.arange(B, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+        pos = torch.arange(n - rows, n, dtype=torch.int32, device=DEV).repeat(B)
+        calls.append(lambda kv=kv, q=q, seq=seq, pos=pos, rows=rows, n=n, form=form: ops.attention_q8(
+            q, kv, pos, True, n, row_seq=seq, seq_rows=rows, form=form, key_chunk=512))
+    alone = [f() for f in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, f in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append([f() for _ in range(3)])
+        torch.cuda.synchronize()
+        for a, outs in zip(alone, got):
+            assert all(torch.equal(a, x) for x in outs)
+    assert ops.device_error() == 0
