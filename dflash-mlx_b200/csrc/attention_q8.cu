@@ -674,8 +674,11 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // 4096 keys 28 us (tc 36), at 1024 27 (16); 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256,
 // 46 us (tc 55).
 // Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for
-// several runs (warp form: that have four and more), as their lengths may differ (those 8 sequences in tc: 55 us
-// with it, 71 without). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
+// several runs (warp form: that have four and more; tc: unless it makes them two where the CTAs nearly fill the
+// wave), as their lengths may differ (those 8 sequences in tc: 55 us with it, 71 without). Runs of one chunk in the
+// warp form and half to 1.35 waves: long ones are cut so that their rest fills the SMs at the end, in halves up to
+// 0.8 waves (single tokens of 36 sequences of 512 to 4096 keys 56 -> 45 us, all of 4096 76 -> 67), at three quarters
+// beyond (64 sequences 72 -> 64, all of 4096 117 -> 104; 52 of 4096 82 -> 86). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
 // keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and
 // 8.0, with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05 forms 512, and no split of 512 keys where half
 // the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6).
@@ -697,10 +700,12 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
   p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? small : want <= 32 || hd == 256 ? 32 : 64;
   if (key_chunk <= 0) {
     const long long slots = tc ? 148 * (p.rows == 64 && hd < 256 ? 2 : 1) : p.rows == 64 ? 148 : wave, u = units(p.rows);
-    long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 : slots >= 4 * u) ? 1 : 0);
+    long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 && 4 * slots >= 5 * u : slots >= 4 * u) ? 1 : 0);
     if (!tc && u > 74 && max_kv <= 512) n = 1;
     const long long lo = tc ? 512 : max_kv <= 8 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
     long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
+    if (!tc && n <= 1 && runs > 1 && max_kv >= 2048 && 20 * u <= 27 * slots)
+      c = 5 * u <= 4 * slots ? (max_kv + 1) / 2 : (3LL * max_kv + 3) / 4;
     c = c < lo ? lo : c > 8192 ? 8192 : c;
     key_chunk = (int)((c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT);
   }
