@@ -665,23 +665,25 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // The form, tile rows and keys per chunk of a call.
 // Few: runs of at most 16 (token, head) rows, and calls small enough that tiles of 16 rows with 384 keys each
 // fit one wave (three CTAs an SM; at head_dim 256 one, of 32 rows where there are more than 16). They take the
-// warp form in such tiles, for their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128, 10.3 us when
-// chosen (64-row tiles 15.2, tcgen05 16.2), 9.4 since Q is loaded beside the positions; 4096 keys 16.0 (20.5, 16.5),
-// now 14.9. Others take a tcgen05 form, tc of 64 rows a
-// CTA: four such sequences of 2048 keys 18.3 us (16-row tiles 28.5, 64-row 21.3), 64 of 512 to 4096 keys 119
-// (338 in 64-row tiles); 64 single tokens 107, in the warp form 66 (now 63). Wide, of 256 rows (head_dim 256: 128), for
-// runs that fill more than half of them and calls with a CTA, or 384 keys, for every SM: 128 rows of 32 heads at
-// 4096 keys 28 us (tc 36), at 1024 27 (16); 8 sequences of 512 to 6000 keys, 16 tokens of 24 heads of 256,
-// 46 us (tc 55).
+// warp form in such tiles, for their latency: one sequence of 1024 keys, 16 tokens of 32 heads of 128, 10.3 us
+// when chosen (64-row tiles 15.2, tcgen05 16.2), 9.4 since Q is loaded beside the positions; 4096 keys 16.0
+// (20.5, 16.5), now 14.9.
+// Others take a tcgen05 form, tc of 64 rows a CTA: four such sequences of 2048 keys 18.3 us (16-row tiles 28.5,
+// 64-row 21.3), 64 of 512 to 4096 keys 119 (338 in 64-row tiles); 64 single tokens 107, in the warp form 61.
+// Wide, of 256 rows (head_dim 256: 128), for runs that fill more than half of them and calls with a CTA, or 384
+// keys, for every SM: 128 rows of 32 heads at 4096 keys 28 us (tc 36), at 1024 27 (16); 8 sequences of 512 to
+// 6000 keys, 16 tokens of 24 heads of 256, 46 us (tc 55). Also where tc would take a second wave (25
+// sequences of 51 keys, 16 tokens of 32 heads of 256: 15 us, tc 22; 48 of 99, 82 tokens of 8 heads of 64: 14, 20).
 // Chunks: as many as keep every CTA in one wave (tc: two an SM, at head_dim 256 and wide one), one more for
 // several runs (warp form: that have four and more; tc: unless it makes them two where the CTAs nearly fill the
-// wave), as their lengths may differ (those 8 sequences in tc: 55 us with it, 71 without). Runs of one chunk in the
-// warp form and half to 1.35 waves: long ones are cut so that their rest fills the SMs at the end, in halves up to
-// 0.8 waves (single tokens of 36 sequences of 512 to 4096 keys 56 -> 45 us, all of 4096 76 -> 67), at three quarters
-// beyond (64 sequences 72 -> 64, all of 4096 117 -> 104; 52 of 4096 82 -> 86). One chunk needs no merge, and each costs the merge and its CTA's start: at least 128
-// keys, 256 where those make more than 8 chunks (one token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and
-// 8.0, with 16 tokens and a cold L2 18.4 and 20.5), in the tcgen05 forms 512, and no split of 512 keys where half
-// the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6).
+// wave), as their lengths may differ (those 8 sequences in tc: 55 us with it, 71 without). Runs of one chunk in
+// the warp form and half to 1.35 waves: long ones are cut so that their rest fills the SMs at the end, in halves
+// up to 0.8 waves (single tokens of 36 sequences of 512 to 4096 keys 55 -> 45 us, all of 4096 76 -> 72), at three
+// quarters beyond (64 sequences 72 -> 64, all of 4096 117 -> 104; 52 of 4096 82 -> 86). One chunk needs no merge,
+// and each costs the merge and its CTA's start: at least 128 keys, 256 where those make more than 8 chunks (one
+// token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and 8.0, with 16 tokens and a cold L2 18.4 and 20.5),
+// in the tcgen05 forms 512, at most 64 chunks (one kv head, 2 tokens at 48k keys: 15 us, in 190 chunks 24), and no
+// split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6).
 struct Q8Plan {
   int form, rows, key_chunk, n_chunks;  // rows: (token, head) pairs a CTA takes
 };
@@ -692,16 +694,18 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
   const int small = hd == 256 && want > 16 ? 32 : 16;
   const bool few = want <= 16 || (units(small) <= wave && units(small) * max_kv <= wave * 384);
   const int wide = hd == 256 ? 128 : 256;
-  p.form = form != DFL_Q8_AUTO                                              ? form
-           : few                                                          ? DFL_Q8_WARP
-           : want > wide / 2 && units(wide) * (max_kv < 384 ? 384 : max_kv) >= 148 * 384LL ? DFL_Q8_WIDE
-                                                                          : DFL_Q8_TC;
+  const long long tc_wave = 148 * (hd == 256 ? 1 : 2);
+  const bool busy = units(wide) * (max_kv < 384 ? 384 : max_kv) >= 148 * 384LL || units(64) > tc_wave;
+  if (form != DFL_Q8_AUTO) p.form = form;
+  else if (few) p.form = DFL_Q8_WARP;
+  else p.form = want > wide / 2 && busy ? DFL_Q8_WIDE : DFL_Q8_TC;
   const bool tc = p.form >= DFL_Q8_TC;
   p.rows = p.form == DFL_Q8_WIDE ? wide : tc ? 64 : few ? small : want <= 32 || hd == 256 ? 32 : 64;
   if (key_chunk <= 0) {
-    const long long slots = tc ? 148 * (p.rows == 64 && hd < 256 ? 2 : 1) : p.rows == 64 ? 148 : wave, u = units(p.rows);
+    const long long slots = tc ? (p.rows == 64 ? tc_wave : 148) : p.rows == 64 ? 148 : wave, u = units(p.rows);
     long long n = slots / u + (runs > 1 && (tc ? slots % u != 0 && 4 * slots >= 5 * u : slots >= 4 * u) ? 1 : 0);
     if (!tc && u > 74 && max_kv <= 512) n = 1;
+    if (n > 64) n = 64;
     const long long lo = tc ? 512 : max_kv <= 8 * Q8_CHUNK_UNIT ? Q8_CHUNK_UNIT : 256;
     long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
     if (!tc && n <= 1 && runs > 1 && max_kv >= 2048 && 20 * u <= 27 * slots)
