@@ -18,11 +18,11 @@
 // issues the MMAs. The converters load codes straight into registers, one block ahead of the one they convert.
 // What bounds it is the chain of these roles, not one unit (64 blocks of 16, 512 to 4096 keys: 119 us, 44 % of
 // the copy rate; at 130 us leaving out the softmax arithmetic gave 108, the MMAs 113, the loads 122; issue slots
-// are 46 % busy). A block's softmax takes about 1200 clocks, and the issuing thread, at 58 clocks an MMA, 80 a commit and
-// 130 a wait even for a barrier that is complete, nearly as many: it has one wait and two commits a
-// block (with a barrier for each tile: 130 instead of 124 us, wide 129 instead of 111). A CTA's start and end, 12000 clocks
-// (18000 with one row after the other in the Q conversion and the epilogue, and Q loaded behind the positions;
-// 124 us, wide 111), are each a chain of latencies: several rows side by side.
+// are 46 % busy). A block's softmax takes about 1200 clocks, and the issuing thread, at 58 clocks an MMA, 80 a
+// commit and 130 a wait even for a barrier that is complete, nearly as many: it has one wait and two commits a
+// block (with a barrier for each tile: 130 instead of 124 us, wide 129 instead of 111). A CTA's start and end,
+// 12000 clocks, are a chain of latencies too, with several rows side by side (one row after the other, and Q loaded
+// behind the positions: 18000 clocks, 124 us).
 // A row's exponent base M follows its maximum lazily: sums, weights and O are rescaled only when
 // M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to 2^-18 of
 // the largest keep all their bits (those below are rounded to multiples of 2^-28 of it).
