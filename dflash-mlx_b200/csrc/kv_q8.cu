@@ -69,8 +69,9 @@ int q8_cache(const dfl_kv_q8* c, const char* who, Q8Cache* out) {
 // With many rows the issue of instructions bounds it before memory does, so a lane of the rotated dims holds four
 // values of the first half and their partners of the second (the rotation needs no other lane), the arithmetic
 // runs two values an instruction, and slots of q heads alone have a loop of their own. 16384 rows of
-// 32 + 16 heads of 128, int8: 80 us, 4.6 TB/s (eight consecutive values a lane, partners by shuffle, one value an
-// instruction, one slot in flight: 135 us; the lane layout and pairs alone: 111; the ring: 97; the q loop: 80).
+// 32 + 16 heads of 128, int8: 84 us, 4.4 TB/s (eight consecutive values a lane, partners by shuffle, one value an
+// instruction, one slot in flight: 135 us; the lane layout and pairs alone: 111; the ring: 97; the q loop: 80; codes
+// that are right at a half, two more instructions for four values: 84).
 // ---------------------------------------------------------------------------
 struct AppendQ8Args {
   const __nv_bfloat16* qkv;
@@ -103,11 +104,13 @@ __device__ __forceinline__ float2 rope_cos_sin(int p, float f) {
   return make_float2(c, s);
 }
 
-// Codes of four values x * up, rounded to nearest even: int8 by an addition of 1.5 * 2^23, whose sum's low
-// byte is the integer (|x * up| <= 127 up to rounding, so none is out of range).
+// Codes of four values x * (up + lo), rounded to nearest even: int8 by an addition of 1.5 * 2^23, whose sum's low
+// byte is the integer (|x * up| <= 127 up to rounding, so none is out of range). lo is what up leaves out of
+// TOP / max|x|: bf16 values meet halves of a code often (half of an int8 row's maximum is code 63.5, three quarters
+// of an e4m3 row's 336), and up's rounding alone would push one product in two off its half.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t q8_codes4(uint64_t x01, uint64_t x23, uint64_t up) {
-  const uint64_t y01 = q8_mul2(x01, up), y23 = q8_mul2(x23, up);
+__device__ __forceinline__ uint32_t q8_codes4(uint64_t x01, uint64_t x23, uint64_t up, uint64_t lo) {
+  const uint64_t y01 = q8_fma2(x01, up, q8_mul2(x01, lo)), y23 = q8_fma2(x23, up, q8_mul2(x23, lo));
   if constexpr (E4M3) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(q8_unpack(y01), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(q8_unpack(y23), __NV_SATFINITE, __NV_E4M3);
@@ -296,9 +299,10 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS, ROWS == 1 ? 1 : 4) append_q
       const bool some = finite && amax >= 1.5046328e-36f;
       const float up = some ? __fdiv_rn(TOP, amax) : 0.f;
       const float scale = finite ? (some ? __fdiv_rn(amax, TOP) : 0.f) : __uint_as_float(0x7fc00000u);
-      const uint64_t up2 = q8_pack(up, up);
-      const uint32_t c0 = some ? q8_codes4<E4M3>(x[0], x[1], up2) : 0u;
-      const uint32_t c1 = some ? q8_codes4<E4M3>(x[2], x[3], up2) : 0u;
+      const float lo = fmaf(-up, amax, TOP) * (up * (1.f / TOP));  // the remainder is exact, 1 / amax near enough
+      const uint64_t up2 = q8_pack(up, up), lo2 = q8_pack(lo, lo);
+      const uint32_t c0 = some ? q8_codes4<E4M3>(x[0], x[1], up2, lo2) : 0u;
+      const uint32_t c1 = some ? q8_codes4<E4M3>(x[2], x[3], up2, lo2) : 0u;
       const int kh = h - a.Hq - (is_k ? 0 : Hkv);
       unsigned char* codes = (is_k ? a.c.k : a.c.v) + code0 + kh * a.c.head_stride;
       *reinterpret_cast<uint32_t*>(codes + d0) = c0;
