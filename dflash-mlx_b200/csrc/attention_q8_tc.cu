@@ -602,16 +602,17 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     }
     s_ml[threadIdx.x] = make_float2(mu_used, q8_unpack(l).x + q8_unpack(l).y);
     asm volatile("bar.sync 1, %0;\n" ::"n"(SG * 128) : "memory");
-    // a thread a row: the copies' weights, with the quotient where this chunk is the only one, and where it goes
-    // (over the row factors, and the thread's own (M, l), read no more)
+    // a thread a row: the copies' weights, the quotient where this chunk is the only one, and where it goes (over
+    // the row factors, and the thread's own (M, l), read no more)
     long long* s_dst = reinterpret_cast<long long*>(s_rowf);
     long long* s_gate = reinterpret_cast<long long*>(s_ml);
     if (threadIdx.x < ROWS) {
       const int r = threadIdx.x, th = s_row[r], tok = th >> 4;
       const float2 x0 = s_ml[r], x1 = CP == 2 ? s_ml[r + ROWS] : make_float2(-INFINITY, 0.f);
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
-      float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
+      const float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
       const float den = w0 * x0.y + w1 * x1.y;
+      float inv = 1.f;
       long long dst = -1, gate = 0;  // where the row of the output (or of the partials) begins, and its gate's
       if (ok && th >= 0 && s_tok_ok[tok] && (a.n_chunks == 1 || lim > k_begin)) {
         const long long m = m0 + tok, head = kvh * a.G + (th & 15);
@@ -620,14 +621,12 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
           a.part_ml[to] = make_float2(mm, den);
           dst = to * HD;
         } else {
-          const float inv = lim > 0 ? Q8_SUM_UNIT / den : 0.f;
-          w0 *= inv;
-          w1 *= inv;
+          inv = lim > 0 ? Q8_SUM_UNIT / den : 0.f;
           dst = m * a.ldo + head * HD;
           gate = m * a.ldg + head * a.gate_hs;
         }
       }
-      s_w[r] = make_float4(w0, w1, lim > 0 ? 1.f : 0.f, 0.f);
+      s_w[r] = make_float4(w0, w1, lim > 0 ? 1.f : 0.f, inv);
       s_dst[r] = dst;
       s_gate[r] = gate;
     }
@@ -640,11 +639,13 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
 #pragma unroll 1
     for (int r0 = warp * RPW + lane / (32 / RPW); r0 < n_rows; r0 += NR * STEP) {
       float4 y[NR][NC];
+      float inv[NR];
       long long dst[NR];
 #pragma unroll
       for (int u = 0; u < NR; ++u) {
         const int r = min(r0 + u * STEP, ROWS - 1);
         const float4 w = s_w[r];
+        inv[u] = w.w;
         dst[u] = r0 + u * STEP < n_rows ? s_dst[r] : -1;
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -666,6 +667,17 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
             if (dst[u] >= 0) *reinterpret_cast<float4*>(a.part_o + dst[u] + (c0 + 32 * k) * 4) = y[u][k];
         continue;
       }
+      // The copies' sum first, then the quotient, as the merge kernel has it (its sum starts at +0, so that no zero
+      // is negative): a row whose keys lie in the first chunk has the same bits in calls of one chunk and of several.
+#pragma unroll
+      for (int u = 0; u < NR; ++u)
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+          y[u][k].x = (y[u][k].x + 0.f) * inv[u];
+          y[u][k].y = (y[u][k].y + 0.f) * inv[u];
+          y[u][k].z = (y[u][k].z + 0.f) * inv[u];
+          y[u][k].w = (y[u][k].w + 0.f) * inv[u];
+        }
       if (a.gate) {
         uint2 g[NR][NC];
 #pragma unroll

@@ -1,0 +1,35 @@
+"""What the bits of an 8-bit cache's attention do not depend on: the sizes of the call around a row."""
+import pytest
+import torch
+from test_kv_q8_gpu import DEV, Cache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need(lib):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide"])
+@pytest.mark.parametrize("t,Hkv,G,hd,gated", [("int8", 2, 4, 128, False), ("e4m3", 2, 3, 128, True), ("int8", 4, 8, 64, True),
+                                              ("e4m3", 1, 6, 256, False)])
+def test_max_kv_changes_no_bit(form, t, Hkv, G, hd, gated):
+    """One chunk or several: rows whose keys lie in the first give the same bits, signs of zeros among them."""
+    from dflash_b200 import ops
+    B, rows = 24, 16
+    g = torch.Generator().manual_seed(hd + G)
+    lens = [int(n) for n in torch.randint(rows, 513, (B,), generator=g)]
+    lens[0] = 512
+    c = Cache(t, lens, Hkv, hd, 64, seed=G)
+    c.codes[1].view(torch.uint8)[..., 5] = 0x80 if t == "e4m3" else 0  # a dim of negative zeros
+    q = (1.5 * torch.randn(B * rows, Hkv * G, hd, generator=g)).bfloat16().to(DEV)
+    seq = torch.arange(B, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
+    gate = torch.randn(B * rows, Hkv * G * hd, generator=g).bfloat16().to(DEV) if gated else None
+    one, *more = [ops.attention_q8(q, c.kv, pos, True, max_kv, row_seq=seq, seq_rows=rows, form=form, key_chunk=512,
+                                   gate=gate).view(torch.int16) for max_kv in (512, 513, 1024, 5000)]
+    assert ops.device_error() == 0
+    for x in more:
+        assert torch.equal(one, x), int((one != x).sum())
