@@ -26,11 +26,11 @@
 //  * q is scaled by a power of two per row to [2^14, 2^15) at its largest element: every bf16 value
 //    down to 2^-29 of it stays exact in fp16.
 //  * The V scale goes into the weight, w_j = e_j vs_j, which is rounded to fp16 (2^-11 relative).
-//    e_j is taken relative to a base M that follows max x - 4 + log2 of the largest V scale the row has
-//    seen; it is raised, and sums and accumulators rescaled, only when it has fallen behind by more than
-//    10. So w_j < 2^15 whatever the scales are, and weights down to 2^-18 of the largest keep all their
-//    bits (those below are rounded to multiples of 2^-28 of it); the sum of e_j uses the same M, which
-//    cancels in the quotient.
+//    e_j is taken relative to a base M that follows the largest x_j + floor(log2 vs_j) that the row has seen (or up
+//    to 4 more: attention_q8.cuh), less 4; it is raised, and sums and accumulators rescaled, only when it has fallen
+//    behind by more than 10. So w_j < 2^15 whatever the scales are, and weights down to 2^-14 of the largest keep all
+//    their bits, down to 2^-18 where the V scales are alike (those below are rounded to multiples of 2^-24, of 2^-28
+//    of it); the sum of e_j uses the same M, which cancels in the quotient.
 // Rows' statistics, sums and accumulators are fp32. Masked keys are selected away (their scales
 // and query products may be anything), so infinities and NaN there do not reach the row; codes are
 // numbers (a weight of 0 times e4m3's NaN code would not be 0; the append writes none).
@@ -63,7 +63,7 @@ __device__ __forceinline__ int q8_swz(int r, int c) {
 template <int HD, int MT, int RG, int ST>
 struct AttnQ8Layout {
   static constexpr int ROWS = 16 * MT * RG;
-  static constexpr int STAGE = 2 * Q8_KB * HD + 2 * Q8_KB * 4;
+  static constexpr int STAGE = 2 * Q8_KB * HD + 3 * Q8_KB * 4;  // K and V codes; K scales, V scales, V exponents
   static constexpr int RING = Q8_STRANDS * ST * STAGE;
   static constexpr int MERGE = Q8_STRANDS * ROWS * HD * 4 + Q8_STRANDS * ROWS * 8;
   static constexpr int BASE = RING > MERGE ? RING : MERGE;  // the merge reuses the ring
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
   __syncthreads();
 
   const int r0 = rg * MT * 16;  // this warp's rows: r0 + mt * 16 + g (+ 8)
-  float rowf[MT][2], Mr[MT][2], mrow[MT][2], lrow[MT][2];
-  int lim[MT][2], er[MT][2];
+  float rowf[MT][2], Mr[MT][2], mrow[MT][2], lrow[MT][2];  // mrow: largest x_j + exponent of vs_j
+  int lim[MT][2];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -272,7 +272,6 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
       lim[mt][h] = s_lim[r0 + mt * 16 + g + 8 * h];
       mrow[mt][h] = Mr[mt][h] = -INFINITY;
       lrow[mt][h] = 0.f;
-      er[mt][h] = Q8_ER_MIN;
     }
   float o[MT][2 * NC][4];
 #pragma unroll
@@ -292,9 +291,9 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
     sync_strand();  // block i is there for every warp of the strand; the stage refilled below was read last time
     if (i + ST - 1 < my_n) load(i + ST - 1);
     cp_async_commit();
-    const unsigned char* sK = ring + (i % ST) * L::STAGE;
+    unsigned char* sK = ring + (i % ST) * L::STAGE;
     const unsigned char* sV = sK + Q8_KB * HD;
-    const float* sc = reinterpret_cast<const float*>(sK + 2 * Q8_KB * HD);
+    float* sc = reinterpret_cast<float*>(sK + 2 * Q8_KB * HD);
     const int kb = k_begin + (strand + i * Q8_STRANDS) * Q8_KB;
     const bool full = kb + Q8_KB <= lim_min;  // every row with keys sees the whole block
 
@@ -334,10 +333,12 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
         ks[j] = *reinterpret_cast<const float2*>(sc + j * 8 + 2 * t);
         vs[j] = *reinterpret_cast<const float2*>(sc + Q8_KB + j * 8 + 2 * t);
       }
-      uint32_t vmax_all = 0;
-      if (FULL) {
-        const uint32_t b = __float_as_uint(sc[Q8_KB + lane]) & 0x7fffffffu;
-        vmax_all = __reduce_max_sync(0xffffffffu, b < 0x7f800000u ? b : 0u);
+      const int e = q8_exponent(sc[Q8_KB + lane]);
+      const int e_max = __reduce_max_sync(0xffffffffu, e);
+      const bool near = e_max - __reduce_min_sync(0xffffffffu, e) <= Q8_NEAR;
+      if (!FULL || !near) {
+        sc[2 * Q8_KB + lane] = (float)e;  // by every warp of the strand alike
+        __syncwarp();
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -346,7 +347,6 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
         for (int h = 0; h < 2; ++h) {
           const int lm = lim[mt][h];
           float mx = -INFINITY;
-          uint32_t vm = vmax_all;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kb + j * 8 + 2 * t;
@@ -354,25 +354,26 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
             if (!FULL) {
               t0 = key < lm ? t0 : -INFINITY;
               t1 = key + 1 < lm ? t1 : -INFINITY;
-              const uint32_t v0 = __float_as_uint(vs[j].x) & 0x7fffffffu, v1 = __float_as_uint(vs[j].y) & 0x7fffffffu;
-              if (key < lm && v0 < 0x7f800000u) vm = max(vm, v0);
-              if (key + 1 < lm && v1 < 0x7f800000u) vm = max(vm, v1);
             }
             s[mt][j][2 * h] = t0;
             s[mt][j][2 * h + 1] = t1;
             mx = fmaxf(mx, fmaxf(t0, t1));
           }
+          mx = __fmaf_rn(mx, rowf[mt][h], (float)e_max);
+          if (!FULL || !near) {
+            float z = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 ex = *reinterpret_cast<const float2*>(sc + 2 * Q8_KB + j * 8 + 2 * t);
+              z = fmaxf(z, fmaxf(__fmaf_rn(s[mt][j][2 * h], rowf[mt][h], ex.x),
+                                 __fmaf_rn(s[mt][j][2 * h + 1], rowf[mt][h], ex.y)));
+            }
+            if (!near || kb + Q8_KB > lm) mx = z;
+          }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (!FULL) {
-            vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-            vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
-          }
-          const float mn = fmaxf(mrow[mt][h], mx * rowf[mt][h]);
-          const int en = max(er[mt][h], (int)(vm >> 23) - 127);
-          mrow[mt][h] = mn;
-          er[mt][h] = en;
-          const float Mn = mn + ((float)en - Q8_BASE);  // -inf while the row has seen no key
+          mrow[mt][h] = fmaxf(mrow[mt][h], mx);
+          const float Mn = mrow[mt][h] - Q8_BASE;  // -inf while the row has seen no key
           const bool grow = Mn > Mr[mt][h] + Q8_LAZY || (Mr[mt][h] == -INFINITY && Mn > -INFINITY);
           fac[h] = grow ? q8_exp2(Mr[mt][h] - Mn) : 1.f;
           if (grow) Mr[mt][h] = Mn;

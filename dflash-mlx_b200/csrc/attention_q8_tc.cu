@@ -23,9 +23,9 @@
 // block (with a barrier for each tile: 130 instead of 124 us, wide 129 instead of 111). A CTA's start and end,
 // 12000 clocks, are a chain of latencies too, with several rows side by side (one row after the other, and Q loaded
 // behind the positions: 18000 clocks, 124 us).
-// A row's exponent base M follows its maximum lazily: sums, weights and O are rescaled only when
-// M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to 2^-18 of
-// the largest keep all their bits (those below are rounded to multiples of 2^-28 of it).
+// A row's exponent base M follows its largest weight (score plus exponent of the V scale) lazily: sums, weights and
+// O are rescaled only when M would grow by more than 10 (log2), so weights stay below 2^15 in fp16, and those down to
+// 2^-14 of the largest keep all their bits (attention_q8.cuh).
 // Every wait is bounded (device error 350-359).
 #include "attention_q8.cuh"
 #include "tcgen05.cuh"
@@ -45,8 +45,9 @@ struct QtLayout {
   static constexpr int OFF_K = 0;               // 2 stages
   static constexpr int OFF_V = 2 * TILE;        // 2 stages
   static constexpr int OFF_Q = 4 * TILE;        // [group][units][128 rows][128 B]; the epilogue reuses K, V and Q for O
-  static constexpr int OFF_S = OFF_Q + SG * 128 * HD * 2;  // scales [4][2][64], largest V scales [4][2]
-  static constexpr int OFF_R = OFF_S + QT_SCALES * (2 * QT_KB + 4) * 4;  // row factor, limit, (M, l) of all copies, output weights
+  static constexpr int OFF_S = OFF_Q + SG * 128 * HD * 2;  // [4][64]: K scales, V scales, V exponents
+  static constexpr int OFF_E = OFF_S + QT_SCALES * 3 * QT_KB * 4;  // [4][2]: largest, smallest V exponent of 32 keys
+  static constexpr int OFF_R = OFF_E + QT_SCALES * 16;             // row factor, limit, (M, l) of all copies, output weights
   static constexpr int OFF_BAR = OFF_R + ROWS * 8 + SG * 128 * 8 + ROWS * 16;
   static constexpr int N_BAR = 2 + SG * 2 * 3;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
@@ -121,8 +122,8 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float* s_sc = reinterpret_cast<float*>(smem + L::OFF_S);  // [ring][K, V][64]
-  uint32_t* s_vmax = reinterpret_cast<uint32_t*>(s_sc + QT_SCALES * 2 * QT_KB);  // [ring][half], finite scales' bits
+  float* s_sc = reinterpret_cast<float*>(smem + L::OFF_S);  // [ring][K, V, exponents of V][64]
+  float2* s_ve = reinterpret_cast<float2*>(smem + L::OFF_E);  // [ring][half]
   float* s_rowf = reinterpret_cast<float*>(smem + L::OFF_R);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::OFF_R + ROWS * 8);  // [128 SG]
   float4* s_w = reinterpret_cast<float4*>(s_ml + SG * 128);  // [rows]
@@ -312,12 +313,13 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
         continue;
       }
       if (!is_v) {
-        float* sd = sdst + (i & (QT_SCALES - 1)) * 2 * QT_KB;
+        float* sd = sdst + (i & (QT_SCALES - 1)) * 3 * QT_KB;
         sd[0] = ks;
         sd[QT_KB] = vs;
-        const uint32_t v = __float_as_uint(vs) & 0x7fffffffu;  // a warp holds 32 keys
-        const uint32_t vm = __reduce_max_sync(0xffffffffu, v < 0x7f800000u ? v : 0u);
-        if (lane == 0) s_vmax[(i & (QT_SCALES - 1)) * 2 + (ct >> 5)] = vm;
+        const int e = q8_exponent(vs);
+        sd[2 * QT_KB] = (float)e;
+        const int e_max = __reduce_max_sync(0xffffffffu, e), e_min = __reduce_min_sync(0xffffffffu, e);  // of 32 keys
+        if (lane == 0) s_ve[(i & (QT_SCALES - 1)) * 2 + (ct >> 5)] = make_float2((float)e_max, (float)e_min);
       }
       unsigned char* d = dst + s * L::TILE + dst0;
 #pragma unroll
@@ -467,16 +469,15 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
     const int row = threadIdx.x & (ROWS - 1), half = CP == 2 ? threadIdx.x >> 6 : 0;
     const int lim = s_row[row] < 0 ? 0 : s_tok_lim[s_row[row] >> 4];
     const float rowf = s_rowf[row];
-    float m = -INFINITY, mu_used = -INFINITY;
+    float m = -INFINITY, mu_used = -INFINITY;  // m: largest x_j + exponent of vs_j
     uint64_t l = 0;  // two partial sums
-    int er = Q8_ER_MIN;
     bool ok = true;
     // a warp whose 32 rows all lie behind the tile's does nothing: what its lanes hold goes to its own
     // rows of O, which nobody reads
     const int my_blocks = (row & ~31) < n_rows ? n_blocks : 0;
     for (int i = 0; i < my_blocks && ok; ++i) {
       const int s = i & 1;
-      const float* sc = s_sc + (i & (QT_SCALES - 1)) * 2 * QT_KB + half * 32;
+      const float* sc = s_sc + (i & (QT_SCALES - 1)) * 3 * QT_KB + half * 32;
       const int kb = k_begin + i * QT_KB + half * 32;
       ok = qt_wait(&s_full[s], (i >> 1) & 1, 356, a.err);
       if (!__all_sync(0xffffffffu, ok)) {
@@ -497,21 +498,14 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
           x[k / 2 + c + 1] = q8_mul2(q8_pack(sv[2 * c + 2], sv[2 * c + 3]), ks.y);
         }
       }
-      uint32_t vm = s_vmax[(i & (QT_SCALES - 1)) * 2 + half];
-      if (CP == 1) vm = max(vm, s_vmax[(i & (QT_SCALES - 1)) * 2 + 1]);
       if (!full) {
-        vm = 0;
 #pragma unroll
         for (int c = 0; c < KT / 2; ++c) {
           const float2 y = q8_unpack(x[c]);
-          const bool seen0 = kb + 2 * c < lim, seen1 = kb + 2 * c + 1 < lim;
-          x[c] = q8_pack(seen0 ? y.x : -INFINITY, seen1 ? y.y : -INFINITY);
-          const uint2 v = *reinterpret_cast<const uint2*>(sc + QT_KB + 2 * c);
-          const uint32_t v0 = v.x & 0x7fffffffu, v1 = v.y & 0x7fffffffu;
-          if (seen0 && v0 < 0x7f800000u) vm = max(vm, v0);
-          if (seen1 && v1 < 0x7f800000u) vm = max(vm, v1);
+          x[c] = q8_pack(kb + 2 * c < lim ? y.x : -INFINITY, kb + 2 * c + 1 < lim ? y.y : -INFINITY);
         }
       }
+      const uint64_t rf2 = q8_pack(rowf, rowf);
       float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
       for (int c = 0; c < KT / 2; c += 2) {
@@ -519,9 +513,26 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
         mx0 = fmaxf(fmaxf(mx0, y.x), y.y);
         mx1 = fmaxf(fmaxf(mx1, z.x), z.y);
       }
-      m = fmaxf(m, fmaxf(mx0, mx1) * rowf);
-      er = max(er, (int)(vm >> 23) - 127);
-      const float M = m + ((float)er - Q8_BASE);
+      float2 ve = s_ve[(i & (QT_SCALES - 1)) * 2 + half];
+      if (CP == 1) {
+        const float2 other = s_ve[(i & (QT_SCALES - 1)) * 2 + 1];
+        ve = make_float2(fmaxf(ve.x, other.x), fminf(ve.y, other.y));
+      }
+      const bool near = ve.x - ve.y <= (float)Q8_NEAR;
+      float mx = __fmaf_rn(fmaxf(mx0, mx1), rowf, ve.x);
+      if (!full || !near) {
+        mx0 = mx1 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < KT / 2; c += 2) {
+          const ulonglong2 ex = *reinterpret_cast<const ulonglong2*>(sc + 2 * QT_KB + 2 * c);
+          const float2 y = q8_unpack(q8_fma2(x[c], rf2, ex.x)), z = q8_unpack(q8_fma2(x[c + 1], rf2, ex.y));
+          mx0 = fmaxf(fmaxf(mx0, y.x), y.y);
+          mx1 = fmaxf(fmaxf(mx1, z.x), z.y);
+        }
+        if (!near || kb + KT > lim) mx = fmaxf(mx0, mx1);
+      }
+      m = fmaxf(m, mx);
+      const float M = m - Q8_BASE;
       const bool grow = M > mu_used + Q8_LAZY || (mu_used == -INFINITY && M > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
         const float fac = grow ? q8_exp2(mu_used - M) : 1.f;
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
         }
       }
       const float mu = mu_used == -INFINITY ? 0.f : mu_used;
-      const uint64_t rf2 = q8_pack(rowf, rowf), mu2 = q8_pack(-mu, -mu), unit2 = q8_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
+      const uint64_t mu2 = q8_pack(-mu, -mu), unit2 = q8_pack(Q8_SUM_UNIT, Q8_SUM_UNIT);
       const uint32_t t_w = tmem + lane_base + (uint32_t)(s * 64);
 #pragma unroll
       for (int k = 0; k < KT; k += 32) {

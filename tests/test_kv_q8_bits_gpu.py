@@ -33,3 +33,25 @@ def test_max_kv_changes_no_bit(form, t, Hkv, G, hd, gated):
     assert ops.device_error() == 0
     for x in more:
         assert torch.equal(one, x), int((one != x).sum())
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide"])
+@pytest.mark.parametrize("t,G,hd", [("int8", 4, 128), ("e4m3", 6, 256), ("int8", 2, 64)])
+def test_rows_alone_and_together_over_scales_far_apart(form, t, G, hd):
+    """Blocks of keys whose V scales are near one another beside blocks where they are not, cut by rows' limits: the
+    base of a row's weights is its own."""
+    from dflash_b200 import ops
+    lens, rows, Hkv = [700, 90, 333], 40, 2
+    c = Cache(t, lens, Hkv, hd, 64, seed=8)
+    g = torch.Generator().manual_seed(8)
+    shape = c.scale.shape[1:]
+    far = 2.0 ** torch.randint(-40, 40, shape, generator=g) * (torch.rand(shape, generator=g) < 0.01)
+    c.scale[1] *= torch.where(far > 0, far, torch.ones(shape)).to(DEV)
+    q = (1.5 * torch.randn(len(lens) * rows, Hkv * G, hd, generator=g)).bfloat16().to(DEV)
+    seq = torch.arange(len(lens), dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
+    kw = dict(causal=True, max_kv=700, form=form, key_chunk=256)
+    whole = ops.attention_q8(q, c.kv, pos, row_seq=seq, seq_rows=rows, **kw)
+    alone = ops.attention_q8(q, c.kv, pos, row_seq=seq, seq_rows=1, **kw)
+    assert ops.device_error() == 0 and whole.isfinite().all()
+    assert torch.equal(whole, alone), int((whole != alone).sum())

@@ -1,0 +1,83 @@
+"""attention_q8 over V scales far apart."""
+import pytest
+import torch
+from test_kv_q8_gpu import DEV, TOP, Cache
+
+pytestmark = pytest.mark.gpu
+FORMS = [("warp", 128), ("tc", 128), ("wide", 128)]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need(lib):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def _reference(q, k, v, scale):
+    """(o, tolerance) of rows that see all keys: q [M, H, hd], k, v [n, hd] in 64 bits."""
+    n, hd = v.shape
+    x = q.double() @ k.T * scale
+    p = torch.softmax(x, -1)
+    o, A = p @ v, p @ v.abs()
+    smax = (q.double().abs() @ k.abs().T * abs(scale)).amax()
+    # fp16's lower end: the largest weight p_j vs_j is held as 1 at least, the others as multiples of 2^-24 there:
+    # off by at most 2^-25 of the largest each, times codes of at most TOP, whose product with vs_j is max |v_j|
+    low = n * 2.0 ** -25 * (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+    # the other terms as in test_kv_q8_gpu.py: the output's bf16, the weights' fp16, scores and sums in fp32
+    return o, 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18 + 2 * hd * 2.0 ** -23 * smax) * A + low
+
+
+def _case(t, n, hd, seed):
+    c = Cache(t, [n], 1, hd, seed=seed, slack=0)
+    g = torch.Generator().manual_seed(seed)
+    q = (1.5 * torch.randn(4, 4, hd, generator=g)).bfloat16()
+    return c, q
+
+
+def _run(c, q, n, form, chunk):
+    from dflash_b200 import ops
+    out = ops.attention_q8(q.to(DEV), c.kv, torch.full((q.shape[0],), n - 1, dtype=torch.int32, device=DEV), True, n,
+                           form=form, key_chunk=chunk)
+    assert ops.device_error() == 0
+    return out.double().cpu().view(*q.shape)
+
+
+@pytest.mark.parametrize("form,chunk", FORMS + [("warp", 1024), ("tc", 1024), ("wide", 1024)])
+@pytest.mark.parametrize("t,hd", [("int8", 128), ("e4m3", 64), ("int8", 256)])
+@pytest.mark.parametrize("at", [0, 37, 600])
+@pytest.mark.parametrize("shift", [24, 30, 60])
+def test_a_key_of_no_weight_and_a_large_value_costs_no_bits(form, chunk, t, hd, at, shift):
+    """A key that the softmax all but leaves out (below 2^-75) but whose V scale is 2^shift times the others':
+    the weights are held relative to the largest product of weight and scale, not of the two maxima."""
+    n = 700
+    c, q = _case(t, n, hd, 21)
+    q = q.abs().clamp_min(0.5)  # every query points one way, the key the other
+    c.codes[0, 0, 0, at] = torch.full((hd,), -TOP[t]).to(c.codes.dtype).to(DEV)
+    c.scale[0, 0, 0, at] = 5 / TOP[t]
+    c.val[0, 0, 0, at] = -TOP[t] * float(c.scale[0, 0, 0, at])
+    c.scale[1, 0, 0, at] *= 2.0 ** shift
+    c.val[1, 0, 0, at] *= 2.0 ** shift
+    k, v = c.val[0, 0, 0, :n], c.val[1, 0, 0, :n]
+    scale = hd ** -0.5
+    p = torch.softmax(q.double() @ k.T * scale, -1)
+    assert float(p[..., at].max()) * 2.0 ** shift < 2.0 ** -10 * float(p.max())  # what it adds is small
+    o, tol = _reference(q, k, v, scale)
+    err = (_run(c, q, n, form, chunk) - o).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("form,chunk", FORMS + [("warp", 1024), ("tc", 1024), ("wide", 1024)])
+@pytest.mark.parametrize("t,hd", [("int8", 128), ("e4m3", 64), ("e4m3", 256)])
+@pytest.mark.parametrize("exps", [(-90, 0), (0, -90), (0, 80)])
+def test_v_scales_far_apart_leave_the_softmax_sum_whole(form, chunk, t, hd, exps):
+    """Halves of the keys whose V scales lie 2^80 and 2^90 apart: the small half adds nothing to the output but its
+    softmax weights still divide it."""
+    n = 512
+    c, q = _case(t, n, hd, 22)
+    for half, e in enumerate(exps):
+        s = slice(half * n // 2, (half + 1) * n // 2)
+        c.scale[1, 0, 0, s] *= 2.0 ** e
+        c.val[1, 0, 0, s] *= 2.0 ** e
+    o, tol = _reference(q, c.val[0, 0, 0, :n], c.val[1, 0, 0, :n], hd ** -0.5)
+    err = (_run(c, q, n, form, chunk) - o).abs()
+    assert (err <= tol).all(), float((err / tol).max())
