@@ -375,7 +375,8 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
           mrow[mt][h] = fmaxf(mrow[mt][h], mx);
           const float Mn = mrow[mt][h] - Q8_BASE;  // -inf while the row has seen no key
           const bool grow = Mn > Mr[mt][h] + Q8_LAZY || (Mr[mt][h] == -INFINITY && Mn > -INFINITY);
-          fac[h] = grow ? q8_exp2(Mr[mt][h] - Mn) : 1.f;
+          const float root = grow ? q8_exp2(0.5f * (Mr[mt][h] - Mn)) : 1.f;
+          fac[h] = root * root;
           if (grow) Mr[mt][h] = Mn;
           const float mu = Mr[mt][h] == -INFINITY ? 0.f : Mr[mt][h];
           float ps = 0.f;
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
             const __half2 w = __floats2half2_rn(w0, w1);
             pf[mt][j >> 1][(j & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&w);
           }
-          lrow[mt][h] = __fmaf_rn(ps, Q8_SUM_UNIT, lrow[mt][h] * fac[h]);
+          lrow[mt][h] = __fmaf_rn(ps, Q8_SUM_UNIT, lrow[mt][h] * root * root);
         }
         if (__any_sync(0xffffffffu, fac[0] != 1.f || fac[1] != 1.f)) {  // a factor of 1 is exact
 #pragma unroll
@@ -472,8 +473,9 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
       float w[Q8_STRANDS], den = 0.f;
 #pragma unroll
       for (int u = 0; u < Q8_STRANDS; ++u) {
-        w[u] = exp2f(ml[u].x - mu);
-        den += w[u] * ml[u].y;
+        const float root = exp2f(0.5f * (ml[u].x - mu));
+        w[u] = root * root;
+        den += root * ml[u].y * root;
       }
       const int m = m0 + tok, head = kvh * a.G + hg;
       const long long base = ((long long)chunk * a.M + m) * a.Hq + head;
@@ -567,8 +569,8 @@ __global__ void __launch_bounds__(256) attn_q8_merge_kernel(const __grid_constan
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   for (int c0 = 0; c0 < nch; c0 += 32) {
     if (c0 > 0) x = c0 + lane < nch ? ml[(c0 + lane) * cstride] : make_float2(-INFINITY, 0.f);
-    const float w = exp2f(x.x - mu);
-    den += warp_sum(w * x.y);
+    const float root = exp2f(0.5f * (x.x - mu)), w = root * root;
+    den += warp_sum(root * x.y * root);
     const int n = min(32, nch - c0);
     for (int j0 = 0; j0 < n; j0 += FL) {
       if (c0 + j0 > 0) fetch(c0 + j0);

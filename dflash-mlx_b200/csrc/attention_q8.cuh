@@ -11,6 +11,9 @@ namespace dfl {
 // its scale's exponent: that counts as Q8_EXP_MIN at least (V scales below 2^-104 are the first to lose bits), and the
 // sums of e_j are kept in units of 2^16, so that with V scales up to 2^90 neither they nor the weights leave fp32's
 // normal range, over 2^20 keys and more.
+// Two bases may so lie more than 2^126 apart with sums that count alike (a key of weight 1/2 and V scale 2^-90, then
+// one of 2^80): sums are rescaled by the root of the factor twice, at every place where they are. For weights and
+// accumulators a factor below fp32's range may be 0.
 // In a block of keys whose exponents lie within Q8_NEAR of one another the maximum of the x_j plus the largest
 // exponent stands for that maximum, at most Q8_NEAR above it. Rows that see the whole of such a block take it, all
 // others the exact one: a rule on the row's own keys. (Exact in every block, 64 x 16 rows of 32 heads take 127 us in

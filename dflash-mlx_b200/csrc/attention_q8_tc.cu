@@ -535,9 +535,9 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
       const float M = m - Q8_BASE;
       const bool grow = M > mu_used + Q8_LAZY || (mu_used == -INFINITY && M > -INFINITY);
       if (__any_sync(0xffffffffu, grow)) {  // a factor of 1 is exact
-        const float fac = grow ? q8_exp2(mu_used - M) : 1.f;
+        const float root = grow ? q8_exp2(0.5f * (mu_used - M)) : 1.f, fac = root * root;
         if (grow) mu_used = M;
-        l = q8_mul2(l, q8_pack(fac, fac));
+        l = q8_mul2(q8_mul2(l, q8_pack(root, root)), q8_pack(root, root));
         if (i > 0) {
           ok = qt_wait(&pv_done[2 * grp + ((i - 1) & 1)], ((i - 1) >> 1) & 1, 357, a.err);
           if (!__all_sync(0xffffffffu, ok)) {
@@ -621,8 +621,8 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
       const int r = threadIdx.x, th = s_row[r], tok = th >> 4;
       const float2 x0 = s_ml[r], x1 = CP == 2 ? s_ml[r + ROWS] : make_float2(-INFINITY, 0.f);
       const float mm = fmaxf(x0.x, x1.x), mu = mm == -INFINITY ? 0.f : mm;
-      const float w0 = q8_exp2(x0.x - mu), w1 = q8_exp2(x1.x - mu);
-      const float den = w0 * x0.y + w1 * x1.y;
+      const float r0 = q8_exp2(0.5f * (x0.x - mu)), r1 = q8_exp2(0.5f * (x1.x - mu)), w0 = r0 * r0, w1 = r1 * r1;
+      const float den = r0 * x0.y * r0 + r1 * x1.y * r1;
       float inv = 1.f;
       long long dst = -1, gate = 0;  // where the row of the output (or of the partials) begins, and its gate's
       if (ok && th >= 0 && s_tok_ok[tok] && (a.n_chunks == 1 || lim > k_begin)) {

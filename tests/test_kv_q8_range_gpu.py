@@ -68,9 +68,9 @@ def test_a_key_of_no_weight_and_a_large_value_costs_no_bits(form, chunk, t, hd, 
 
 @pytest.mark.parametrize("form,chunk", FORMS + [("warp", 1024), ("tc", 1024), ("wide", 1024)])
 @pytest.mark.parametrize("t,hd", [("int8", 128), ("e4m3", 64), ("e4m3", 256)])
-@pytest.mark.parametrize("exps", [(-90, 0), (0, -90), (0, 80)])
+@pytest.mark.parametrize("exps", [(-90, 0), (0, -90), (0, 80), (-60, 70), (70, -60), (-90, 80), (80, -90)])
 def test_v_scales_far_apart_leave_the_softmax_sum_whole(form, chunk, t, hd, exps):
-    """Halves of the keys whose V scales lie 2^80 and 2^90 apart: the small half adds nothing to the output but its
+    """Halves of the keys whose V scales lie 2^80 to 2^170 apart: the small half adds nothing to the output but its
     softmax weights still divide it."""
     n = 512
     c, q = _case(t, n, hd, 22)
