@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
       *reinterpret_cast<__half2*>(sQ + r * HD + ((cc ^ (r & 7)) << 3) + (kp & 7)) = h;
     }
     if (lane == 0) {
-      s_rowf[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
+      s_rowf[r] = q8_row_factor(a.scale_log2, sh);
       s_lim[r] = q_ok[i] ? s_tok_lim[r / a.G] : 0;
     }
   }

@@ -26,6 +26,12 @@ constexpr float Q8_SUM_UNIT = 1.f / 65536.f;
 // oftener: 64 x 16 rows 118 -> 126 us, 8 gated blocks at head_dim 256 50 -> 55.)
 constexpr float Q8_BASE = 4.f, Q8_LAZY = 10.f;
 
+// What a row's products q' . Kc ks are multiplied by to be x_j: the softmax scale and the power of two that q' was
+// scaled by. At least 2^-126, with which the scores of such a row are all alike: 0 times a masked key's -inf is NaN.
+__device__ __forceinline__ float q8_row_factor(float scale_log2, int sh) {
+  return fmaxf(scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23), 1.17549435e-38f);
+}
+
 // floor(log2 |v|) of a V scale, at least Q8_EXP_MIN; Q8_EXP_MIN too for infinities and NaN, whose exponent field
 // becomes 0 when 1 is added
 __device__ __forceinline__ int q8_exponent(float v) {

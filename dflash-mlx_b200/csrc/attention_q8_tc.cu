@@ -454,7 +454,7 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
             *(d0[t] - GR * 8) = h0;  // the first copy, 64 rows of 128 bytes before
             *(d1 - GR * 8) = h1;
           }
-          if (ql == 0) s_rowf[g0 + r + t * 4 * QPW] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
+          if (ql == 0) s_rowf[g0 + r + t * 4 * QPW] = q8_row_factor(a.scale_log2, sh);
         }
       }
     }

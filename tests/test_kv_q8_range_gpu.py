@@ -81,3 +81,24 @@ def test_v_scales_far_apart_leave_the_softmax_sum_whole(form, chunk, t, hd, exps
     o, tol = _reference(q, c.val[0, 0, 0, :n], c.val[1, 0, 0, :n], hd ** -0.5)
     err = (_run(c, q, n, form, chunk) - o).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("form,chunk", FORMS)
+@pytest.mark.parametrize("qs,scale", [(1e-38, 1e-10), (2.0 ** -126, 2.0 ** -60), (1.0, 1e-44)])
+def test_scores_that_vanish_average_the_keys_that_a_row_sees(form, chunk, qs, scale):
+    """Queries and softmax scales so small that their product is below fp32's range: the weights are alike, and keys
+    behind a row's position stay out (0 times their -inf would be NaN)."""
+    from dflash_b200 import ops
+    n, hd = 200, 128
+    c, q = _case("int8", n, hd, 23)
+    q = q.sign() * qs
+    pos = torch.tensor([3, 150, 190, 199], dtype=torch.int32)
+    out = ops.attention_q8(q.bfloat16().to(DEV), c.kv, pos.to(DEV), True, n, form=form, key_chunk=chunk, scale=scale)
+    assert ops.device_error() == 0
+    out = out.double().cpu().view(4, 4, hd)
+    for m, p in enumerate(pos.tolist()):
+        v = c.val[1, 0, 0, :p + 1]
+        o, A = v.mean(0), v.abs().mean(0)
+        # as above, with scores of 0
+        tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18) * A + n * 2.0 ** -25 * v.abs().amax() / (p + 1)
+        assert ((out[m] - o).abs() <= tol).all(), m
