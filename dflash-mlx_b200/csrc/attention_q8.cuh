@@ -91,9 +91,10 @@ __device__ __forceinline__ void q8_to_half(uint32_t w, uint32_t& lo, uint32_t& h
   }
 }
 
-// keys row m sees: clamped to what the cache and the call allow (an excess sets the error word)
+// keys row m sees: clamped to what the cache and the call allow (an excess sets the error word). kv_len from L2: the
+// merge kernel asks before it waits, when this SM's L1 may still hold the entry as an earlier kernel read it.
 __device__ __forceinline__ int q8_row_limit(const AttnQ8Args& a, int m, int p, int seq, int* err) {
-  const long long lim = a.causal ? (long long)p + 1 : a.kv_len[seq];
+  const long long lim = a.causal ? (long long)p + 1 : __ldcg(a.kv_len + seq);
   const int most = min(a.max_kv, a.c.cap);
   if (lim > most) q8_error(err, Q8_ERR_POS);
   return lim > most ? most : lim < 0 ? 0 : (int)lim;

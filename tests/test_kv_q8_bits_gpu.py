@@ -55,3 +55,33 @@ def test_rows_alone_and_together_over_scales_far_apart(form, t, G, hd):
     alone = ops.attention_q8(q, c.kv, pos, row_seq=seq, seq_rows=1, **kw)
     assert ops.device_error() == 0 and whole.isfinite().all()
     assert torch.equal(whole, alone), int((whole != alone).sum())
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide"])
+def test_lengths_that_a_graph_changes_between_its_replays(form):
+    """kv_len, rewritten on the device each step as a draft's is: the merge kernel looks up a row's chunks before it
+    waits for the chunk kernel, and must find the new ones."""
+    from dflash_b200 import ops
+    B, rows, Hkv, G, hd = 8, 4, 2, 4, 128
+    c = Cache("int8", [1200] * B, Hkv, hd, 64, seed=14)
+    g = torch.Generator().manual_seed(14)
+    q = torch.randn(B * rows, Hkv * G, hd, generator=g).bfloat16().to(DEV)
+    seq = torch.arange(B, dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.zeros(B * rows, dtype=torch.int32, device=DEV)
+    kv_len, step = torch.full((B,), 20, dtype=torch.int32, device=DEV), torch.arange(100, 100 + B, dtype=torch.int32, device=DEV)
+    out = torch.zeros(B * rows, Hkv * G * hd, dtype=torch.bfloat16, device=DEV)
+
+    def call(lens, o):
+        return ops.attention_q8(q, c.kv, pos, False, 1200, kv_len=lens, row_seq=seq, seq_rows=rows, form=form, key_chunk=128,
+                                out=o)
+
+    call(kv_len, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv_len.add_(step)
+        call(kv_len, out)
+    for i in range(1, 11):
+        graph.replay()
+        assert torch.equal(out, call(20 + i * step, torch.zeros_like(out))), i
+    assert ops.device_error() == 0
