@@ -10,7 +10,7 @@ import torch
 
 from .adapters import LoadedTargetModel, load_target_model
 from .config import PRESETS
-from .model import DraftModel, kv_dtype as _kv_dtype
+from .model import DraftModel, kv_dtype as _kv_dtype, model_kv_dtype
 from .runtime import dflash_generate, dflash_generate_stream
 from .weights import random_draft_weights
 
@@ -152,6 +152,8 @@ class DFlashGenerator:
             self.draft_quantization = maybe_quantize_draft_model(ckpt, draft_quant_bits, draft_quant_group_size)
             self.draft = ckpt.bind(self.target)
         self.draft.mask_mode = draft_attention_mask
+        for m in (self.target.model, self.draft):
+            model_kv_dtype(m.cfg, kv_dtype)
 
     @property
     def target_model_path(self):

@@ -28,7 +28,7 @@ import torch
 
 from . import ops
 from .config import TargetConfig
-from .model import KVCache, alloc_kv, kv_dtype
+from .model import KVCache, alloc_kv, model_kv_dtype
 from .weights import pack_gate_up, rope_inv_freq
 
 
@@ -129,7 +129,8 @@ class HybridTargetModel:
         if rollback not in ("snapshot", "replay"):
             raise ValueError(f"rollback must be 'snapshot' or 'replay', not {rollback!r}")
         c, dev = self.cfg, self.device
-        kv = alloc_kv(max(1, len(self.attn_index)), batch, c.num_key_value_heads, cap, c.head_dim, dev, kv_dtype(dtype))
+        kv = alloc_kv(max(1, len(self.attn_index)), batch, c.num_key_value_heads, cap, c.head_dim, dev,
+                      model_kv_dtype(c, dtype))
         n = len(self.gdn_index)
         S = (self.Hv, self.Dv, self.Dk)
         Tw = max(block, window_rows)

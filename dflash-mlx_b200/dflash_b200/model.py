@@ -123,6 +123,20 @@ def kv_dtype(name: str) -> torch.dtype:
     return KV_DTYPES[name]
 
 
+def model_kv_dtype(cfg: TargetConfig | DraftConfig, name: str) -> torch.dtype:
+    """kv_dtype() for caches of this model: refuses 8 bits, before anything is allocated or launched, where the 8-bit
+    kernels do not take its heads."""
+    dtype = kv_dtype(name)
+    if dtype != torch.bfloat16:
+        Hq, Hkv, hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        rot = getattr(cfg, "rope_dim", hd)
+        if Hq % Hkv or Hq // Hkv > ops.Q8_MAX_GROUP or hd not in ops.Q8_HEAD_DIMS or rot % 16:
+            raise ValueError(f"kv_dtype {name!r} takes head_dim {ops.Q8_HEAD_DIMS}, at most {ops.Q8_MAX_GROUP} query heads "
+                             f"per kv head and rotary dims in multiples of 16; this model has head_dim {hd}, {Hq} query "
+                             f"and {Hkv} kv heads and {rot} rotary dims")
+    return dtype
+
+
 def _zero_kv(shape: tuple, dtype: torch.dtype, device) -> dict:
     """Zeroed K/V (and, in 8 bits, scales) of the given shape, as KVCache fields."""
     if dtype == torch.bfloat16:
@@ -248,11 +262,11 @@ class TargetModel:
         a paged cache holding pages for those lengths only; in bf16 or 8 bits (``dtype``: "bf16",
         "int8", "e4m3")."""
         c = self.cfg
+        kvt = model_kv_dtype(c, dtype)
         if lengths is not None:
             return alloc_kv_paged(c.num_hidden_layers, lengths, c.num_key_value_heads, c.head_dim, self.device,
-                                  page_table, dtype=kv_dtype(dtype))
-        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device,
-                        kv_dtype(dtype))
+                                  page_table, dtype=kvt)
+        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device, kvt)
 
     def buffers(self, M: int) -> dict[str, torch.Tensor]:
         b = self._bufs.get(M)
@@ -516,11 +530,11 @@ class DraftModel:
     def make_cache(self, batch: int, cap: int, lengths: list[int] | None = None,
                    page_table: torch.Tensor | None = None, dtype: str = "bf16") -> KVCache:
         c = self.cfg
+        kvt = model_kv_dtype(c, dtype)
         if lengths is not None:
             return alloc_kv_paged(c.num_hidden_layers, lengths, c.num_key_value_heads, c.head_dim, self.device,
-                                  page_table, dtype=kv_dtype(dtype))
-        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device,
-                        kv_dtype(dtype))
+                                  page_table, dtype=kvt)
+        return alloc_kv(c.num_hidden_layers, batch, c.num_key_value_heads, cap, c.head_dim, self.device, kvt)
 
     def buffers(self, M: int, kind: str) -> dict[str, torch.Tensor]:
         key = (M, kind)

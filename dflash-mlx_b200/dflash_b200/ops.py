@@ -459,6 +459,7 @@ class KvQ8(ctypes.Structure):
 
 
 Q8_CHUNK = 128  # the unit of attention_q8's key_chunk
+Q8_HEAD_DIMS, Q8_MAX_GROUP = (64, 128, 256), 16  # head_dim and query heads per kv head that the 8-bit kernels take
 Q8_FORMS = {"auto": 0, "warp": 1, "tc": 2, "wide": 3}  # DFL_Q8_AUTO, DFL_Q8_WARP, DFL_Q8_TC, DFL_Q8_WIDE
 KV_Q8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # DFL_KV_INT8, DFL_KV_E4M3
 

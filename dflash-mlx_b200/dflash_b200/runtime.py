@@ -24,7 +24,7 @@ from typing import Any
 import torch
 
 from . import ops
-from .model import DraftModel, TargetModel, kv_dtype as _kv_dtype, q8_split
+from .model import DraftModel, TargetModel, model_kv_dtype, q8_split
 
 STATE_INTS = 16  # sizeof(dfl_seq_state) / 4
 S_START, S_PENDING, S_DRAFT_LEN, S_ACCEPTED, S_BONUS, S_FINISHED, S_STOP, S_STEPS, S_TOTAL, S_PROMPT = range(10)
@@ -119,7 +119,9 @@ class SpecSession:
         self.batched = batch >= 4
         self.key_chunk = 1024 if self.batched else 64
         self.out_cap = self.cap
-        _kv_dtype(kv_dtype)  # refuses an unknown name before anything is allocated
+        for m in (target, draft):  # refuses a name or heads that do not fit before anything is allocated
+            if m is not None:
+                model_kv_dtype(m.cfg, kv_dtype)
         self.kv_dtype = kv_dtype
         # an 8-bit cache's attention: form and keys per split of the steps and of the prefill chunks
         self.step_split, self.prefill_split = {"key_chunk": self.key_chunk}, {"key_chunk": self.key_chunk}
