@@ -625,6 +625,8 @@ def attention_q8(q: torch.Tensor, kv: QuantKV, pos: torch.Tensor, causal: bool, 
         if len(kv._scratch) < 256:
             kv._scratch[sizes] = need
     if ws is not None:
+        if ws.attn.get_device() != idx:
+            raise ValueError(f"the workspace must be one of cuda:{idx}")
         ws.ensure_attn(need)
         scratch, size = ws.attn.data_ptr(), ws.attn.numel()
     else:

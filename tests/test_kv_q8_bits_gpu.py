@@ -1,4 +1,4 @@
-"""What the bits of an 8-bit cache's attention do not depend on: the sizes of the call around a row."""
+"""What the bits of an 8-bit cache's attention do not depend on: the sizes of the call around a row; and its scratch."""
 import pytest
 import torch
 from test_kv_q8_gpu import DEV, Cache
@@ -84,4 +84,21 @@ def test_lengths_that_a_graph_changes_between_its_replays(form):
     for i in range(1, 11):
         graph.replay()
         assert torch.equal(out, call(20 + i * step, torch.zeros_like(out))), i
+    assert ops.device_error() == 0
+
+
+def test_a_workspace_of_another_device_is_refused():
+    """Before any launch, whether the call has partial results to put there or not."""
+    from types import SimpleNamespace
+
+    from dflash_b200 import ops
+    c = Cache("int8", [300], 2, 128)
+    q, pos = torch.randn(1, 4, 128).bfloat16().to(DEV), torch.full((1,), 299, dtype=torch.int32, device=DEV)
+    elsewhere = SimpleNamespace(attn=torch.empty(1 << 20, dtype=torch.uint8), ensure_attn=lambda n: None)
+    for chunk in (128, 512):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.attention_q8(q, c.kv, pos, True, 300, ws=elsewhere, form="warp", key_chunk=chunk)
+        mine = ops.Workspace(torch.device(DEV), gemm_bytes=256, attn_bytes=256)
+        a = ops.attention_q8(q, c.kv, pos, True, 300, ws=mine, form="warp", key_chunk=chunk)
+        assert torch.equal(a, ops.attention_q8(q, c.kv, pos, True, 300, form="warp", key_chunk=chunk))
     assert ops.device_error() == 0
