@@ -690,7 +690,11 @@ static int q8_run_rows(int M, int seq_rows, bool one_seq) {
 // and each costs the merge and its CTA's start: at least 128 keys, 256 where those make more than 8 chunks (one
 // token, 4096 keys: 9.2 us, with 128 11.1; 1536 keys: 8.4 and 8.0, with 16 tokens and a cold L2 18.4 and 20.5),
 // in the tcgen05 forms 512, at most 64 chunks (one kv head, 2 tokens at 48k keys: 15 us, in 190 chunks 24), and no
-// split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6).
+// split of 512 keys where half the SMs have a CTA (four sequences, 16 tokens: 11.1 us, split in two 13.6). At most
+// 8192 keys for every full wave, so that the last wave is a small part of the whole: 2048 prompt rows at 65536 keys
+// 2.82 ms (uncut 3.03), 64 sequences of 16384, 16 tokens, 0.74 (0.76); and no more chunks than that, as each
+// holds its partials in the scratch: 16384 rows at 65536 keys 19.8 ms in one, 19.7 and 2 GB in eight; 256 single
+// tokens of 512 to 16384 keys 0.76 ms, 0.80 in two.
 struct Q8Plan {
   int form, rows, key_chunk, n_chunks;  // rows: (token, head) pairs a CTA takes
 };
@@ -717,7 +721,8 @@ static Q8Plan q8_plan(int form, int key_chunk, long long runs, int run_rows, int
     long long c = n > 1 ? (max_kv + n - 1) / n : max_kv;
     if (!tc && n <= 1 && runs > 1 && max_kv >= 2048 && 20 * u <= 27 * slots)
       c = 5 * u <= 4 * slots ? (max_kv + 1) / 2 : (3LL * max_kv + 3) / 4;
-    c = c < lo ? lo : c > 8192 ? 8192 : c;
+    const long long hi = u < 2 * slots ? 8192 : u < 128 * slots ? 8192 * (u / slots) : 1 << 20;
+    c = c < lo ? lo : c > hi ? hi : c;
     key_chunk = (int)((c + Q8_CHUNK_UNIT - 1) / Q8_CHUNK_UNIT * Q8_CHUNK_UNIT);
   }
   p.key_chunk = key_chunk;

@@ -67,3 +67,16 @@ def test_generators(monkeypatch):
     with pytest.raises(ValueError, match="kv_dtype"):
         api.DFlashGenerator(target, draft, kv_dtype="int8")
     assert api.DFlashGenerator(target, draft).kv_dtype == "bf16"
+
+
+@pytest.mark.parametrize("rows,max_kv", [(1024, 131072), (4096, 32768), (4096, 131072), (16384, 65536), (16384, 131072),
+                                         (65536, 131072), (16384, 2 ** 31 - 1)])
+def test_scratch_of_long_prompts_stays_bounded(lib, rows, max_kv):
+    """The partials of a call that fills the SMs many times over: at most 8 KB a key of the longest row, whatever the rows
+    (a chunk of 8192 keys for each wave of 148 CTAs, of 256 (row, head) pairs of 128 floats and two: 19.7 MB / 8192)."""
+    import ctypes
+
+    from dflash_b200 import _lib, ops
+    desc = ops.KvQ8(n_kv_heads=8, n_seqs=1, cap=max_kv, head_dim=128)
+    need = _lib.query("dfl_attention_q8_workspace_bytes", ctypes.byref(desc), rows, 32, rows, 1, max_kv, 0, 0)
+    assert need <= 8192 * max_kv
