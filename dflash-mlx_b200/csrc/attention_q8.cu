@@ -13,8 +13,8 @@
 // on its own query and keys alone, whatever the tile's other rows, row groups or masks are: the
 // rows of a verify block and of single-token decode agree bit for bit.
 //
-// Single tokens are bound by memory: 64 sequences of 512 to 4096 keys (e4m3) 61 us, 80 % of the copy rate; 4 of up to
-// 131k keys (int8) 162 us, 88 %. Small calls are bound by latency, 8 us for one token at 1536 keys, 9.4 for 16 at
+// Single tokens are bound by memory: 64 sequences of 512 to 4096 keys (e4m3) 62 us, 80 % of the copy rate; 4 of up to
+// 131k keys (int8) 165 us, 87 %. Small calls are bound by latency, 8 us for one token at 1536 keys, 9.4 for 16 at
 // 1024: two dependent launches, and in each positions, then codes, then the strands' merge.
 //
 // Codes go to fp16 exactly (int8 by placing the biased byte into 1024 + u and subtracting 1152;

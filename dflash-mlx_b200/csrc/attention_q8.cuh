@@ -147,7 +147,7 @@ __device__ __forceinline__ Q8Tile q8_tile(const AttnQ8Args& a) {
   return t;
 }
 
-// The tcgen05 forms (attention_q8_tc.cu), tiles of 64 or 128 rows: the chunk kernel alone.
+// The tcgen05 forms (attention_q8_tc.cu), tiles of 64 rows or, wide, of 256 (head_dim 256: 128): the chunk kernel alone.
 int launch_attention_q8_tc(const AttnQ8Args& a, int hd, bool e4m3, int rows, int tiles, cudaStream_t st);
 
 }  // namespace dfl

@@ -8,7 +8,7 @@
 //    warps have work; the copies are merged at the end. Two CTAs an SM (one at head_dim 256).
 //  * wide, for prefill: a row once, and two groups of 128 rows and four softmax warps each that share the
 //    converted tiles (256 rows; at head_dim 256, where TMEM holds one group, 128). One CTA an SM. 1024 rows of
-//    32 heads of 128 at 4096 keys: 103 us, 0.58 PFLOP/s (tc: 171 us).
+//    32 heads of 128 at 4096 keys: 109 us, 0.55 PFLOP/s (tc: 175 us).
 // Per block and group:
 //   S = Q K^T      M = 128, N = 64, K = hd, both operands fp16 in shared memory
 //   w = e vs       one thread per (row, copy), 32 (wide: 64) keys each; fp16, over S's own TMEM columns, the
@@ -146,8 +146,8 @@ __global__ void __launch_bounds__((QtLayout<HD, CP, SG>::THREADS), HD == 256 || 
   const int m0 = run * a.run_rows + tile * a.tile_toks;
   const int ntok = min(min(a.tile_toks, a.run_rows - tile * a.tile_toks), a.M - m0);
   if (ntok <= 0) return;
-  // the tile's rows, two or four a lane, by every warp alike: their positions and sequences, the run's
-  // sequence (that of the first row with a position), limits
+  // the tile's rows, two, four or eight a lane (tiles of 64, 128, 256), by every warp alike: their positions and
+  // sequences, the run's sequence (that of the first row with a position), limits
   int pos2[LANE_ROWS], sq2[LANE_ROWS], seq = 0;
   bool any = false;
 #pragma unroll

@@ -69,9 +69,9 @@ int q8_cache(const dfl_kv_q8* c, const char* who, Q8Cache* out) {
 // With many rows the issue of instructions bounds it before memory does, so a lane of the rotated dims holds four
 // values of the first half and their partners of the second (the rotation needs no other lane), the arithmetic
 // runs two values an instruction, and slots of q heads alone have a loop of their own. 16384 rows of
-// 32 + 16 heads of 128, int8: 84 us, 4.4 TB/s (eight consecutive values a lane, partners by shuffle, one value an
+// 32 + 16 heads of 128, int8: 82 us, 4.5 TB/s (eight consecutive values a lane, partners by shuffle, one value an
 // instruction, one slot in flight: 135 us; the lane layout and pairs alone: 111; the ring: 97; the q loop: 80; codes
-// that are right at a half, two more instructions for four values: 84).
+// that are right at a half, two more instructions for four values: 82).
 // ---------------------------------------------------------------------------
 struct AppendQ8Args {
   const __nv_bfloat16* qkv;

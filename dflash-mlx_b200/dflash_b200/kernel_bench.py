@@ -176,7 +176,7 @@ def _quant_cache(dtype, B, Hkv, cap, hd, gen):
     codes = torch.randint(-127, 128, (2, B, Hkv, cap, hd), device="cuda", generator=gen, dtype=torch.int8)
     if dtype != torch.int8:
         codes = (codes.half() / 127).to(dtype)
-    scale = torch.rand((2, B, Hkv, cap), device="cuda", generator=gen) / 127
+    scale = (1 + torch.rand((2, B, Hkv, cap), device="cuda", generator=gen)) / 127  # rows of like magnitude
     return ops.QuantKV(codes[0], codes[1], scale[0], scale[1])
 
 

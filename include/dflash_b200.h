@@ -323,9 +323,10 @@ int dfl_attention_qkv(const void* qkv, int64_t ldqkv, const void* q_norm, const 
  * decoding with another block length, leaves every other row's codes and therefore every
  * token as they were (a scale shared by several positions would have to follow each of them).
  * No counterpart in the reference, whose KVCache holds bf16 (adapters.py:600-601).
- * Quantising a row of hd values with a = max |x|: int8 codes are rint(x * (127 / a)) with
- * scale a / 127, e4m3 codes e4m3(x * (448 / a)) (nearest even) with scale a / 448; a = 0 gives
- * scale 0; a row that holds an infinity or a NaN gets scale NaN and codes 0.
+ * Quantising a row of hd values with a = max |x|: int8 codes are rint(x * 127 / a) with
+ * scale a / 127, e4m3 codes e4m3(x * 448 / a) with scale a / 448, both to the nearest and from
+ * half-way to the even code; a below 2^-119, whose reciprocal fp32 does not hold, gives scale 0
+ * and codes 0; a row that holds an infinity or a NaN gets scale NaN and codes 0.
  * Codes are [seq][Hkv][cap][hd] bytes (or pages [page][Hkv][page_size][hd], page_table as in
  * dfl_attention_paged), scales [seq][Hkv][cap] (or [page][Hkv][page_size]) floats: a head's
  * positions follow one another without gaps, sequences (pages) and heads are strides apart;
@@ -382,7 +383,11 @@ int dfl_kv_read_q8(const dfl_kv_q8* cache, const int32_t* pos, const int32_t* ro
  * of the call but the row's own query and keys, so calls to be compared bit for bit name
  * both; DFL_Q8_AUTO and key_chunk 0 choose by the call's sizes. A row with pos >= 0 that sees no key
  * (kv_len <= 0) is zero; rows with pos < 0 are left as they are. max_kv bounds every row's
- * keys. ldo % 4 == 0, q 16-byte and out 8-byte aligned. */
+ * keys. ldo % 4 == 0, q 16-byte and out 8-byte aligned.
+ * Products of a softmax weight and its V scale are rounded to fp16 (2^-11), below 2^-14 of a row's
+ * largest to multiples of 2^-24 of that. V scales from 2^-104 to 2^90 and K scales up to 2^95 keep
+ * this; beyond them a row may lose bits or be infinite or NaN, as fp32's range ends in between.
+ * The scratch query answers 0 for one chunk of keys and for sizes that the call refuses. */
 size_t dfl_attention_q8_workspace_bytes(const dfl_kv_q8* cache, int M, int Hq, int seq_rows, int one_seq, int max_kv,
                                         int form, int key_chunk);
 int dfl_attention_q8(const void* q, const dfl_kv_q8* cache, const int32_t* pos, const int32_t* row_seq,

@@ -102,3 +102,22 @@ def test_scores_that_vanish_average_the_keys_that_a_row_sees(form, chunk, qs, sc
         # as above, with scores of 0
         tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18) * A + n * 2.0 ** -25 * v.abs().amax() / (p + 1)
         assert ((out[m] - o).abs() <= tol).all(), m
+
+
+@pytest.mark.parametrize("form,chunk", FORMS + [("warp", 1024), ("tc", 1024), ("wide", 1024)])
+@pytest.mark.parametrize("t,hd", [("int8", 128), ("e4m3", 64), ("e4m3", 256)])
+@pytest.mark.parametrize("k_to,v_to", [(2.0 ** 95, 2.0 ** 90), (2.0 ** 95, 2.0 ** -104), (2.0 ** -100, 2.0 ** 90)])
+def test_scales_at_the_ends_of_the_stated_range(form, chunk, t, hd, k_to, v_to):
+    from dflash_b200 import ops
+    n = 700
+    c, q = _case(t, n, hd, 24)
+    fk = 2.0 ** torch.floor(torch.log2(torch.tensor(k_to) / c.scale[0].max())).item()
+    lim = c.scale[1].max() if v_to > 1 else c.scale[1].min()
+    fv = 2.0 ** (torch.floor if v_to > 1 else torch.ceil)(torch.log2(torch.tensor(v_to) / lim)).item()
+    for i, f in enumerate((fk, fv)):
+        c.scale[i] *= f
+        c.val[i] *= f
+    q = (q.double() * (1 / fk)).bfloat16()  # a power of two
+    o, tol = _reference(q, c.val[0, 0, 0, :n], c.val[1, 0, 0, :n], hd ** -0.5)
+    err = (_run(c, q, n, form, chunk) - o).abs()
+    assert (err <= tol + 2.0 ** -134).all(), float((err / tol).max())  # half of bf16's smallest step
