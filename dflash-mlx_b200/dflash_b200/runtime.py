@@ -86,7 +86,9 @@ class SpecSession:
                  seed: int = 0, profile: bool = False, paged: bool = True, kv_dtype: str = "bf16"):
         """kv_dtype: "bf16", or "int8" / "e4m3" to hold the target's and the draft's K/V in 8 bits
         (half the cache memory and attention traffic; tokens then follow the rounded cache, and
-        speculative and plain decode of one kv_dtype still agree token for token).
+        speculative and plain decode of one kv_dtype and max_total still agree token for token).
+        The 8-bit attention's form and split follow batch and max_total (model.q8_split; bf16:
+        the batch alone): another max_total may round otherwise and take another token at a near tie.
 
         temperature >= 1e-5 samples (Gumbel-max on the bf16 logits, keyed by sequence and
         absolute position: the speculative decode reproduces the plain sampled decode of the
@@ -123,7 +125,8 @@ class SpecSession:
             if m is not None:
                 model_kv_dtype(m.cfg, kv_dtype)
         self.kv_dtype = kv_dtype
-        # an 8-bit cache's attention: form and keys per split of the steps and of the prefill chunks
+        # an 8-bit cache's attention: form and keys per split of the steps (of target and draft, by the target's heads)
+        # and of the prefill chunks
         self.step_split, self.prefill_split = {"key_chunk": self.key_chunk}, {"key_chunk": self.key_chunk}
         if kv_dtype != "bf16":
             form, chunk = q8_split(batch, tc.num_key_value_heads, max_total, tc.head_dim)
