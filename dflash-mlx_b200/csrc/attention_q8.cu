@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(32 * Q8_STRANDS * RG, MT == 1 && HD <= 128 ? 3
           *reinterpret_cast<float4*>(a.part_o + base * HD + d) = y;
         } else {
           const float inv = lm > 0 ? Q8_SUM_UNIT / den : 0.f;
-          float f[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+          // + 0: a zero of the sum is positive, as it is behind the merge kernel, whose sum starts at +0
+          float f[4] = {(y.x + 0.f) * inv, (y.y + 0.f) * inv, (y.z + 0.f) * inv, (y.w + 0.f) * inv};
           if (a.gate) {
             const __nv_bfloat16* gr = a.gate + (long long)m * a.ldg + (long long)head * a.gate_hs + d;
 #pragma unroll

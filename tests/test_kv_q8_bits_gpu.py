@@ -102,3 +102,24 @@ def test_a_workspace_of_another_device_is_refused():
         a = ops.attention_q8(q, c.kv, pos, True, 300, ws=mine, form="warp", key_chunk=chunk)
         assert torch.equal(a, ops.attention_q8(q, c.kv, pos, True, 300, form="warp", key_chunk=chunk))
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("form", ["warp", "tc", "wide"])
+@pytest.mark.parametrize("t,G,hd", [("int8", 4, 128), ("e4m3", 12, 256), ("int8", 16, 64)])
+def test_zeros_have_one_sign(form, t, G, hd):
+    """A softmax of one key whose values are zero in half of the dims, beside keys of negative values whose weights vanish:
+    the zeros of a call of one chunk are those of a call of several."""
+    from dflash_b200 import ops
+    lens, rows, Hkv = [700, 350, 90], 24, 2
+    c = Cache(t, lens, Hkv, hd, 64, seed=31)
+    g = torch.Generator().manual_seed(31)
+    raw = c.codes[1].view(torch.uint8)
+    neg = 0xF6 if t == "int8" else 0xB4  # -10, -0.75
+    raw.copy_(torch.where(torch.rand(raw.shape, generator=g) < 0.5, 0, neg).to(torch.uint8))
+    q = (30 * torch.randn(len(lens) * rows, Hkv * G, hd, generator=g)).bfloat16().to(DEV)
+    seq = torch.arange(len(lens), dtype=torch.int32, device=DEV).repeat_interleave(rows)
+    pos = torch.tensor([n - rows + i for n in lens for i in range(rows)], dtype=torch.int32, device=DEV)
+    one, several = [ops.attention_q8(q, c.kv, pos, True, max_kv, row_seq=seq, seq_rows=rows, form=form, key_chunk=1024)
+                    for max_kv in (1024, 1025)]
+    assert ops.device_error() == 0 and (one == 0).any()
+    assert torch.equal(one.view(torch.int16), several.view(torch.int16)), int((one.view(torch.int16) != several.view(torch.int16)).sum())
