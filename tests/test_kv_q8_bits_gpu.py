@@ -122,4 +122,5 @@ def test_zeros_have_one_sign(form, t, G, hd):
     one, several = [ops.attention_q8(q, c.kv, pos, True, max_kv, row_seq=seq, seq_rows=rows, form=form, key_chunk=1024)
                     for max_kv in (1024, 1025)]
     assert ops.device_error() == 0 and (one == 0).any()
-    assert torch.equal(one.view(torch.int16), several.view(torch.int16)), int((one.view(torch.int16) != several.view(torch.int16)).sum())
+    one, several = one.view(torch.int16), several.view(torch.int16)
+    assert torch.equal(one, several), int((one != several).sum())
